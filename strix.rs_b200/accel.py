@@ -14,6 +14,9 @@ import numpy as np
 
 ACT_F32, ACT_Q8DOT = 0, 1
 PRE_NONE, PRE_RMSNORM, PRE_SWIGLU, PRE_GEGLU = 0, 1, 2, 3
+KV_F16, KV_E4M3 = 0, 1
+ROPE_NONE, ROPE_HALVES, ROPE_ADJACENT = 0, 1, 2
+SAMPLE_MAX_N = 393216
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -43,11 +46,44 @@ class _DecodeCfg(C.Structure):
                 ("layers", C.POINTER(_LayerCfg)), ("attn_standin_q", C.c_int), ("act", C.c_int)]
 
 
+class KvPages(C.Structure):
+    """The paged KV cache of one layer (strix_kv_pages): device pointers as ints, sizes; the caller owns the memory."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("d_k_scale", C.c_void_p), ("d_v_scale", C.c_void_p), ("page_stride", C.c_size_t),
+                ("n_pages", C.c_uint32), ("n_kv", C.c_uint32), ("page_tokens", C.c_uint32), ("head_dim", C.c_uint32),
+                ("type", C.c_int), ("reserved", C.c_int)]
+
+    def __init__(self, d_k, d_v, n_pages, n_kv, page_tokens, head_dim, type=KV_F16, d_k_scale=0, d_v_scale=0, page_stride=0):
+        super().__init__(d_k or None, d_v or None, d_k_scale or None, d_v_scale or None, page_stride, n_pages, n_kv, page_tokens, head_dim,
+                         type, 0)
+
+
+class KvBatch(C.Structure):
+    """The sequences of a step (strix_kv_batch): d_row0[n_seq + 1], d_ctx[n_seq], d_pages[n_seq][pages_ld], all int32 on the device."""
+    _fields_ = [("d_row0", C.c_void_p), ("d_ctx", C.c_void_p), ("d_pages", C.c_void_p), ("n_seq", C.c_uint32), ("n_rows", C.c_uint32),
+                ("pages_ld", C.c_uint32), ("reserved", C.c_int)]
+
+    def __init__(self, n_seq, n_rows, d_row0, d_ctx, d_pages, pages_ld):
+        super().__init__(d_row0 or None, d_ctx or None, d_pages or None, n_seq, n_rows, pages_ld, 0)
+
+
+class KvPrep(C.Structure):
+    """Norms and rotation on the way into the cache (strix_kv_prep)."""
+    _fields_ = [("d_q_norm", C.c_void_p), ("d_k_norm", C.c_void_p), ("d_freq", C.c_void_p), ("theta", C.c_float), ("eps", C.c_float),
+                ("rope", C.c_int), ("norm_v", C.c_int)]
+
+    def __init__(self, rope=ROPE_HALVES, theta=1e6, d_q_norm=0, d_k_norm=0, d_freq=0, eps=1e-6, norm_v=False):
+        super().__init__(d_q_norm or None, d_k_norm or None, d_freq or None, theta, eps, rope, int(norm_v))
+
+
+class _SampleParams(C.Structure):
+    _fields_ = [("d_temperature", C.c_void_p), ("d_top_k", C.c_void_p), ("d_top_p", C.c_void_p), ("d_min_p", C.c_void_p)]
+
+
 _lib = None
 
 
 def load_library():
-    """Loads libstrix_cuda.so and declares every entry point of include/strix_cuda.h."""
+    """Loads libstrix_cuda.so and declares every entry point of include/strix_cuda.h and include/strix_serve.h."""
     global _lib
     if _lib is not None:
         return _lib
@@ -134,6 +170,14 @@ def load_library():
     sig("strix_cuda_decode_set_peers", C.c_int, H, C.c_int, C.POINTER(C.c_void_p))
     sig("strix_cuda_set_option", C.c_int, H, C.c_char_p, C.c_longlong)
     sig("strix_cuda_decode_trace", C.c_int, H, C.POINTER(C.c_uint64), sz)
+    kvp, kvb, vp = C.POINTER(KvPages), C.POINTER(KvBatch), C.c_void_p
+    sig("strix_cuda_kv_append_dev", C.c_int, H, kvp, kvb, C.POINTER(KvPrep), C.c_uint32, vp, sz, vp, sz, vp, sz, vp, sz, vp)
+    sig("strix_cuda_kv_check", C.c_int, kvp, kvb, C.c_uint32)
+    sig("strix_cuda_attn_pages_workspace", sz, H, kvp, kvb, C.c_uint32)
+    sig("strix_cuda_attn_pages_dev", C.c_int, H, kvp, kvb, C.c_uint32, vp, sz, C.c_float, C.c_uint32, vp, sz, vp, sz, vp)
+    sig("strix_cuda_sample_dev", C.c_int, H, vp, sz, sz, sz, C.POINTER(_SampleParams), vp, vp, vp, vp)
+    sig("strix_cuda_decode_step_sample", C.c_int, H, f32p, sz, C.c_float, C.c_int32, C.c_float, C.c_float, C.c_float,
+        C.POINTER(C.c_uint32), f32p)
     _lib = L
     return L
 
@@ -157,6 +201,11 @@ def _f32(a):
 
 def _fp(a):
     return a.ctypes.data_as(C.POINTER(C.c_float))
+
+
+def kv_check(cache, batch=None, n_heads=0):
+    """The argument checks of the paged-cache calls, without a handle or a device: 1 = taken, 0 = declined, -1 = an error."""
+    return int(load_library().strix_cuda_kv_check(cache, batch, n_heads))
 
 
 def fold_argmax_shards(ids, vals):
@@ -539,6 +588,44 @@ class CudaWeightAccel:
             self._h, C.c_void_p(int(d_x)), n, stride, rows, C.c_void_p(int(d_ids)) if d_ids else None,
             C.c_void_p(int(d_vals)) if d_vals else None, C.c_void_p(int(stream)) if stream else None))
         return rc == 1
+
+    # -- serving: a paged KV cache, attention over it, drawing tokens (include/strix_serve.h) ----
+    def kv_append_dev(self, cache, batch, d_k, d_v, prep, n_heads=0, d_q=0, d_q_out=0, ld_k=0, ld_v=0, ld_q=0, ld_q_out=0, stream=0):
+        """Rows of k and v into the cache, normed and rotated by `prep`; q (when given) prepared into d_q_out. False = declined."""
+        rc = self._L.strix_cuda_kv_append_dev(self._h, cache, batch, prep, n_heads, d_k or None, ld_k, d_v or None, ld_v, d_q or None, ld_q,
+                                              d_q_out or None, ld_q_out, stream or None)
+        return self._check(rc) == 1
+
+    def attn_pages_workspace(self, cache, batch, n_heads):
+        """Bytes of (once zeroed) device workspace attn_pages_dev needs for these sizes, 0 = declined."""
+        n = int(self._L.strix_cuda_attn_pages_workspace(self._h, cache, batch, n_heads))
+        if n == 0:
+            msg = self._L.strix_cuda_last_error(self._h).decode()
+            if msg:
+                raise StrixCudaError(msg)
+        return n
+
+    def attn_pages_dev(self, cache, batch, n_heads, d_q, d_out, scale, d_work, work_bytes, window=0, ld_q=0, ld_out=0, stream=0):
+        """out[row][head] = softmax(scale q k^T) v over the cached tokens each row sees. False = declined."""
+        rc = self._L.strix_cuda_attn_pages_dev(self._h, cache, batch, n_heads, d_q or None, ld_q, scale, window, d_out or None, ld_out,
+                                               d_work or None, work_bytes, stream or None)
+        return self._check(rc) == 1
+
+    def sample_dev(self, d_x, n, stride, rows, d_u, d_ids, d_probs=0, d_temperature=0, d_top_k=0, d_top_p=0, d_min_p=0, stream=0):
+        """One token per row of device logits by temperature, top-k, top-p and min-p (device arrays, 0 = neutral) at d_u in [0, 1)."""
+        p = _SampleParams(d_temperature or None, d_top_k or None, d_top_p or None, d_min_p or None)
+        rc = self._L.strix_cuda_sample_dev(self._h, d_x or None, n, stride, rows, p, d_u or None, d_ids or None, d_probs or None, stream or None)
+        return self._check(rc) == 1
+
+    def decode_step_sample(self, h, pos, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """(token id, its probability) of one decode step, drawn on the device at u in [0, 1), or None."""
+        if not getattr(self, "_vocab", None):
+            return None
+        ha = _f32(h)
+        out, prob = C.c_uint32(0), C.c_float(0.0)
+        rc = self._check(self._L.strix_cuda_decode_step_sample(self._h, _fp(ha), pos, temperature, top_k, top_p, min_p, u, C.byref(out),
+                                                               C.byref(prob)))
+        return (int(out.value), float(prob.value)) if rc == 1 else None
 
     def decode_chain_dev(self, d_h, d_logits, stream=0):
         rc = self._check(self._L.strix_cuda_decode_chain_dev(self._h, C.c_void_p(int(d_h)), C.c_void_p(int(d_logits)),

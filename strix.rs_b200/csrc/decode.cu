@@ -39,6 +39,7 @@
 #include <vector>
 
 #include "accel.h"
+#include "serve.h"
 
 using namespace strix;
 
@@ -76,6 +77,7 @@ struct strix_decode_state {
     float *h = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *gate = nullptr, *up = nullptr, *logits = nullptr;
     void *pin_h = nullptr, *pin_logits = nullptr;
     cudaGraphExec_t exec = nullptr;
+    uint32_t *smp = nullptr, *smp_pin = nullptr;  // decode_step_sample: parameters, then the token and its probability
     // real attention (attn_standin_q = 0): KV cache (per layer [max_seq][n_kv * hd] for k and for v, f32 or f16,
     // one allocation), the softmax partials, the attention output, and the position word the kernels read (a graph
     // replays unchanged)
@@ -127,6 +129,8 @@ static void decode_free(strix_decode_state *d) {
     if (d->r_pos) cudaFree(d->r_pos);
     if (d->r_pin_in) cudaFreeHost(d->r_pin_in);
     if (d->r_pin_out) cudaFreeHost(d->r_pin_out);
+    if (d->smp) cudaFree(d->smp);
+    if (d->smp_pin) cudaFreeHost(d->smp_pin);
     if (d->d_pos) cudaFree(d->d_pos);
     if (d->pin_pos) cudaFreeHost(d->pin_pos);
     if (d->pin_h) cudaFreeHost(d->pin_h);
@@ -958,6 +962,37 @@ int strix_cuda_decode_step_argmax(strix_cuda *h, const float *hvec, size_t pos, 
     CU_TRY(h, cudaMemcpyAsync(h->am_pin, h->am_idx, 4, cudaMemcpyDeviceToHost, h->stream));
     if ((rc = decode_finish(h, "decode_step_argmax")) < 0) return rc;
     *id = h->am_pin[0];
+    return 1;
+}
+
+// The same with a draw in place of the argmax (sample.cu). The parameters and the number go to the device as one small copy;
+// the token and its probability come back.
+int strix_cuda_decode_step_sample(strix_cuda *h, const float *hvec, size_t pos, float temperature, int32_t top_k, float top_p,
+                                  float min_p, float u, uint32_t *id, float *prob) {
+    if (!h || !hvec || !id) return -1;
+    h->err.clear();
+    strix_decode_state *d = h->decode;
+    if (!d || h->world > 1 || d->cfg.vocab > STRIX_SAMPLE_MAX_N) return 0;
+    CU_TRY(h, cudaSetDevice(h->device));
+    if (!d->smp) CU_TRY(h, cudaMalloc(&d->smp, 8 * 4));
+    if (!d->smp_pin) CU_TRY(h, cudaMallocHost(&d->smp_pin, 8 * 4));
+    int rc = decode_enqueue_step(h, d, hvec, pos);
+    if (rc < 0) return rc;
+    // words: temperature, top_k, top_p, min_p, u | id, probability
+    memcpy(d->smp_pin + 0, &temperature, 4);
+    memcpy(d->smp_pin + 1, &top_k, 4);
+    memcpy(d->smp_pin + 2, &top_p, 4);
+    memcpy(d->smp_pin + 3, &min_p, 4);
+    memcpy(d->smp_pin + 4, &u, 4);
+    CU_TRY(h, cudaMemcpyAsync(d->smp, d->smp_pin, 5 * 4, cudaMemcpyHostToDevice, h->stream));
+    if (d->cfg.final_softcap > 0.f) CU_TRY(h, launch_softcap(d->logits, d->cfg.vocab, d->cfg.final_softcap, h->stream));
+    const float *f = reinterpret_cast<const float *>(d->smp);
+    const strix_sample_params p{f, reinterpret_cast<const int32_t *>(d->smp + 1), f + 2, f + 3};
+    CU_TRY(h, launch_sample(h, d->logits, d->cfg.vocab, d->cfg.vocab, 1, p, f + 4, d->smp + 5, reinterpret_cast<float *>(d->smp + 6), h->stream));
+    CU_TRY(h, cudaMemcpyAsync(d->smp_pin + 5, d->smp + 5, 2 * 4, cudaMemcpyDeviceToHost, h->stream));
+    if ((rc = decode_finish(h, "decode_step_sample")) < 0) return rc;
+    *id = d->smp_pin[5];
+    if (prob) memcpy(prob, d->smp_pin + 6, 4);
     return 1;
 }
 

@@ -17,7 +17,9 @@ BASE = {"void": "c_void", "char": "c_char", "int": "c_int", "float": "f32", "siz
         "int8_t": "i8", "uint32_t": "u32", "int32_t": "i32", "uint64_t": "u64", "long long": "c_longlong",
         "unsigned long long": "u64", "strix_cuda": "StrixCuda", "strix_cuda_opts": "StrixCudaOpts",
         "strix_gpu_decode_config": "StrixGpuDecodeConfig", "strix_gguf": "StrixGguf",
-        "strix_gguf_tensor": "StrixGgufTensor", "strix_spec_gate": "StrixSpecGate", "strix_embed_fn": "StrixEmbedFn"}
+        "strix_gguf_tensor": "StrixGgufTensor", "strix_spec_gate": "StrixSpecGate", "strix_embed_fn": "StrixEmbedFn",
+        "strix_kv_pages": "StrixKvPages", "strix_kv_batch": "StrixKvBatch", "strix_kv_prep": "StrixKvPrep",
+        "strix_sample_params": "StrixSampleParams"}
 
 
 def rust_type(c):
@@ -110,6 +112,37 @@ pub struct StrixGgufTensor {
 #[repr(C)]
 #[derive(Default, Clone, Copy)]
 pub struct StrixSpecGate { pub zero_rounds: u32, pub plain_left: u32 }
+
+/// strix_kv_pages: the paged KV cache of one layer
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct StrixKvPages {
+    pub k: *mut c_void, pub v: *mut c_void, pub d_k_scale: *mut f32, pub d_v_scale: *mut f32, pub page_stride: usize,
+    pub n_pages: u32, pub n_kv: u32, pub page_tokens: u32, pub head_dim: u32, pub type_: c_int, pub reserved: c_int,
+}
+
+/// strix_kv_batch: the sequences of a step
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct StrixKvBatch {
+    pub d_row0: *const i32, pub d_ctx: *const i32, pub d_pages: *const i32,
+    pub n_seq: u32, pub n_rows: u32, pub pages_ld: u32, pub reserved: c_int,
+}
+
+/// strix_kv_prep: norm and rotation on the way into the cache
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct StrixKvPrep {
+    pub d_q_norm: *const f32, pub d_k_norm: *const f32, pub d_freq: *const f32, pub theta: f32, pub eps: f32,
+    pub rope: c_int, pub norm_v: c_int,
+}
+
+/// strix_sample_params
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct StrixSampleParams {
+    pub d_temperature: *const f32, pub d_top_k: *const i32, pub d_top_p: *const f32, pub d_min_p: *const f32,
+}
 
 pub type StrixEmbedFn = Option<unsafe extern "C" fn(user: *mut c_void, token: u32, hidden_out: *mut f32)>;
 

@@ -48,6 +48,37 @@ pub struct StrixGgufTensor {
 #[derive(Default, Clone, Copy)]
 pub struct StrixSpecGate { pub zero_rounds: u32, pub plain_left: u32 }
 
+/// strix_kv_pages: the paged KV cache of one layer
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct StrixKvPages {
+    pub k: *mut c_void, pub v: *mut c_void, pub d_k_scale: *mut f32, pub d_v_scale: *mut f32, pub page_stride: usize,
+    pub n_pages: u32, pub n_kv: u32, pub page_tokens: u32, pub head_dim: u32, pub type_: c_int, pub reserved: c_int,
+}
+
+/// strix_kv_batch: the sequences of a step
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct StrixKvBatch {
+    pub d_row0: *const i32, pub d_ctx: *const i32, pub d_pages: *const i32,
+    pub n_seq: u32, pub n_rows: u32, pub pages_ld: u32, pub reserved: c_int,
+}
+
+/// strix_kv_prep: norm and rotation on the way into the cache
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct StrixKvPrep {
+    pub d_q_norm: *const f32, pub d_k_norm: *const f32, pub d_freq: *const f32, pub theta: f32, pub eps: f32,
+    pub rope: c_int, pub norm_v: c_int,
+}
+
+/// strix_sample_params
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct StrixSampleParams {
+    pub d_temperature: *const f32, pub d_top_k: *const i32, pub d_top_p: *const f32, pub d_min_p: *const f32,
+}
+
 pub type StrixEmbedFn = Option<unsafe extern "C" fn(user: *mut c_void, token: u32, hidden_out: *mut f32)>;
 
 pub const ACT_F32: c_int = 0;
@@ -148,6 +179,13 @@ extern "C" {
     pub fn strix_ggml_block_bytes(ggml_type: u32) -> usize;
     pub fn strix_cuda_upload_gguf_tensor(h: *mut StrixCuda, g: *const StrixGguf, name: *const c_char, drop_pages: c_int) -> c_int;
     pub fn strix_cuda_upload_gguf(h: *mut StrixCuda, g: *const StrixGguf, drop_pages: c_int, adopted: *mut usize, declined: *mut usize) -> c_int;
+    // ---- include/strix_serve.h
+    pub fn strix_cuda_kv_check(cache: *const StrixKvPages, batch: *const StrixKvBatch, n_heads: u32) -> c_int;
+    pub fn strix_cuda_kv_append_dev(h: *mut StrixCuda, cache: *const StrixKvPages, batch: *const StrixKvBatch, prep: *const StrixKvPrep, n_heads: u32, d_k: *const f32, ld_k: usize, d_v: *const f32, ld_v: usize, d_q: *const f32, ld_q: usize, d_q_out: *mut f32, ld_q_out: usize, stream: *mut c_void) -> c_int;
+    pub fn strix_cuda_attn_pages_workspace(h: *mut StrixCuda, cache: *const StrixKvPages, batch: *const StrixKvBatch, n_heads: u32) -> usize;
+    pub fn strix_cuda_attn_pages_dev(h: *mut StrixCuda, cache: *const StrixKvPages, batch: *const StrixKvBatch, n_heads: u32, d_q: *const f32, ld_q: usize, scale: f32, window: u32, d_out: *mut f32, ld_out: usize, d_work: *mut c_void, work_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn strix_cuda_sample_dev(h: *mut StrixCuda, d_x: *const f32, n: usize, stride: usize, rows: usize, params: *const StrixSampleParams, d_u: *const f32, d_ids: *mut u32, d_probs: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn strix_cuda_decode_step_sample(h: *mut StrixCuda, hvec: *const f32, pos: usize, temperature: f32, top_k: i32, top_p: f32, min_p: f32, u: f32, id: *mut u32, prob: *mut f32) -> c_int;
     // ---- include/strix_spec.h
     pub fn strix_spec_propose_ngram(ctx: *const u32, n_ctx: usize, gamma: usize, out: *mut u32) -> usize;
     pub fn strix_spec_accept(proposal: *const u32, n_prop: usize, argmax: *const u32, room: usize, next: *mut u32) -> usize;

@@ -1,0 +1,509 @@
+"""The paged KV cache (append, attention) and sampling on the GPU against their definitions in 64 bits."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+import serve_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+def _i32(torch, v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+class Paged:
+    """A cache on the device with its page table, and what a test knows about it."""
+
+    def __init__(self, torch, pkg, kv, n_kv, page, hd, tokens, seed=0, pad=0, spare=2, fill=None):
+        """tokens: cached capacity of each sequence; pad: extra elements between pages; fill: byte the buffers start with."""
+        self.torch, self.pkg, self.kv, self.n_kv, self.page, self.hd = torch, pkg, kv, n_kv, page, hd
+        rng = np.random.RandomState(seed)
+        need = [-(-t // page) for t in tokens]
+        self.n_pages, self.ld = sum(need) + spare, max(need + [1])
+        ids = rng.permutation(self.n_pages)
+        self.table = np.full((len(tokens), self.ld), -7, np.int32)     # unused entries are no pages
+        at = 0
+        for i, n in enumerate(need):
+            self.table[i, :n] = ids[at:at + n]
+            at += n
+        self.stride = n_kv * page * hd + pad
+        el = 2 if kv == pkg.KV_F16 else 1
+        n = self.n_pages * self.stride * el
+        self.raw = {m: torch.full((n,), 0x7e if fill is None else fill, dtype=torch.uint8, device="cuda") for m in "kv"}
+        self.scale = {m: torch.full((self.n_pages, n_kv), 1.0, device="cuda") for m in "kv"}
+        self.d_table = torch.from_numpy(self.table).cuda()
+        self.desc = pkg.KvPages(self.raw["k"].data_ptr(), self.raw["v"].data_ptr(), self.n_pages, n_kv, page, hd, type=kv,
+                                d_k_scale=self.scale["k"].data_ptr(), d_v_scale=self.scale["v"].data_ptr(), page_stride=self.stride if pad else 0)
+
+    def values(self, m):
+        """float64 [n_pages, n_kv, page, hd]"""
+        raw = self.raw[m].cpu().numpy()
+        x = raw.view(np.float16) if self.kv == self.pkg.KV_F16 else raw
+        x = x.reshape(self.n_pages, self.stride)[:, :self.n_kv * self.page * self.hd].reshape(self.n_pages, self.n_kv, self.page, self.hd)
+        if self.kv == self.pkg.KV_F16:
+            return x.astype(np.float64)
+        return so.e4m3_value(x) * self.scale[m].cpu().numpy().astype(np.float64)[:, :, None, None]
+
+    def tokens(self, m, s, n):
+        """float64 [n, n_kv, hd]: the first n cached tokens of sequence s; unused or bad pages as zeros."""
+        v, out = self.values(m), np.zeros((n, self.n_kv, self.hd))
+        for t in range(n):
+            j = t // self.page
+            pg = self.table[s, j] if j < self.ld else -1
+            if 0 <= pg < self.n_pages:
+                out[t] = v[pg, :, t % self.page]
+        return out
+
+    def batch(self, row0, ctx, n_rows=None):
+        self.row0, self.ctx = _i32(self.torch, row0), _i32(self.torch, ctx)
+        return self.pkg.KvBatch(len(ctx), row0[-1] if n_rows is None else n_rows, self.row0.data_ptr(), self.ctx.data_ptr(),
+                                self.d_table.data_ptr(), self.ld)
+
+    def seed_random(self, seed, lengths):
+        """The first lengths[s] tokens of every sequence as a user might have written them: finite values, scales any power of two.
+        Everything else keeps the bytes it has."""
+        rng = np.random.RandomState(seed)
+        for m in "kv":
+            raw = self.raw[m].cpu().numpy().copy()
+            sc = np.exp2(rng.randint(-9, -4, (self.n_pages, self.n_kv))).astype(np.float32)
+            for s, n in enumerate(lengths):
+                for t in range(n):
+                    pg = self.table[s, t // self.page]
+                    for h in range(self.n_kv):
+                        o = pg * self.stride + (h * self.page + t % self.page) * self.hd
+                        x = rng.randn(self.hd)
+                        if self.kv == self.pkg.KV_F16:
+                            raw.view(np.float16)[o:o + self.hd] = x
+                        else:
+                            code = rng.randint(0, 127, self.hd) | (rng.randint(0, 2, self.hd) << 7)
+                            raw[o:o + self.hd] = np.where((code & 127) > 0x68, code & 0xe7, code)
+            self.raw[m].copy_(self.torch.from_numpy(raw))
+            self.scale[m].copy_(self.torch.from_numpy(sc))
+
+
+def work_of(torch, accel, P, b, heads):
+    n = accel.attn_pages_workspace(P.desc, b, heads)
+    assert n > 0
+    return torch.zeros(n, dtype=torch.uint8, device="cuda")
+
+
+def stream(torch):
+    return torch.cuda.current_stream().cuda_stream
+
+
+# ---------------------------------------------------------------- append
+
+def half_step(kv, pkg, x, s):
+    """How far a stored value may be from x: half a step of its type there, and the f32 arithmetic that made it (norm,
+    rotation: a dozen roundings of 2^-24 of the largest value of the head)."""
+    a = np.abs(x)
+    if kv == pkg.KV_F16:
+        return np.maximum(a * 2.0 ** -11, 2.0 ** -25)
+    return np.maximum(a * 2.0 ** -4, s * 2.0 ** -10)
+
+
+@pytest.mark.parametrize("hd,page", [(64, 16), (96, 32), (128, 64), (192, 128), (256, 16), (128, 128)])
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("rope,norm", [(1, True), (2, False), (0, True)])
+def test_append_many_sequences(torch, pkg, accel, kv, hd, page, rope, norm):
+    """Ragged new rows, an idle slot, an empty sequence, rows of nobody, strided inputs, frequency factors, padded pages."""
+    n_kv, heads = 2, 6
+    new = [1, 0, 5, 2 * page + 3, 1, 1]
+    ctx = [0, 4, page - 2, 3, -1, 2 * page]
+    row0 = np.cumsum([0] + new).tolist()
+    rows, all_rows = row0[-1], row0[-1] + 2
+    P = Paged(torch, pkg, kv, n_kv, page, hd, [c + n if c >= 0 else 0 for c, n in zip(ctx, new)], seed=hd + page, pad=32)
+    P.seed_random(5, [max(c, 0) for c in ctx])
+    before = {m: P.raw[m].clone() for m in "kv"}
+    old = {m: P.values(m) for m in "kv"}
+    old_scale = {m: P.scale[m].cpu().numpy().copy() for m in "kv"}
+    b = P.batch(row0, ctx, all_rows)
+    g = torch.Generator(device="cuda").manual_seed(hd + 7 * rope)
+    fused = torch.randn(all_rows, (heads + 2 * n_kv) * hd + 4, generator=g, device="cuda") * 3.0   # q | k | v slices of one buffer
+    q, k, v = fused[:, :heads * hd], fused[:, heads * hd:(heads + n_kv) * hd], fused[:, (heads + n_kv) * hd:(heads + 2 * n_kv) * hd]
+    qn, kn = (1 + 0.1 * torch.randn(hd, generator=g, device="cuda") for _ in range(2))
+    freq = 1 + torch.rand(hd // 2, generator=g, device="cuda") * 7
+    out = torch.full((all_rows, heads * hd + 8), 7.0, device="cuda")
+    prep = pkg.KvPrep(rope=rope, theta=5e5, eps=1e-5, norm_v=norm, d_freq=freq.data_ptr(), d_q_norm=qn.data_ptr() if norm else 0,
+                      d_k_norm=kn.data_ptr() if norm else 0)
+    ld = fused.shape[1]
+    assert accel.kv_append_dev(P.desc, b, k.data_ptr(), v.data_ptr(), prep, n_heads=heads, d_q=q.data_ptr(), d_q_out=out.data_ptr(),
+                               ld_k=ld, ld_v=ld, ld_q=ld, ld_q_out=out.shape[1], stream=stream(torch))
+    torch.cuda.synchronize()
+    assert accel.device_status() == 0
+    got = {m: P.values(m) for m in "kv"}
+    gq = out.cpu().numpy().astype(np.float64)
+    hq, hk, hv = (t.cpu().numpy() for t in (q, k, v))
+    wq, wk = (t.cpu().numpy() if norm else None for t in (qn, kn))
+    fr = freq.cpu().numpy()
+    touched = {}
+    for s, (n, c) in enumerate(zip(new, ctx)):
+        for i in range(n):
+            r = row0[s] + i
+            if c < 0:
+                assert (gq[r] == 7.0).all()
+                continue
+            pos = c + i
+            want = so.prepared(hq[r].reshape(heads, hd), wq, pos, rope, 5e5, 1e-5, fr, norm)
+            tol = 16 * 2.0 ** -24 * np.abs(want).max()
+            assert np.abs(gq[r, :heads * hd].reshape(heads, hd) - want).max() <= tol
+            pg, slot = P.table[s, pos // page], pos % page
+            wk_ = so.prepared(hk[r].reshape(n_kv, hd), wk, pos, rope, 5e5, 1e-5, fr, norm)
+            wv_ = so.prepared(hv[r].reshape(n_kv, hd), None, pos, 0, 1.0, 1e-5, None, norm)
+            t = touched.setdefault(pg, dict(first=slot, slots={}))
+            t["slots"][slot] = dict(k=wk_, v=wv_)
+    assert (gq[:, heads * hd:] == 7.0).all() and (gq[rows:] == 7.0).all()
+    for pg, t in touched.items():
+        for m in "kv":
+            for h in range(n_kv):
+                s_now = float(P.scale[m][pg, h])
+                if kv == pkg.KV_E4M3:
+                    amax = max(np.abs(x[m][h]).max() for x in t["slots"].values())
+                    want_s = max(so.scale_for(amax), float(old_scale[m][pg, h]) if t["first"] else 0.0)
+                    assert s_now == want_s
+                for slot, x in t["slots"].items():
+                    w = x[m][h]
+                    assert (np.abs(got[m][pg, h, slot] - w) <= half_step(kv, pkg, w, s_now) + 16 * 2.0 ** -24 * np.abs(w).max()).all()
+                for slot in range(t["first"]):       # earlier tokens: moved to the new scale, at most half a (subnormal) step lost
+                    w = old[m][pg, h, slot]
+                    assert (np.abs(got[m][pg, h, slot] - w) <= (s_now * 2.0 ** -10 if kv else 0.0)).all()
+    # bytes that no token owns keep their values: other pages whole, the padding between pages, slots behind the last token
+    el = 2 if kv == pkg.KV_F16 else 1
+    for m in "kv":
+        a, z = (x.cpu().numpy().reshape(P.n_pages, P.stride * el) for x in (before[m], P.raw[m]))
+        own = n_kv * page * hd * el
+        assert (a[:, own:] == z[:, own:]).all()
+        for pg in range(P.n_pages):
+            if pg not in touched:
+                assert (a[pg] == z[pg]).all()
+                continue
+            last = max(touched[pg]["slots"]) + 1
+            x, y = (u[pg, :own].reshape(n_kv, page, hd * el)[:, last:] for u in (a, z))
+            assert (x == y).all()
+
+
+def test_append_token_by_token_grows_the_scale(torch, pkg, accel):
+    """Values that double again and again: every code moves down with the scale and stays within one rounding of each growth."""
+    hd, page, n_kv = 64, 16, 1
+    P = Paged(torch, pkg, pkg.KV_E4M3, n_kv, page, hd, [40])
+    rng = np.random.RandomState(3)
+    rows = (rng.randn(40, hd) * np.exp2(rng.randint(-6, 7, 40))[:, None]).astype(np.float32)
+    prep = pkg.KvPrep(rope=pkg.ROPE_NONE)
+    for t in range(40):
+        x = torch.from_numpy(rows[t:t + 1]).cuda()
+        b = P.batch([0, 1], [t])
+        assert accel.kv_append_dev(P.desc, b, x.data_ptr(), x.data_ptr(), prep, stream=stream(torch))
+        torch.cuda.synchronize()
+    got, sc = P.tokens("k", 0, 40)[:, 0], P.scale["k"].cpu().numpy()
+    for t in range(40):
+        j = t // page
+        first, last = j * page, min(40, (j + 1) * page)
+        s = float(sc[P.table[0, j], 0])
+        assert s == so.scale_for(np.abs(rows[first:last]).max())
+        # one rounding when it came (2^-4 of the value or 2^-10 of the scale then), and less than one subnormal half step,
+        # 2^-10 of the final scale, for all later moves together with the first: 1 + 1/2 + 1/4 + ...
+        assert (np.abs(got[t] - rows[t]) <= np.abs(rows[t]) * 2.0 ** -4 + 2 * s * 2.0 ** -10).all()
+    assert (P.values("k") == P.values("v")).all()
+
+
+def test_append_special_values_and_recycled_pages(torch, pkg, accel):
+    """Zeros, NaN, infinities; a page that starts anew forgets its old scale."""
+    for kv in (pkg.KV_F16, pkg.KV_E4M3):
+        P = Paged(torch, pkg, kv, 1, 16, 64, [16])
+        P.scale["k"].fill_(64.0)
+        P.scale["v"].fill_(64.0)
+        z = torch.zeros(1, 64, device="cuda")
+        prep = pkg.KvPrep(rope=pkg.ROPE_NONE)
+        assert accel.kv_append_dev(P.desc, P.batch([0, 1], [0]), z.data_ptr(), z.data_ptr(), prep, stream=stream(torch))
+        torch.cuda.synchronize()
+        assert (P.tokens("k", 0, 1) == 0).all()
+        if kv == pkg.KV_E4M3:
+            assert float(P.scale["k"][P.table[0, 0], 0]) == 2.0 ** -120
+        x = torch.randn(1, 64, device="cuda")
+        x[0, 3], x[0, 5], x[0, 7] = float("nan"), float("inf"), -float("inf")
+        assert accel.kv_append_dev(P.desc, P.batch([0, 1], [1]), x.data_ptr(), z.data_ptr(), prep, stream=stream(torch))
+        torch.cuda.synchronize()
+        got = P.tokens("k", 0, 2)[1, 0]
+        assert np.isfinite(got).all() and got[3] == 0
+        most = 65504.0 if kv == pkg.KV_F16 else 3.0e38
+        assert abs(got[5] - most) <= most * 2.0 ** -4 and got[7] == -got[5]
+
+
+def test_append_bad_device_data_is_skipped(torch, pkg, accel):
+    """Page ids out of range, positions beyond the table, offsets out of range or descending: the good part is stored, the
+    status bit is set, nothing else changes."""
+    hd, page = 64, 16
+    P = Paged(torch, pkg, pkg.KV_F16, 1, page, hd, [32, 32, 32], fill=0)
+    P.table[1, 0] = P.n_pages            # out of range
+    P.table[2, 1] = -1
+    P.d_table.copy_(torch.from_numpy(P.table))
+    prep = pkg.KvPrep(rope=pkg.ROPE_HALVES)
+    x = torch.ones(60, hd, device="cuda")
+    q = torch.zeros(60, hd, device="cuda")
+    for row0, ctx, good in (([0, 3, 6, 26], [30, 0, 0], {0: [30, 31], 1: [], 2: list(range(16))}),
+                            ([0, 2, 1 << 30, 5], [0, 16, 0], {0: [0, 1], 1: list(range(16, 32)), 2: []})):
+        for m in "kv":
+            P.raw[m].zero_()
+        b = P.batch(row0, ctx, 60)
+        assert accel.kv_append_dev(P.desc, b, x.data_ptr(), x.data_ptr(), prep, n_heads=1, d_q=x.data_ptr(), d_q_out=q.data_ptr(), stream=stream(torch))
+        torch.cuda.synchronize()
+        assert accel.device_status() & 2
+        accel.clear_device_status()
+        v = P.values("v")
+        want = np.zeros_like(v)
+        for s, ts in good.items():
+            for t in ts:
+                if 0 <= P.table[s, t // page] < P.n_pages:
+                    want[P.table[s, t // page], 0, t % page] = 1.0
+        assert (v == want).all()
+
+
+# ---------------------------------------------------------------- attention
+
+def check_attention(torch, accel, P, b, row0, ctx, heads, q, out, scale, window, hole=None, strict=1.0):
+    """Every row against 64 bits. The bound: a score is a sum of hd products of f32 accuracy, so it is off by at most
+    (hd + 8) 2^-24 of the sum of their magnitudes (times `strict` <= 1), a probability by twice that relatively, and the sum over v
+    adds as many roundings as it has terms, at most 2^-24 each of the largest magnitude; plus 2^-20 for exp and the joins."""
+    hq, ho = q.cpu().numpy().reshape(q.shape[0], heads, P.hd), out.cpu().numpy().reshape(q.shape[0], heads, P.hd)
+    cap = P.ld * P.page
+    for s, c in enumerate(ctx):
+        rows = range(row0[s], row0[s + 1])
+        if c < 0:
+            assert all((ho[r] == 0).all() for r in rows)
+            continue
+        n = min(c + len(rows), cap)
+        k, v = P.tokens("k", s, n), P.tokens("v", s, n)
+        for i, r in enumerate(rows):
+            h = None if hole is None else hole[s][:n]
+            want = so.attend(hq[r], k, v, c + i, scale, window, h)
+            g = heads // P.n_kv
+            for hh in range(heads):
+                mag = np.abs(k[:, hh // g]) @ np.abs(hq[r, hh].astype(np.float64)) * scale
+                d = 2 * (P.hd + 8) * 2.0 ** -24 * (mag.max() if n else 0.0) * strict + 2.0 ** -20
+                top = np.abs(v[:, hh // g]).max() if n else 0.0
+                err = np.abs(ho[r, hh] - want[hh]).max()
+                assert err <= d * top, (s, i, hh, err, d * top)
+
+
+def run_attention(torch, pkg, accel, kv, n_kv, group, page, hd, new, ctx, window=0, seed=1, pad=0, extra=1, qs=1.0, fill=None, ldpad=0):
+    heads = n_kv * group
+    row0 = np.cumsum([0] + new).tolist()
+    P = Paged(torch, pkg, kv, n_kv, page, hd, [c + n if c >= 0 else 0 for c, n in zip(ctx, new)], seed=seed, pad=pad, fill=fill)
+    P.seed_random(seed, [c + n if c >= 0 else 0 for c, n in zip(ctx, new)])
+    b = P.batch(row0, ctx, row0[-1] + extra)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randn(row0[-1] + extra, heads * hd + ldpad, generator=g, device="cuda") * qs
+    out = torch.full((row0[-1] + extra, heads * hd + ldpad), 5.0, device="cuda")
+    w = work_of(torch, accel, P, b, heads)
+    scale = 1.0 / math.sqrt(hd)
+    for _ in range(2):      # twice: the workspace is ready for the next call
+        out.fill_(5.0)
+        assert accel.attn_pages_dev(P.desc, b, heads, q.data_ptr(), out.data_ptr(), scale, w.data_ptr(), w.numel(), window=window,
+                                    ld_q=q.shape[1] if ldpad else 0, ld_out=q.shape[1] if ldpad else 0, stream=stream(torch))
+        torch.cuda.synchronize()
+        assert accel.device_status() == 0
+        assert (out[row0[-1]:] == 5.0).all() and (out[:, heads * hd:] == 5.0).all()
+        check_attention(torch, accel, P, b, row0, ctx, heads, q[:, :heads * hd].contiguous(), out[:, :heads * hd].contiguous(), scale, window)
+    return P, b, row0, q, out, w
+
+
+@pytest.mark.parametrize("hd,page", [(64, 16), (64, 128), (96, 32), (128, 64), (128, 16), (192, 128), (256, 16), (256, 64)])
+@pytest.mark.parametrize("kv", [0, 1])
+def test_attention_single_tokens(torch, pkg, accel, kv, hd, page):
+    """One new row a sequence, contexts of every ending, an idle slot, a sequence without rows, garbage (NaN codes) behind the end."""
+    ctx = [0, 1, 14, 15, 16, 31, page - 1, page, 2 * page + 1, -1, 5, 300]
+    new = [1] * 10 + [0, 1]
+    run_attention(torch, pkg, accel, kv, 2, 4, page, hd, new, ctx, fill=0xff)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 7, 8, 9, 16, 17])
+@pytest.mark.parametrize("kv", [0, 1])
+def test_attention_head_groups(torch, pkg, accel, kv, group):
+    run_attention(torch, pkg, accel, kv, 3, group, 32, 64, [1, 2, 1], [100, 33, 0], pad=16, ldpad=4)
+
+
+@pytest.mark.parametrize("window", [0, 1, 5, 16, 40, 100])
+@pytest.mark.parametrize("kv,hd,page,group", [(0, 64, 16, 2), (1, 128, 64, 4), (0, 256, 32, 1), (1, 96, 16, 3)])
+def test_attention_several_rows_and_windows(torch, pkg, accel, kv, hd, page, group, window):
+    run_attention(torch, pkg, accel, kv, 2, group, page, hd, [5, 1, 33, 8, 2], [0, 70, 3, 200, -1], window=window)
+
+
+@pytest.mark.parametrize("kv,hd,group,rows", [(1, 128, 4, 150), (0, 64, 8, 70), (1, 256, 2, 40), (0, 96, 1, 300)])
+def test_attention_prompt_chunks(torch, pkg, accel, kv, hd, group, rows):
+    run_attention(torch, pkg, accel, kv, 1, group, 64, hd, [rows, 1, rows // 3], [0, 64, 129])
+
+
+def test_attention_long_contexts_split_and_joined(torch, pkg, accel):
+    run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 4, 128, 64, [1, 1], [5000, 17])
+    run_attention(torch, pkg, accel, pkg.KV_F16, 2, 1, 16, 64, [3], [3001])
+
+
+def test_attention_extreme_scores(torch, pkg, accel):
+    """Scores of thousands: one token has all the weight; and all scores equal."""
+    run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 4, 16, 64, [1, 2], [90, 200], qs=500.0)
+    run_attention(torch, pkg, accel, pkg.KV_F16, 1, 4, 16, 64, [1, 2], [90, 200], qs=0.0)
+
+
+def test_attention_scales_of_pages_far_apart(torch, pkg, accel):
+    """Pages whose scales differ by 2^30: no page overflows or hides another."""
+    P, b, row0, q, out, w = run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 2, 16, 64, [1], [100])
+    for m, lo, hi in (("v", -15, 15), ("k", -20, -3)):
+        P.scale[m].copy_(torch.exp2(torch.linspace(lo, hi, P.n_pages, device="cuda").round())[:, None])
+    assert accel.attn_pages_dev(P.desc, b, 2, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+    torch.cuda.synchronize()
+    check_attention(torch, accel, P, b, row0, [100], 2, q, out, 0.125, 0)
+
+
+def test_attention_nan_query_stays_in_its_row(torch, pkg, accel):
+    for new in ([1, 1], [3, 20]):
+        P, b, row0, q, out, w = run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 2, 16, 64, new, [40, 50])
+        good = out.clone()
+        q[1, 0] = float("nan")         # row 1, head 0
+        assert accel.attn_pages_dev(P.desc, b, 2, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        assert torch.isnan(out[1, :64]).all()
+        out[1, :64] = good[1, :64]
+        assert torch.equal(out, good)
+
+
+def test_attention_bad_device_data_is_masked(torch, pkg, accel):
+    """A bad page id hides its tokens; a length beyond the table ends there; a row that then sees nothing gets zeros."""
+    page, hd = 16, 64
+    for kv in (pkg.KV_F16, pkg.KV_E4M3):
+        P = Paged(torch, pkg, kv, 1, page, hd, [64, 16, 48])
+        P.seed_random(3, [64, 16, 48])
+        P.table[0, 1], P.table[1, 0] = P.n_pages, -5
+        P.d_table.copy_(torch.from_numpy(P.table))
+        row0, ctx = [0, 1, 2, 4], [60, 10, 46]
+        hole = [np.repeat((P.table[s] < 0) | (P.table[s] >= P.n_pages), page) for s in range(3)]
+        b = P.batch(row0, ctx, 6)
+        q = torch.randn(6, 2 * hd, device="cuda")
+        out = torch.full_like(q, 5.0)
+        w = work_of(torch, accel, P, b, 2)
+        assert accel.attn_pages_dev(P.desc, b, 2, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        assert accel.device_status() & 2
+        accel.clear_device_status()
+        assert (out[1] == 0).all() and (out[4:] == 5.0).all()
+        check_attention(torch, accel, P, b, row0, ctx, 2, q, out, 0.125, 0, hole=hole)
+        # beyond the table: 64 tokens of capacity, the row claims position 1000
+        P.table[0, 1] = P.table[2, 0]
+        P.d_table.copy_(torch.from_numpy(P.table))
+        b = P.batch([0, 1], [1000], 1)
+        assert accel.attn_pages_dev(P.desc, b, 2, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        assert accel.device_status() & 2
+        accel.clear_device_status()
+        check_attention(torch, accel, P, b, [0, 1], [1000], 2, q[:1], out[:1], 0.125, 0)
+
+
+# ---------------------------------------------------------------- sampling
+
+def sample(torch, accel, x, u, temperature=None, top_k=None, top_p=None, min_p=None, stride=None):
+    rows, n = x.shape
+    stride = stride or n
+    buf = torch.full((rows, stride), 9.0e9, device="cuda")
+    buf[:, :n] = torch.from_numpy(x).cuda()
+    f = lambda a, t: None if a is None else torch.tensor(np.asarray(a), dtype=t, device="cuda")  # noqa: E731
+    T, K, TP, MP, U = f(temperature, torch.float32), f(top_k, torch.int32), f(top_p, torch.float32), f(min_p, torch.float32), f(u, torch.float32)
+    ids = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    probs = torch.full((rows,), -1.0, device="cuda")
+    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    assert accel.sample_dev(buf.data_ptr(), n, stride, rows, p(U), p(ids), d_probs=p(probs), d_temperature=p(T), d_top_k=p(K), d_top_p=p(TP),
+                            d_min_p=p(MP), stream=stream(torch))
+    torch.cuda.synchronize()
+    return ids.cpu().numpy(), probs.cpu().numpy()
+
+
+def check_sample(x, u, ids, probs, T=None, K=None, TP=None, MP=None):
+    """Equal ids; a probability is off by f32 rounding of the exponent (|x - max| / T at most about 60 where it counts) and of
+    the weights: 2^-17 is eight times that."""
+    at = lambda a, r, d: d if a is None else float(np.float32(a[r]))  # noqa: E731
+    for r in range(x.shape[0]):
+        i, p = so.draw(x[r], float(np.float32(u[r])), at(T, r, 1.0), int(at(K, r, 0)), at(TP, r, 1.0), at(MP, r, 0.0))
+        assert ids[r] == i, (r, ids[r], i)
+        assert abs(probs[r] - p) <= p * 2.0 ** -17, (r, probs[r], p)
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 31, 33, 1000, 4097, 50001, 151936])
+def test_sample_all_parameters(torch, accel, n):
+    rng = np.random.RandomState(n)
+    rows = 24
+    x = (rng.randn(rows, n) * 3).astype(np.float32)
+    x[:, rng.randint(0, n, 5)] += 6
+    u = rng.rand(rows).astype(np.float32)
+    T = rng.choice([0.0, 0.3, 0.7, 1.0, 1.7], rows)
+    K = rng.choice([0, 1, 2, 40, 1000, n, n + 5, -3], rows)
+    TP = rng.choice([0.0, 0.1, 0.5, 0.9, 0.95, 1.0, 2.0], rows)
+    MP = rng.choice([0.0, 0.01, 0.05, 0.5, 1.0, 3.0], rows)
+    ids, probs = sample(torch, accel, x, u, T, K, TP, MP, stride=n + 3)
+    check_sample(x, u, ids, probs, T, K, TP, MP)
+    ids, probs = sample(torch, accel, x, u)
+    check_sample(x, u, ids, probs)
+    ids, probs = sample(torch, accel, x, u, top_k=K)
+    check_sample(x, u, ids, probs, K=K)
+    ids, probs = sample(torch, accel, x, u, top_p=TP)
+    check_sample(x, u, ids, probs, TP=TP)
+
+
+def test_sample_ties(torch, accel):
+    """Logits from a few values only (whole rows of ties): top-k and top-p cut inside the ties, lower indices first."""
+    rng = np.random.RandomState(1)
+    for n in (7, 500, 9999, 151936):
+        rows = 16
+        x = rng.randint(0, 3, (rows, n)).astype(np.float32)
+        x[3] = 1.0
+        x[4] = np.where(np.arange(n) % 2, 0.0, -0.0)         # equal, whatever their signs
+        u = rng.rand(rows).astype(np.float32)
+        K = rng.randint(1, n + 1, rows)
+        # whole numbers of equal weights: the border falls between tokens, not on one
+        TP = (rng.randint(0, 8, rows) + 0.37) / 8
+        ids, probs = sample(torch, accel, x, u, top_k=K)
+        check_sample(x, u, ids, probs, K=K)
+        ids, probs = sample(torch, accel, x, u, top_k=K, top_p=TP)
+        check_sample(x, u, ids, probs, K=K, TP=TP)
+
+
+def test_sample_special_logits(torch, accel):
+    inf, nan, n = np.inf, np.nan, 3000
+    x = np.random.RandomState(2).randn(12, n).astype(np.float32)
+    x[0] = -inf
+    x[1] = nan
+    x[2, ::2] = -inf
+    x[3, ::3] = nan
+    x[4, [5, 700, 2999]] = inf
+    x[5] = -inf
+    x[5, 2999] = -3.0e38
+    x[6] = 3.0e38
+    x[7] = -inf
+    x[7, 17] = inf
+    x[8] = x[8] * 1e30
+    x[9, 0] = nan
+    u = np.array([0.3, 0.9, 0.5, 0.1, 0.7, 0.5, 0.99, 0.2, 0.4, 0.6, 0.0, 1.0], np.float32)
+    for kw in (dict(), dict(top_k=[40] * 12), dict(top_p=[0.9] * 12), dict(temperature=[0.0] * 12), dict(top_k=[2] * 12, top_p=[0.6] * 12, min_p=[0.3] * 12)):
+        ids, probs = sample(torch, accel, x, u, **kw)
+        check_sample(x, u, ids, probs, kw.get("temperature"), kw.get("top_k"), kw.get("top_p"), kw.get("min_p"))
+
+
+def test_sample_greedy_is_argmax(torch, accel):
+    x = np.random.RandomState(4).randn(3, 151936).astype(np.float32)
+    ids, probs = sample(torch, accel, x, [0.1, 0.5, 0.999], temperature=[0.0, -1.0, float("nan")])
+    assert (ids == x.argmax(1)).all() and (probs == 1.0).all()
+
+
+def test_sample_follows_the_distribution(torch, accel):
+    """u on a grid: the counts of the drawn tokens are their probabilities to within one grid step."""
+    n, grid = 5, 1000
+    row = np.array([0.1, 2.0, -1.0, 1.0, 0.0], np.float32)
+    ids, _ = sample(torch, accel, np.tile(row, (grid, 1)), (np.arange(grid) + 0.5) / grid)
+    p = np.exp(row.astype(np.float64)) / np.exp(row.astype(np.float64)).sum()
+    assert (np.abs(np.bincount(ids, minlength=n) / grid - p) <= 1.0 / grid + 1e-6).all()
