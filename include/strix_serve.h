@@ -80,7 +80,7 @@ STRIX_API int strix_cuda_kv_check(const strix_kv_pages *cache, const strix_kv_ba
  * d_q_out may be d_q with the same ld; rows of idle slots and rows of nobody are left as they were in d_q_out.
  * F16: values rounded to nearest, beyond +-65504 to that. E4M3: the scale of a page and head is the least power of two s with
  * |value| <= 448 s for every row that entered the page (at least 2^-120). It starts anew when slot 0 is written and only
- * grows afterwards; when it does, the page's earlier codes move down by that power of two (exact until they
+ * grows afterwards; when it does, all other codes of the page and head move down by that power of two (exact until they
  * become subnormal). NaN is stored as 0, an infinity as the largest finite value.
  * Two rows of one call must not have the same page and slot, and a page that one call appends to must belong to one
  * sequence of the batch: the stored values are otherwise unspecified. */

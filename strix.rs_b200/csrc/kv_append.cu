@@ -328,10 +328,11 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
             for (int w = 1; w < WARPS; w++) m = fmaxf(m, red[w]);
             const float need = scale_for(m), s_new = s_old > need ? s_old : need, inv_s = 1.0f / s_new;
             if (threadIdx.x == 0) *scale = s_new;
-            if (slot && s_new != s_old) {  // the page's earlier codes move to the new scale
+            if (slot && s_new != s_old) {  // the page's other codes move to the new scale
                 const float f = s_old * inv_s;
                 uint4 *old = reinterpret_cast<uint4 *>(dst);
-                for (uint32_t i = threadIdx.x; i < slot * (HD / 16); i += WARPS * 32) {
+                for (uint32_t i = threadIdx.x; i < V.page_tokens * (HD / 16); i += WARPS * 32) {
+                    if (i / (HD / 16) - slot < cnt) continue;  // (unsigned: slots from `slot` on, cnt of them, are the new rows')
                     uint4 u = old[i];
                     uint32_t *p = &u.x;
 #pragma unroll
