@@ -16,34 +16,40 @@
 // output columns: each thread takes the dimensions that lie next to each other in a cached row, so that shared memory is read in
 // 16-byte words.
 //
-// Work split. A tile is TT tokens of one KV head (about 8 KB of k and v). All tiles of all (sequence, row block, KV head)
-// items stand in one line; block c of the grid takes an equal stretch of it, and each of the block's workers an equal part
-// of that. A worker is a warp (or several, over the row blocks of a prompt) with a ring of stages of its own, filled by bulk
-// copies that the block's producer warp issues, one lane for each worker. An item that one worker has whole is written
-// out by it; the parts of the others meet in shared memory at the block's end, and where an item goes on in another block, in the
-// workspace: the last block to arrive joins the parts, in the order of the line. Cuts that would fall into an item of at most
-// PA_SNAP tiles move to its nearer end.
+// Work split. A tile is TT tokens of one KV head (about 4 KB of k, as much of v). All tiles of all (sequence, row block, KV
+// head) items stand in one line; block c of the grid takes an equal stretch of it, and each of the block's workers an equal part
+// of that. A worker is a warp (or several, over the row blocks of a prompt) with a ring of half tiles (k, v, k, v, ...) of its
+// own, which its first warp refills by bulk copies as soon as a half is done with: k is on its way again while v is multiplied.
+// Page ids and scales are fetched 32 at a time, one to a lane. An item that one worker has whole is written out by it; the
+// parts of the others meet in shared memory at the block's end, and where an item goes on in another block, in the workspace:
+// the last block to arrive joins the parts, in the order of the line. Cuts that would fall into an item of at most PA_SNAP
+// tiles move to its nearer end.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "kv_pages.cuh"
 
 namespace strix {
 
 constexpr uint32_t PA_MAX_BLOCKS = 1024;  // tickets at the start of the workspace
+constexpr uint32_t PA_MAX_SEQ = 8192;     // their running tile counts lie in shared memory while a block finds its place
 constexpr uint32_t PA_SNAP = 16;
-constexpr size_t PA_STATIC = 1024;  // static shared memory and what the system keeps
+constexpr size_t PA_STATIC = 2048;  // 1024 to align the rings, the rest static shared memory and what the system keeps
 
 struct PagedAttnArgs {
+    CUtensorMap k_map, v_map;  // [page][KV head and slot][element]
     PagedView V;
     const float *q;
     float *out;
     size_t ld_q, ld_out;
     uint32_t n_heads, group, window, cap;  // cap: tokens a row of the page table can hold
+    uint32_t g_mul, g_shift;               // division by group
     float scale;
-    uint32_t wm, stages, vec;  // warps of a worker; stages of a ring; q and out rows start on 16 bytes
+    uint32_t wm, halves, vec;  // warps of a worker; half tiles of a ring; q and out rows start on 16 bytes
     uint32_t *ticket;          // [PA_MAX_BLOCKS]
     float *part;               // [blocks][2][rows of a worker][HD + 2]
 };
@@ -52,28 +58,39 @@ struct PagedAttnArgs {
 template <int HD, int TYPE, bool WIDE>
 struct PaShape {
     static constexpr int EL = TYPE == STRIX_KV_F16 ? 2 : 1;
-    static constexpr int NW = HD >= 192 && (WIDE || EL == 2) ? 4 : 8;  // consumer warps
+    // warps: three to a scheduler where 168 registers do, else two (a wide row block of a large head has 16 rows of O: one)
+    static constexpr int NW = HD >= 192 ? (WIDE ? 4 : 8) : (WIDE ? 8 : 12);
     static constexpr int ROWS = WIDE ? 16 : 8;                         // rows of a warp
     static constexpr int TT = HD * EL <= 64 ? 64 : HD * EL <= 128 ? 32 : 16;
-    static constexpr int KBYTES = TT * HD * EL, STAGE = 2 * KBYTES;
+    static constexpr int HALF = TT * HD * EL;                          // bytes of the k or the v of a tile
+    // In shared memory a half tile is BOXES blocks of TT rows by BOXB bytes. Rows of a multiple of 128 bytes all start in the same
+    // bank, so they come as blocks of 128-byte rows whose 16-byte words are swizzled (word c of row r at c ^ (r & 7)); rows of
+    // 64, 96 and 192 bytes lie as they are.
+    static constexpr bool SWZ = HD * EL % 128 == 0;
+    static constexpr int BOXB = SWZ ? 128 : HD * EL, BOXES = HD * EL / BOXB;
     static constexpr int PSTRIDE = HD + 2;                             // floats of a partial row: sums, maximum, sum of weights
     static constexpr bool QSMEM = WIDE && HD >= 192;                   // q fragments in shared memory instead of registers
     static constexpr int QBYTES = QSMEM ? NW * 16 * HD * 4 : 0;
     static constexpr int SLOTS = NW * ROWS * PSTRIDE * 4;              // one partial for each worker
-    static constexpr int DESC = 64, WORKER = 64;
-    static constexpr int fixed(int workers, int stages) { return SLOTS + QBYTES + workers * (WORKER + stages * (DESC + 16)); }
-    static int stages_for(int wm, size_t smem) {
+    static constexpr int DESCS = 8;                                    // tiles described at a time; above half the ring
+    static constexpr int WORKER = 64 + DESCS * 64;
+    __host__ __device__ static constexpr size_t fixed(int workers, int halves) { return SLOTS + QBYTES + workers * (WORKER + halves * 16); }
+    // the rings, and the parts that take their place at the end
+    __host__ __device__ static constexpr size_t rings(int workers, int halves) {
+        return (size_t)workers * halves * HALF > SLOTS ? (size_t)workers * halves * HALF : SLOTS;
+    }
+    static int halves_for(int wm, size_t smem) {  // half tiles of a ring
         const int workers = NW / wm;
-        int s = 16;
-        while (s > 1 && (size_t)fixed(workers, s) + (size_t)workers * s * STAGE > smem) s--;
-        return s;
+        int n = 2 * DESCS - 4;
+        while (n > 1 && fixed(workers, n) + rings(workers, n) > smem) n--;
+        return n;
     }
 };
 
-// What the producer tells a worker about a stage.
+// What the first warp tells a worker about a tile.
 struct __align__(16) PaTile {
-    uint32_t seq_first, seq_rows, ctx, tile;  // first row of the sequence, its new rows, tokens before them; tile of the item
-    uint32_t row0, head, flags, valid;        // first row of the block (in rows of the KV head), KV head; one bit for each page of the tile
+    uint32_t tile, flags, valid, row0;        // tile of the item; PA_*; one bit for each page of the tile; first row of the block
+    uint32_t seq_first, seq_rows, ctx, head;  // with PA_NEW: first row of the sequence, its new rows, tokens before them, KV head
     float ks[4], vs[4];                       // the scales of the tile's pages
 };
 enum : uint32_t { PA_NEW = 1, PA_END = 2, PA_WHOLE = 4, PA_HEAD = 8 };  // first / last tile of the segment here; item complete here; begun elsewhere
@@ -88,9 +105,14 @@ struct __align__(16) PaWorker {
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_from0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -102,6 +124,21 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_
     hi = f32_to_f16x2(x0, x1);
     const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
     lo = f32_to_f16x2(x0 - h.x, x1 - h.y);
+}
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+// true in one lane of the warp, in a form that lets the compiler know it is one
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0u;
 }
 template <int BYTES>
 __device__ __forceinline__ void lds_words(uint32_t *w, const uint8_t *p) {
@@ -116,57 +153,64 @@ __device__ __forceinline__ void lds_words(uint32_t *w, const uint8_t *p) {
     }
 }
 
-// Tiles of row block mb of a sequence: [lo_tile, lo_tile + n).
+// n / group for n < 2^31
+__device__ __forceinline__ uint32_t by_group(const PagedAttnArgs &A, uint32_t n) { return (__umulhi(n, A.g_mul) + n) >> A.g_shift; }
+
+// Tiles of row block mb of a sequence: [lo_tile, lo_tile + n). rb: rows of a block, a power of two.
 template <int TT>
 __device__ __forceinline__ uint32_t block_tiles(const PagedAttnArgs &A, uint32_t rb, uint32_t rows, uint32_t ctx, uint32_t mb,
                                                 uint32_t &lo_tile) {
     const uint32_t R = rows * A.group, r0 = mb * rb, r1 = min(R, r0 + rb) - 1u;
-    const uint32_t p0 = ctx + r0 / A.group, p1 = ctx + r1 / A.group;  // positions of the first and last row (below 2^32)
+    const uint32_t p0 = ctx + by_group(A, r0), p1 = ctx + by_group(A, r1);  // positions of the first and last row (below 2^32)
     const uint32_t hi = min(A.cap, p1 + 1u);
     const uint32_t lo = A.window && p0 >= A.window ? p0 + 1u - A.window : 0u;
     lo_tile = lo / TT;
     return hi > lo ? (hi + TT - 1u) / TT - lo_tile : 0u;
 }
-// All tiles of a sequence; rows and ctx are 0 and < 0 where there is nothing to do.
-template <int TT>
-__device__ __forceinline__ uint32_t seq_tiles(const PagedAttnArgs &A, uint32_t rb, uint32_t s, uint32_t &first, uint32_t &rows, int &ctx) {
-    uint32_t end;
-    bool bad = false;
-    seq_rows(A.V, s, first, end, bad);
-    rows = end - first;
-    ctx = A.V.ctx[s];
-    if (ctx < 0 || rows == 0u) return 0u;
-    uint32_t n = 0, lo;
-    const uint32_t blocks = (rows * A.group + rb - 1u) / rb;
-    for (uint32_t mb = 0; mb < blocks; mb++) n += block_tiles<TT>(A, rb, rows, (uint32_t)ctx, mb, lo);
-    return n * A.V.n_kv;
-}
 
 // A place in the line of tiles.
-struct PaPlace {
+struct __align__(16) PaPlace {
     uint32_t s, first, rows, ctx, mb, head, lo_tile, tiles, at;  // item: tiles of it, `at` the place within
     uint32_t item0;                                              // the line's index of the item's first tile
+    uint32_t left, pad;                                          // tiles of the worker from here on
 };
 
-// A lane's place from the sequence that holds line index x (whose own tiles start at base).
-template <int TT>
-__device__ __forceinline__ void place_in_seq(const PagedAttnArgs &A, uint32_t rb, uint32_t s, uint32_t base, uint32_t x, PaPlace &P) {
-    uint32_t first, rows;
-    int ctx;
-    (void)seq_tiles<TT>(A, rb, s, first, rows, ctx);
+__device__ __forceinline__ void load_seq(const PagedAttnArgs &A, uint32_t s, PaPlace &P) {
+    uint32_t end;
+    bool bad = false;
     P.s = s;
-    P.first = first;
-    P.rows = rows;
-    P.ctx = (uint32_t)ctx;
-    uint32_t off = x - base, mb = 0, lo, n;
-    const uint32_t blocks = (rows * A.group + rb - 1u) / rb;
-    for (;; mb++) {
-        n = block_tiles<TT>(A, rb, rows, P.ctx, mb, lo);
-        if (off < n * A.V.n_kv || mb + 1u >= blocks) break;
+    seq_rows(A.V, s, P.first, end, bad);
+    P.rows = end - P.first;
+    P.ctx = (uint32_t)A.V.ctx[s];
+}
+// All tiles of a sequence.
+template <int TT>
+__device__ __forceinline__ uint32_t seq_tiles(const PagedAttnArgs &A, uint32_t rb, uint32_t s) {
+    PaPlace P;
+    load_seq(A, s, P);
+    if ((int)P.ctx < 0 || P.rows == 0u) return 0u;
+    uint32_t n = 0, lo;
+    const uint32_t blocks = (P.rows * A.group + rb - 1u) / rb;
+    for (uint32_t mb = 0; mb < blocks; mb++) n += block_tiles<TT>(A, rb, P.rows, P.ctx, mb, lo);
+    return n * A.V.n_kv;
+}
+// The place of line index x; upto[s]: tiles of the sequences up to and including s.
+template <int TT>
+__device__ __forceinline__ void find_place(const PagedAttnArgs &A, uint32_t rb, const uint32_t *upto, uint32_t x, PaPlace &P) {
+    uint32_t lo = 0, hi = A.V.n_seq - 1u;  // the first sequence with upto > x
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (upto[mid] > x) hi = mid; else lo = mid + 1u;
+    }
+    load_seq(A, lo, P);
+    uint32_t off = x - (lo ? upto[lo - 1u] : 0u), n = 0, first_tile = 0;
+    const uint32_t blocks = (P.rows * A.group + rb - 1u) / rb;
+    for (P.mb = 0;; P.mb++) {
+        n = block_tiles<TT>(A, rb, P.rows, P.ctx, P.mb, first_tile);
+        if (off < n * A.V.n_kv || P.mb + 1u >= blocks) break;
         off -= n * A.V.n_kv;
     }
-    P.mb = mb;
-    P.lo_tile = lo;
+    P.lo_tile = first_tile;
     P.tiles = n;
     P.head = n ? off / n : 0u;
     P.at = n ? off - P.head * n : 0u;
@@ -186,52 +230,26 @@ __device__ __forceinline__ void next_item(const PagedAttnArgs &A, uint32_t rb, P
             if (P.tiles) return;
             continue;
         }
-        if (++P.s >= A.V.n_seq) {
+        if (P.s + 1u >= A.V.n_seq) {
             P.tiles = 0;
             return;
         }
-        uint32_t end;
-        bool bad = false;
-        seq_rows(A.V, P.s, P.first, end, bad);
-        P.rows = end - P.first;
-        P.ctx = (uint32_t)A.V.ctx[P.s];
+        load_seq(A, P.s + 1u, P);
         P.mb = 0xffffffffu;
         if (P.rows == 0u) P.ctx = 0xffffffffu;
     }
 }
 
-// Finds the places of up to 8 line indices (x[i] < total, ascending not needed) by one pass over the sequences; lane i gets place i.
-template <int TT>
-__device__ __forceinline__ void find_places(const PagedAttnArgs &A, uint32_t rb, uint32_t x, uint32_t count, PaPlace &P) {
-    const uint32_t lane = threadIdx.x & 31u;
-    uint32_t base = 0, mine_s = 0, mine_base = 0;
-    uint32_t left = count == 32u ? 0xffffffffu : (1u << count) - 1u;
-    for (uint32_t c = 0; c < A.V.n_seq && left; c += 32u) {
-        uint32_t first, rows;
-        int ctx;
-        const uint32_t n = c + lane < A.V.n_seq ? seq_tiles<TT>(A, rb, c + lane, first, rows, ctx) : 0u;
-        uint32_t incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-            if ((int)lane >= o) incl += v;
-        }
-        for (uint32_t i = 0; i < count; i++) {
-            if (!((left >> i) & 1u)) continue;
-            const uint32_t xi = __shfl_sync(0xffffffffu, x, i) - base;
-            const uint32_t m = __ballot_sync(0xffffffffu, incl > xi);
-            if (m == 0u) continue;
-            const uint32_t j = __ffs(m) - 1u, before = __shfl_sync(0xffffffffu, incl - n, j);
-            if (lane == i) {
-                mine_s = c + j;
-                mine_base = base + before;
-            }
-            left &= ~(1u << i);
-        }
-        base += __shfl_sync(0xffffffffu, incl, 31);
+// The line's division among blocks: equal to within a tile.
+struct PaCuts {
+    uint32_t per, rem;
+    __device__ PaCuts(uint32_t total, uint32_t parts) : per(total / parts), rem(total - per * parts) {}
+    __device__ uint32_t cut(uint32_t c) const { return c * per + min(c, rem); }
+    __device__ uint32_t part_of(uint32_t x) const {  // the part that holds index x
+        const uint32_t big = rem * (per + 1u);
+        return x < big ? x / (per + 1u) : rem + (x - big) / per;
     }
-    if (lane < count) place_in_seq<TT>(A, rb, mine_s, mine_base, x, P);
-}
+};
 
 // Where cut x of the line falls: cuts inside a short item move to its nearer end.
 __device__ __forceinline__ uint32_t snapped(const PaPlace &P, uint32_t x) {
@@ -240,209 +258,251 @@ __device__ __forceinline__ uint32_t snapped(const PaPlace &P, uint32_t x) {
 }
 
 template <int HD, int TYPE, bool WIDE>
-__global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs A) {
+__global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs A) {
     using S = PaShape<HD, TYPE, WIDE>;
     constexpr int EL = S::EL, NW = S::NW, TT = S::TT, NT = TT / 8, KS = HD / 16;
-    constexpr int PS = S::PSTRIDE, NO = HD / 8;          // NO: output tiles of eight columns
+    constexpr int PS = S::PSTRIDE, NO = HD / 8;           // NO: output tiles of eight columns
     constexpr int KW = (HD / 4 * EL) % 16 == 0 ? 16 : 8;  // bytes of a thread's k loads
     constexpr int KL = HD / 4 * EL / KW;                  // ... and how many a token
     constexpr int VB = HD / 8 * EL;                       // bytes of a cached value row that a thread turns into output columns
-    constexpr int VW = VB % 16 == 0 ? 16 : VB % 8 == 0 ? 8 : 4, VL = VB / VW;
+    constexpr int VW = S::SWZ ? 16 : VB % 16 == 0 ? 16 : VB % 8 == 0 ? 8 : 4, VL = VB / VW;
+    // output column n of output tile i is dimension col_dim(n) + tile_dim(i): with swizzled rows a thread's columns are one
+    // 16-byte word of each block of 128 bytes, else they are neighbours
+    constexpr int WD = S::SWZ ? 16 / EL : NO;
+    auto tile_dim = [](int i) { return i / WD * (S::BOXB / EL) + i % WD; };
     constexpr int RW = WIDE ? 2 : 1;                      // rows of a thread
-    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr uint32_t DESCS = S::DESCS;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (the swizzle goes by address)
     const PagedView &V = A.V;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t wm = WIDE ? A.wm : 1u, workers = NW / wm, rb = S::ROWS * wm, stages = A.stages;
+    const uint32_t wm = WIDE ? A.wm : 1u, workers = NW / wm, rb = S::ROWS * wm, halves = A.halves;
     uint8_t *rings = smem;
-    float *slots = reinterpret_cast<float *>(smem + (size_t)workers * stages * S::STAGE);
+    float *slots = reinterpret_cast<float *>(smem + S::rings(workers, halves));
     uint8_t *qsm = reinterpret_cast<uint8_t *>(slots) + S::SLOTS;
-    PaTile *desc = reinterpret_cast<PaTile *>(qsm + S::QBYTES);
-    PaWorker *info = reinterpret_cast<PaWorker *>(desc + workers * stages);
-    uint64_t *full = reinterpret_cast<uint64_t *>(info + workers), *empty = full + workers * stages;
-    __shared__ uint32_t range[2], last_here;
+    PaTile *descs = reinterpret_cast<PaTile *>(qsm + S::QBYTES);
+    PaWorker *info = reinterpret_cast<PaWorker *>(descs + workers * DESCS);
+    uint64_t *full = reinterpret_cast<uint64_t *>(info + workers), *empty = full + workers * halves;
+    __shared__ uint32_t last_here[2], scan[NW];
 
-    if (threadIdx.x < workers * stages) {
-        mbar_init(&full[threadIdx.x], 1);
-        mbar_init(&empty[threadIdx.x], wm);
+    // ---- running tile counts of the sequences (where the rings will be)
+    uint32_t *upto = reinterpret_cast<uint32_t *>(rings);
+    uint32_t total = 0;
+    for (uint32_t c = 0; c < V.n_seq; c += NW * 32) {
+        uint32_t n = c + threadIdx.x < V.n_seq ? seq_tiles<TT>(A, rb, c + threadIdx.x) : 0u;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, n, d);
+            if ((int)lane >= d) n += v;
+        }
+        if (lane == 31u) scan[warp] = n;
+        __syncthreads();
+        uint32_t before = total;
+        for (uint32_t w = 0; w < NW; w++) {
+            if (w < warp) before += scan[w];
+            total += scan[w];
+        }
+        if (c + threadIdx.x < V.n_seq) upto[c + threadIdx.x] = before + n;
+        __syncthreads();
+    }
+    for (uint32_t i = threadIdx.x; i < workers * halves; i += NW * 32) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], wm);
         mbar_fence_init();
     }
-    if (threadIdx.x < workers) {
-        info[threadIdx.x].has_head = info[threadIdx.x].head_ended = info[threadIdx.x].has_tail = 0u;
-    }
+    for (uint32_t i = threadIdx.x; i < workers * DESCS * 4u; i += NW * 32) descs[i / 4u].ks[i & 3u] = descs[i / 4u].vs[i & 3u] = 0.f;
+    if (threadIdx.x < workers) info[threadIdx.x].has_head = info[threadIdx.x].head_ended = info[threadIdx.x].has_tail = 0u;
 
-    // ---- this block's stretch of the line, by the producer warp
-    uint32_t total = 0, blocks = 0;
+    // ---- this block's stretch of the line and this worker's part of it
+    const uint32_t worker = warp / wm, wi = warp - worker * wm;  // warp of the worker
+    const uint32_t line_blocks = min(gridDim.x, (total + workers - 1u) / workers);  // blocks with work
+    uint32_t n_block = 0, n_mine = 0;
     PaPlace place{};
-    uint32_t w_begin = 0, w_end = 0;  // producer lanes: the worker's stretch
-    if (warp == NW) {
-        for (uint32_t c = lane; c < V.n_seq; c += 32u) {
-            uint32_t first, rows;
-            int ctx;
-            total += seq_tiles<TT>(A, rb, c, first, rows, ctx);
+    if (blockIdx.x < line_blocks) {
+        const PaCuts line(total, line_blocks);
+        uint32_t x = line.cut(blockIdx.x + (lane & 1u));
+        if (x < total) {
+            find_place<TT>(A, rb, upto, x, place);
+            x = snapped(place, x);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        blocks = min(gridDim.x, (total + workers - 1u) / workers);  // blocks with work
-        uint32_t lo = 0, hi = 0;
-        if (blockIdx.x < blocks) {
-            uint32_t x = (uint32_t)((uint64_t)(blockIdx.x + (lane == 1u)) * total / blocks);
-            const bool at_end = x >= total;
-            PaPlace P{};
-            find_places<TT>(A, rb, at_end ? total - 1u : x, 2u, P);
-            if (!at_end) x = snapped(P, x);
-            lo = __shfl_sync(0xffffffffu, x, 0);
-            hi = __shfl_sync(0xffffffffu, x, 1);
-        }
-        if (lane == 0) {
-            range[0] = lo;
-            range[1] = hi;
-        }
-        if (hi > lo) {
-            const uint32_t n = hi - lo;
-            w_begin = lo + (uint32_t)((uint64_t)min(lane, workers) * n / workers);
-            w_end = lo + (uint32_t)((uint64_t)min(lane + 1u, workers) * n / workers);
-            if (lane >= workers) w_begin = w_end = 0;
-            find_places<TT>(A, rb, min(w_begin, total - 1u), workers, place);
+        const uint32_t lo = __shfl_sync(0xffffffffu, x, 0), hi = __shfl_sync(0xffffffffu, x, 1);
+        n_block = hi - lo;
+        if (n_block) {
+            const PaCuts mine(n_block, workers);
+            const uint32_t w0 = mine.cut(worker);
+            n_mine = mine.cut(worker + 1u) - w0;
+            if (n_mine) find_place<TT>(A, rb, upto, lo + w0, place);
         }
     }
     __syncthreads();
+    uint8_t *ring = rings + (size_t)worker * halves * S::HALF;
+    PaTile *desc = descs + worker * DESCS;
+    full += worker * halves;
+    empty += worker * halves;
 
-    const uint32_t n_block = range[1] - range[0];
-    const uint32_t worker = warp == NW ? 0u : warp / wm;
-    // consumer state that outlives the loop (a part that goes on in the next worker)
+    // ---- the worker's first warp: copies of the next half tile. All of this is the same in every lane but the batch.
+    uint32_t is_half = 0, is_tile = 0, is_left = 2u * n_mine;  // ring place, tile and number of the halves still to be issued
+    uint32_t ds_half = 0, ds_tile = 0, ds_from = 0, ds_left = is_left;  // the same of those still to be described
+    uint32_t b_from = 0, b_stop = 0, seg_stop = 0;             // batch: its next lane, its end and the segment's in tiles of the item
+    uint32_t new_flag = 0, end_flag = 0;
+    bool started = false;
+    int b_page = -1, c_page = -1;                              // this lane's page of the batch; of the tile whose k went last
+    float b_ks = 0.f, b_vs = 0.f;
+    uint32_t c_y = 0;
+    bool bad = false;
+    b_stop = seg_stop = place.at;
+    const uint32_t sub = TT > 16 ? min((uint32_t)TT, V.page_tokens) : 16u;  // tokens of a copy
+    const uint32_t sub_shift = TT / sub == 4u ? 2u : TT / sub == 2u ? 1u : 0u, n_sub = 1u << sub_shift, sub_at = lane & (n_sub - 1u);
+    const bool leader = elect_lane();
+    // Completes the description of the next issued half: the scales came last from memory, the copies did not wait for them.
+    auto describe = [&] {
+        if ((ds_left & 1u) == 0u) {
+            if (lane - ds_from < n_sub) {
+                desc[ds_tile].ks[lane - ds_from] = b_ks;
+                desc[ds_tile].vs[lane - ds_from] = b_vs;
+            }
+            ds_from += n_sub;
+            ds_tile = (ds_tile + 1u) & (DESCS - 1u);
+            __syncwarp();
+        }
+        if (leader) mbar_arrive(&full[ds_half]);
+        if (++ds_half == halves) ds_half = 0;
+        ds_left--;
+    };
+    // The next segment, if one has ended, and the page ids and scales of its next 32 pages.
+    auto next_batch = [&] {
+        while (ds_left > is_left) describe();
+        if (place.at == seg_stop) {
+            if (started) next_item<TT>(A, rb, place);
+            started = true;
+            const uint32_t left = is_left / 2u, seg = min(left, place.tiles - place.at);
+            const bool ends = place.at + seg == place.tiles;
+            seg_stop = place.at + seg;
+            new_flag = PA_NEW;
+            end_flag = PA_END | (place.at ? PA_HEAD : ends ? PA_WHOLE : 0u);
+            if (lane == 0) {  // how the segment relates to its item
+                const PaWorker::Part part{place.first, place.rows, place.mb * rb, place.head, place.item0, place.tiles};
+                PaWorker *me = info + worker;
+                if (place.at) {
+                    me->head = part;
+                    me->has_head = 1u;
+                    me->head_ended = ends;
+                } else if (!ends) {
+                    me->tail = part;
+                    me->has_tail = 1u;
+                }
+            }
+        }
+        ds_from = b_from = 0;
+        const uint32_t n = min(32u >> sub_shift, seg_stop - place.at);
+        b_stop = place.at + n;
+        const uint32_t tok = (place.lo_tile + place.at) * TT + lane * sub, nth = tok >> V.page_shift;
+        b_page = -1;
+        b_ks = b_vs = 0.f;
+        if (lane < n << sub_shift && tok <= place.ctx + (place.rows - 1u) && nth < V.pages_ld) {
+            b_page = V.pages[(size_t)place.s * V.pages_ld + nth];
+            if (b_page < 0 || (uint32_t)b_page >= V.n_pages) {
+                b_page = -1;
+                bad = true;
+            } else if (TYPE == STRIX_KV_E4M3) {
+                b_ks = V.k_scale[(size_t)b_page * V.n_kv + place.head];
+                b_vs = V.v_scale[(size_t)b_page * V.n_kv + place.head];
+            } else {
+                b_ks = b_vs = 1.f;
+            }
+        }
+    };
+    auto issue = [&] {
+        const bool is_v = is_left & 1u;
+        if (!is_v) {  // k: a new tile
+            if (place.at == b_stop) next_batch();
+            const uint32_t tile = place.lo_tile + place.at;
+            c_page = __shfl_sync(0xffffffffu, b_page, b_from + sub_at);
+            c_y = place.head * V.page_tokens + ((tile * TT + sub_at * sub) & (V.page_tokens - 1u));
+            const uint32_t valid = __ballot_sync(0xffffffffu, c_page >= 0) & ((1u << n_sub) - 1u);
+            if (lane == 0) {
+                PaTile &d = desc[is_tile];
+                *reinterpret_cast<uint4 *>(&d.tile) = make_uint4(tile, new_flag | (place.at + 1u == seg_stop ? end_flag : 0u), valid, place.mb * rb);
+                if (new_flag) *reinterpret_cast<uint4 *>(&d.seq_first) = make_uint4(place.first, place.rows, place.ctx, place.head);
+            }
+            __syncwarp();
+            new_flag = 0u;
+            b_from += n_sub;
+            place.at++;
+            is_tile = (is_tile + 1u) & (DESCS - 1u);
+        }
+        uint64_t *bar = &full[is_half];
+        uint8_t *dst = ring + is_half * S::HALF;
+        const CUtensorMap *map = is_v ? &A.v_map : &A.k_map;
+        for (uint32_t i = 0; i < n_sub; i++) {
+            const int page = TT > 16 ? __shfl_sync(0xffffffffu, c_page, i) : c_page;
+            const uint32_t y = TT > 16 ? __shfl_sync(0xffffffffu, c_y, i) : c_y;
+            if (page >= 0 && leader) {
+                mbar_expect_tx(bar, sub * HD * EL);
+#pragma unroll
+                for (int box = 0; box < S::BOXES; box++)
+                    tma_load_3d(dst + box * (TT * S::BOXB) + i * sub * S::BOXB, map, box * (S::BOXB / EL), y, (uint32_t)page, bar);
+            }
+        }
+        if (++is_half == halves) is_half = 0;
+        is_left--;
+    };
+
+    // ---- rows that see nothing, and lengths beyond the table: each sequence is looked at by one warp of the grid
+    for (uint32_t s = blockIdx.x * NW + warp; s < V.n_seq; s += gridDim.x * NW) {
+        uint32_t first, end;
+        seq_rows(V, s, first, end, bad);
+        const int ctx = V.ctx[s];
+        const uint32_t rows = end - first;
+        const bool over = ctx >= 0 && rows && (uint64_t)(uint32_t)ctx + rows > A.cap;
+        bad |= over;
+        if (ctx < 0 || over) {
+            const uint32_t R = rows * A.group, nb = (R + rb - 1u) / rb;
+            for (uint32_t mb = 0; mb < nb; mb++) {
+                uint32_t lo;
+                if (ctx >= 0 && block_tiles<TT>(A, rb, rows, (uint32_t)ctx, mb, lo)) continue;
+                for (uint32_t r = mb * rb; r < min(R, (mb + 1u) * rb); r++)
+                    for (uint32_t h = 0; h < V.n_kv; h++) {
+                        float *dst = A.out + (size_t)(first + by_group(A, r)) * A.ld_out + (size_t)(h * A.group + r - by_group(A, r) * A.group) * HD;
+                        for (uint32_t i = lane; i < HD; i += 32u) dst[i] = 0.f;
+                    }
+            }
+        }
+    }
+
+    // ---- the loop over half tiles: k to weights, v to sums. The worker's first warp runs ahead by a ring.
     float o[NO][2 * RW], m[RW], l[RW];
     bool open_tail = false;
-
-    if (warp == NW) {
-        // ---- producer: lane w fills the ring of worker w
-        uint32_t left = w_end - w_begin, stage = 0, phase = 1;  // (the first pass over a ring finds it empty)
-        uint32_t idle = 0;
-        bool fresh = true, bad = false;
-        PaWorker *me = info + min(lane, workers - 1u);
-        const uint32_t sub = TT > 16 ? min((uint32_t)TT, V.page_tokens) : 16u;  // tokens of one copy
-        while (__any_sync(0xffffffffu, left > 0u)) {
-            if (left > 0u && mbar_test_wait(&empty[lane * stages + stage], phase)) {
-                idle = 0;
-                const uint32_t tile = place.lo_tile + place.at, tok = tile * TT;
-                PaTile d;
-                d.seq_first = place.first;
-                d.seq_rows = place.rows;
-                d.ctx = place.ctx;
-                d.tile = tile;
-                d.row0 = place.mb * rb;
-                d.head = place.head;
-                d.flags = fresh ? PA_NEW : 0u;
-                const bool item_end = place.at + 1u == place.tiles, seg_end = item_end || left == 1u;
-                if (fresh) {  // how the segment relates to its item
-                    const uint32_t seg = min(left, place.tiles - place.at);
-                    PaWorker::Part part{place.first, place.rows, d.row0, place.head, place.item0, place.tiles};
-                    if (place.at > 0u) {
-                        me->head = part;
-                        me->has_head = 1u;
-                        me->head_ended = place.at + seg == place.tiles;
-                    } else if (seg < place.tiles) {
-                        me->tail = part;
-                        me->has_tail = 1u;
-                    }
-                }
-                if (seg_end) {
-                    d.flags |= PA_END;
-                    if (me->has_head && me->head.item0 == place.item0) d.flags |= PA_HEAD;
-                    else if (item_end) d.flags |= PA_WHOLE;
-                }
-                d.valid = 0u;
-                uint32_t bytes = 0;
-                int page[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    page[i] = -1;
-                    if (i * sub < TT) {
-                        const uint32_t nth = (tok + i * sub) >> V.page_shift;
-                        page[i] = nth < V.pages_ld ? V.pages[(size_t)place.s * V.pages_ld + nth] : -2;  // (-2: past the table's end)
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    d.ks[i] = d.vs[i] = 0.f;
-                    if (i * sub >= TT || tok + i * sub > place.ctx + (place.rows - 1u)) continue;  // behind the sequence: no page to look at
-                    if (page[i] < 0 || (uint32_t)page[i] >= V.n_pages) {
-                        bad |= page[i] != -2;
-                        continue;
-                    }
-                    d.valid |= 1u << i;
-                    bytes += 2u * sub * HD * EL;
-                    if (TYPE == STRIX_KV_E4M3) {
-                        const size_t at = (size_t)page[i] * V.n_kv + place.head;
-                        d.ks[i] = V.k_scale[at];
-                        d.vs[i] = V.v_scale[at];
-                    } else {
-                        d.ks[i] = d.vs[i] = 1.f;
-                    }
-                }
-                desc[lane * stages + stage] = d;
-                uint64_t *bar = &full[lane * stages + stage];
-                uint8_t *dst = rings + (size_t)(lane * stages + stage) * S::STAGE;
-                mbar_arrive_expect_tx(bar, bytes);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if (!((d.valid >> i) & 1u)) continue;
-                    const size_t src = (size_t)page[i] * V.page_bytes + (size_t)place.head * V.head_bytes +
-                                       (size_t)((tok + i * sub) & (V.page_tokens - 1u)) * HD * EL;
-                    bulk_g2s(dst + i * sub * HD * EL, V.k + src, sub * HD * EL, bar);
-                    bulk_g2s(dst + S::KBYTES + i * sub * HD * EL, V.v + src, sub * HD * EL, bar);
-                }
-                if (++stage == stages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-                left--;
-                place.at++;
-                fresh = seg_end;
-                if (item_end && left > 0u) next_item<TT>(A, rb, place);
-            } else if (left > 0u && ++idle > (1u << 24)) {  // a worker that takes nothing for seconds: report and stop feeding it
-                atomicOr(V.status, STATUS_WAIT_TIMEOUT);
-                left = 0;
+    const uint32_t g = lane >> 2, t = lane & 3u;   // row and column of the fragments
+    // Column n of eight tokens is token n ^ 4 for odd n: with the swizzle, that spreads the words that eight neighbouring
+    // threads read over all banks, in k (rows g, g + 1) and in v (rows of columns 2 t, or 2 t + 1, and words g, g + 1).
+    const uint32_t kr = g ^ ((g & 1u) << 2), vr[2] = {2u * t, (2u * t + 1u) ^ 4u};
+    const uint32_t k_off[2] = {S::SWZ ? kr * 128u + ((t ^ kr) << 4) : kr * (HD * EL) + t * KW, S::SWZ ? kr * 128u + (((t + 4u) ^ kr) << 4) : 0u};
+    const uint32_t v_off[2] = {S::SWZ ? vr[0] * 128u + ((g ^ vr[0]) << 4) : vr[0] * (HD * EL) + g * VB,
+                               S::SWZ ? vr[1] * 128u + ((g ^ vr[1]) << 4) : vr[1] * (HD * EL) + g * VB};
+    uint32_t half = 0, phase = 0, e_half = 0, e_phase = 0;  // next half to use; next to refill
+    uint32_t qf[S::QSMEM ? 1 : KS][WIDE ? 8 : 4];  // fragments of q: values (and remainders, in the same rows or apart)
+    uint4 *qs = reinterpret_cast<uint4 *>(qsm) + warp * (KS * 2 * 32) + lane;
+    float qc[RW], vref = 0.f;                      // factor from the products to exponents of two; scale of the tile's values
+    uint32_t pos[RW], pos_lo = 0, pos_hi = 0;      // positions of this thread's rows, of the warp's first and last row
+    uint32_t pf[TT / 16][WIDE ? 8 : 4];            // fragments of the weights
+    bool tail_tok = false;
+    uint32_t it_first = 0, it_rows = 0, it_row0 = 0, it_head = 0;  // the item: first row of its sequence, new rows, first row of its own, KV head
+    const int steps = (int)(2u * n_mine);
+    for (int step = wi == 0 ? -(int)min(halves, 2u * n_mine) : 0; step < steps; step++) {
+        if (step >= 0) {
+        const PaTile &d = desc[(uint32_t)step / 2u & (DESCS - 1u)];
+        if ((step & 1) == 0) {
+            if (wm > 1u) {  // (the other warps get the description with the copy)
+                if (wi == 0)
+                    while (ds_left > is_left) describe();
+                if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
             }
-        }
-        report_bad(V, bad);
-    } else {
-        // ---- rows that see nothing, and lengths beyond the table: each sequence is looked at by one warp of the grid
-        for (uint32_t s = blockIdx.x * NW + warp; s < V.n_seq; s += gridDim.x * NW) {
-            uint32_t first, end;
-            bool bad = false;
-            seq_rows(V, s, first, end, bad);
-            const int ctx = V.ctx[s];
-            const uint32_t rows = end - first;
-            if (ctx >= 0 && (uint64_t)(uint32_t)ctx + rows > A.cap && rows) bad = true;
-            if (ctx < 0 || (uint64_t)(uint32_t)ctx + rows > A.cap) {
-                const uint32_t R = rows * A.group, nb = (R + rb - 1u) / rb;
-                for (uint32_t mb = 0; mb < nb; mb++) {
-                    uint32_t lo;
-                    if (ctx >= 0 && block_tiles<TT>(A, rb, rows, (uint32_t)ctx, mb, lo)) continue;
-                    for (uint32_t r = mb * rb; r < min(R, (mb + 1u) * rb); r++)
-                        for (uint32_t h = 0; h < V.n_kv; h++) {
-                            float *dst = A.out + (size_t)(first + r / A.group) * A.ld_out + (size_t)(h * A.group + r % A.group) * HD;
-                            for (uint32_t i = lane; i < HD; i += 32u) dst[i] = 0.f;
-                        }
-                }
-            }
-            report_bad(V, bad && lane == 0);
-        }
-
-        // ---- consumer
-        const uint32_t g = lane >> 2, t = lane & 3u, wi = warp - worker * wm;  // row and column of the fragments; warp of the worker
-        const uint32_t n_mine = (uint32_t)((uint64_t)(worker + 1u) * n_block / workers) - (uint32_t)((uint64_t)worker * n_block / workers);
-        uint32_t stage = 0, phase = 0;
-        uint32_t qf[S::QSMEM ? 1 : KS][WIDE ? 8 : 4];  // fragments of q: values (and remainders, in the same rows or apart)
-        uint4 *qs = reinterpret_cast<uint4 *>(qsm) + warp * (KS * 2 * 32) + lane;
-        float qc[RW];                                  // factor from the products to exponents of two
-        uint32_t pos[RW], pos_lo = 0, pos_hi = 0;      // positions of this thread's rows, of the warp's first and last row
-        for (uint32_t n = 0; n < n_mine; n++) {
-            if (!mbar_wait_bounded(&full[worker * stages + stage], phase, V.status)) break;  // (the producer gives up as well)
-            const PaTile &d = desc[worker * stages + stage];
-            const uint8_t *ks = rings + (size_t)(worker * stages + stage) * S::STAGE, *vs = ks + S::KBYTES;
-            const uint32_t flags = d.flags;
-            if (flags & PA_NEW) {
+            if (d.flags & PA_NEW) {
+                it_first = d.seq_first;
+                it_rows = d.seq_rows;
+                it_row0 = d.row0;
+                it_head = d.head;
                 const uint32_t R = d.seq_rows * A.group, rw = d.row0 + wi * S::ROWS;
                 const float *qrow[RW];
                 bool on[RW];
@@ -450,12 +510,12 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
                 for (int i = 0; i < RW; i++) {
                     const uint32_t r = rw + g + 8u * i;
                     on[i] = r < R;
-                    const uint32_t rr = min(r, R - 1u), tk = rr / A.group;
+                    const uint32_t rr = min(r, R - 1u), tk = by_group(A, rr);
                     pos[i] = d.ctx + tk;
                     qrow[i] = A.q + (size_t)(d.seq_first + tk) * A.ld_q + (size_t)(d.head * A.group + rr - tk * A.group) * HD;
                 }
-                pos_lo = d.ctx + min(rw, R - 1u) / A.group;
-                pos_hi = d.ctx + min(rw + S::ROWS - 1u, R - 1u) / A.group;
+                pos_lo = d.ctx + by_group(A, min(rw, R - 1u));
+                pos_hi = d.ctx + by_group(A, min(rw + S::ROWS - 1u, R - 1u));
                 float x[RW][KS][4];
 #pragma unroll
                 for (int i = 0; i < RW; i++) {
@@ -520,72 +580,112 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
             }
 
             // scores: products of q with eight tokens at a time
+            if (wm == 1u) {
+                while (ds_left > is_left) describe();
+                if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
+            }
+            const uint8_t *ks = ring + half * S::HALF;
             const uint32_t tok = d.tile * TT, valid = d.valid;
             float sc[NT][4];
+            // (the token groups go side by side: a product waits for the one before it on the same sums)
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const uint8_t *kr = ks + (8 * j + g) * (HD * EL) + t * KW;
-                uint32_t w[KL * KW / 4];
+            for (int i = 0; i < KL; i++) {
+                uint32_t w[NT][KW / 4];
 #pragma unroll
-                for (int i = 0; i < KL; i++) lds_words<KW>(w + i * (KW / 4), kr + i * 4 * KW);
+                for (int j = 0; j < NT; j++)
+                    lds_words<KW>(w[j], S::SWZ ? ks + k_off[i & 1] + (i >> 1) * (TT * 128) + j * 1024 : ks + k_off[0] + j * (8 * HD * EL) + i * 4 * KW);
 #pragma unroll
-                for (int e = 0; e < 4; e++) sc[j][e] = 0.f;
+                for (int x = 0; x < KW * 4 / (16 * EL); x++) {
+                    const int s = i * (KW * 4 / (16 * EL)) + x;
+                    uint32_t b0[NT], b1[NT];
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    uint32_t b0, b1;
-                    if constexpr (EL == 1) {
-                        b0 = e4m3x2_to_f16x2(w[s] & 0xffffu);
-                        b1 = e4m3x2_to_f16x2(w[s] >> 16);
-                    } else {
-                        b0 = w[2 * s];
-                        b1 = w[2 * s + 1];
+                    for (int j = 0; j < NT; j++) {
+                        if constexpr (EL == 1) {
+                            e4m3x4_to_f16x2(w[j][x], b0[j], b1[j]);
+                        } else {
+                            b0[j] = w[j][2 * x];
+                            b1[j] = w[j][2 * x + 1];
+                        }
                     }
                     if constexpr (!WIDE) {
-                        mma_f16(sc[j], reinterpret_cast<const uint32_t(&)[4]>(qf[s]), b0, b1);
-                    } else if constexpr (!S::QSMEM) {
-                        const uint32_t hi[4] = {qf[s][0], qf[s][1], qf[s][2], qf[s][3]}, lo[4] = {qf[s][4], qf[s][5], qf[s][6], qf[s][7]};
-                        mma_f16(sc[j], lo, b0, b1);
-                        mma_f16(sc[j], hi, b0, b1);
+                        const uint32_t(&q)[4] = reinterpret_cast<const uint32_t(&)[4]>(qf[s]);
+#pragma unroll
+                        for (int j = 0; j < NT; j++) {
+                            if (s == 0) mma_f16_from0(sc[j], q, b0[j], b1[j]);
+                            else mma_f16(sc[j], q, b0[j], b1[j]);
+                        }
                     } else {
-                        const uint4 h4 = qs[(2 * s) * 32], l4 = qs[(2 * s + 1) * 32];
+                        uint4 h4, l4;
+                        if constexpr (S::QSMEM) {
+                            h4 = qs[(2 * s) * 32];
+                            l4 = qs[(2 * s + 1) * 32];
+                        } else {
+                            h4 = make_uint4(qf[s][0], qf[s][1], qf[s][2], qf[s][3]);
+                            l4 = make_uint4(qf[s][4], qf[s][5], qf[s][6], qf[s][7]);
+                        }
                         const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
-                        mma_f16(sc[j], lo, b0, b1);
-                        mma_f16(sc[j], hi, b0, b1);
+#pragma unroll
+                        for (int j = 0; j < NT; j++) {
+                            if (s == 0) mma_f16_from0(sc[j], lo, b0[j], b1[j]);
+                            else mma_f16(sc[j], lo, b0[j], b1[j]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < NT; j++) mma_f16(sc[j], hi, b0[j], b1[j]);
                     }
                 }
             }
             // to exponents of two; scale of the page; masks
             const uint32_t pshift = V.page_shift;
-            const bool all = valid == (TT > 16 && V.page_tokens < TT ? (1u << (TT >> pshift)) - 1u : 1u);
-            const bool tail_tok = tok + TT - 1u > pos_hi || !all;  // tokens that no row of the warp sees, maybe never written
-            const bool masked = tail_tok || tok + TT - 1u > pos_lo || (A.window && pos_hi >= A.window && tok <= pos_hi - A.window);
+            const bool mixed = TT > 16 && V.page_tokens < TT;  // several pages in a tile
+            const bool all = valid == (mixed ? (1u << (TT >> pshift)) - 1u : 1u);
+            tail_tok = __any_sync(0xffffffffu, tok + TT - 1u > pos_hi || !all);  // tokens that no row of the warp sees, maybe never written
+            float k0 = d.ks[0];  // the largest scale of the tile's pages
+            const bool several = TT > 16 && __any_sync(0xffffffffu, mixed);
+            if (several) k0 = fmaxf(fmaxf(k0, d.ks[1]), fmaxf(d.ks[2], d.ks[3]));
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                if constexpr (!WIDE) {
+                    sc[j][0] = (sc[j][0] + sc[j][2]) * (k0 * qc[0]);
+                    sc[j][1] = (sc[j][1] + sc[j][3]) * (k0 * qc[0]);
+                } else {
+                    sc[j][0] *= k0 * qc[0];
+                    sc[j][1] *= k0 * qc[0];
+                    sc[j][2] *= k0 * qc[RW - 1];
+                    sc[j][3] *= k0 * qc[RW - 1];
+                }
+            }
+            vref = d.vs[0];
+            float rvref = 1.f;
+            if (several) {  // scores, and weights before they meet the values, take what another page's scale differs by
+                vref = fmaxf(fmaxf(d.vs[0], d.vs[1]), fmaxf(d.vs[2], d.vs[3]));
+                rvref = vref > 0.f ? 1.0f / vref : 1.f;
+                const float rk0 = k0 > 0.f ? 1.0f / k0 : 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const float f = d.ks[(8u * j) >> pshift] * rk0;
+#pragma unroll
+                    for (int e = 0; e < 2 * RW; e++) sc[j][e] *= f;
+                }
+            }
+            if (__any_sync(0xffffffffu, tail_tok || tok + TT - 1u > pos_lo || (A.window && pos_hi >= A.window && tok <= pos_hi - A.window))) {
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const bool there = (valid >> (mixed ? (8u * j) >> pshift : 0u)) & 1u;
+#pragma unroll
+                    for (int e = 0; e < 2 * RW; e++) {
+                        const uint32_t tk = tok + 8u * j + vr[e & 1], p = pos[e >> 1];
+                        const bool see = tk <= p && (!A.window || p < A.window || tk > p - A.window) && there;
+                        sc[j][e] = see ? sc[j][e] : -INFINITY;
+                    }
+                }
+            }
             float mx[RW];
 #pragma unroll
             for (int i = 0; i < RW; i++) mx[i] = m[i];
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const uint32_t pg = TT > 16 ? (8u * j) >> pshift : 0u;  // (0 where a page is as long as the tile)
-                const float kscale = d.ks[pg];
-                if constexpr (!WIDE) {
-                    sc[j][0] = (sc[j][0] + sc[j][2]) * (kscale * qc[0]);
-                    sc[j][1] = (sc[j][1] + sc[j][3]) * (kscale * qc[0]);
-                } else {
-                    sc[j][0] *= kscale * qc[0];
-                    sc[j][1] *= kscale * qc[0];
-                    sc[j][2] *= kscale * qc[RW - 1];
-                    sc[j][3] *= kscale * qc[RW - 1];
-                }
-                if (masked) {
-#pragma unroll
-                    for (int e = 0; e < 2 * RW; e++) {
-                        const uint32_t tk = tok + 8u * j + 2u * t + (e & 1), p = pos[e >> 1];
-                        const bool see = tk <= p && (!A.window || p < A.window || tk > p - A.window) && ((valid >> pg) & 1u);
-                        if (!see) sc[j][e] = -INFINITY;
-                    }
-                }
+            for (int j = 0; j < NT; j++)
 #pragma unroll
                 for (int e = 0; e < 2 * RW; e++) mx[e >> 1] = fmaxf(mx[e >> 1], sc[j][e]);
-            }
             bool moved = false;
 #pragma unroll
             for (int i = 0; i < RW; i++) {
@@ -609,12 +709,6 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
             float base[RW];
 #pragma unroll
             for (int i = 0; i < RW; i++) base[i] = m[i] == -INFINITY ? 0.f : m[i] - 15.f;  // weights carry 2^15, as their sum does
-            // the largest scale among the tile's value pages; the weights take what another page's scale differs by
-            float vref = d.vs[0];
-            const bool mixed = TT > 16 && V.page_tokens < TT;
-            if (mixed) vref = fmaxf(fmaxf(d.vs[0], d.vs[1]), fmaxf(d.vs[2], d.vs[3]));
-            const float rvref = mixed && vref > 0.f ? 1.0f / vref : 1.f;
-            uint32_t pf[TT / 16][WIDE ? 8 : 4];
 #pragma unroll
             for (int j = 0; j < NT; j++) {
                 float p[2 * RW];
@@ -623,7 +717,7 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
                     p[e] = ex2(sc[j][e] - base[e >> 1]);
                     l[e >> 1] += p[e];
                 }
-                if (mixed) {
+                if (TT > 16 && mixed) {
                     const float f = d.vs[(8u * j) >> pshift] * rvref;
 #pragma unroll
                     for (int e = 0; e < 2 * RW; e++) p[e] *= f;
@@ -636,58 +730,70 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
                     split2(p[2], p[2 * RW - 1], pf[u][hf + 1], pf[u][4 + hf + 1]);
                 }
             }
-            // weighted values: thread (g, t) reads the dimensions g VB.. of the four tokens its weights are for
+        } else {
+            if (wi == 0)
+                while (ds_left > is_left) describe();
+            if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
+            const uint8_t *vs = ring + half * S::HALF;
+            const uint32_t tok = d.tile * TT, valid = d.valid, pshift = V.page_shift;
+            const bool mixed = TT > 16 && V.page_tokens < TT;
+            // weighted values: thread (g, t) reads its output columns of the four tokens its weights are for
 #pragma unroll
             for (int c = 0; c < VL; c++) {
                 uint32_t r[TT / 16][4][VW / 4];
 #pragma unroll
                 for (int u = 0; u < TT / 16; u++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t row = 16u * u + 2u * t + (k & 1) + 8u * (k >> 1);
-                        lds_words<VW>(r[u][k], vs + row * (HD * EL) + g * VB + c * VW);
-                        if (tail_tok && !(tok + row <= pos_hi && ((valid >> (TT > 16 ? row >> pshift : 0u)) & 1u))) {
+                    for (int k = 0; k < 4; k++)
+                        lds_words<VW>(r[u][k], vs + v_off[k & 1] + (S::SWZ ? c * (TT * 128) + (16 * u + 8 * (k >> 1)) * 128
+                                                                            : c * VW + (16 * u + 8 * (k >> 1)) * (HD * EL)));
+                if (__any_sync(0xffffffffu, tail_tok)) {  // what no row sees may hold anything: zeros
 #pragma unroll
-                            for (int w = 0; w < VW / 4; w++) r[u][k][w] = 0u;
+                    for (int u = 0; u < TT / 16; u++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t row = 16u * u + vr[k & 1] + 8u * (k >> 1);
+                            const uint32_t keep = tok + row <= pos_hi && ((valid >> (mixed ? row >> pshift : 0u)) & 1u) ? 0xffffffffu : 0u;
+#pragma unroll
+                            for (int w = 0; w < VW / 4; w++) r[u][k][w] &= keep;
                         }
-                    }
+                }
 #pragma unroll
                 for (int w = 0; w < VW / 4; w++) {
                     constexpr int PER = 4 / EL;  // dimensions of a word
                     float acc[PER][4];
-#pragma unroll
-                    for (int e = 0; e < PER; e++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) acc[e][k] = 0.f;
 #pragma unroll
                     for (int u = 0; u < TT / 16; u++) {
                         uint32_t b0[PER], b1[PER];
                         if constexpr (EL == 1) {
                             const uint32_t a = __byte_perm(r[u][0][w], r[u][1][w], 0x5140), b = __byte_perm(r[u][0][w], r[u][1][w], 0x7362);
                             const uint32_t cc = __byte_perm(r[u][2][w], r[u][3][w], 0x5140), dd = __byte_perm(r[u][2][w], r[u][3][w], 0x7362);
-                            b0[0] = e4m3x2_to_f16x2(a & 0xffffu);
-                            b0[1] = e4m3x2_to_f16x2(a >> 16);
-                            b0[2 % PER] = e4m3x2_to_f16x2(b & 0xffffu);
-                            b0[3 % PER] = e4m3x2_to_f16x2(b >> 16);
-                            b1[0] = e4m3x2_to_f16x2(cc & 0xffffu);
-                            b1[1] = e4m3x2_to_f16x2(cc >> 16);
-                            b1[2 % PER] = e4m3x2_to_f16x2(dd & 0xffffu);
-                            b1[3 % PER] = e4m3x2_to_f16x2(dd >> 16);
+                            e4m3x4_to_f16x2(a, b0[0], b0[1]);
+                            e4m3x4_to_f16x2(b, b0[2 % PER], b0[3 % PER]);
+                            e4m3x4_to_f16x2(cc, b1[0], b1[1]);
+                            e4m3x4_to_f16x2(dd, b1[2 % PER], b1[3 % PER]);
                         } else {
                             b0[0] = __byte_perm(r[u][0][w], r[u][1][w], 0x5410);
                             b0[1] = __byte_perm(r[u][0][w], r[u][1][w], 0x7632);
                             b1[0] = __byte_perm(r[u][2][w], r[u][3][w], 0x5410);
                             b1[1] = __byte_perm(r[u][2][w], r[u][3][w], 0x7632);
                         }
+                        if constexpr (!WIDE) {
+                            const uint32_t(&p)[4] = reinterpret_cast<const uint32_t(&)[4]>(pf[u]);
 #pragma unroll
-                        for (int e = 0; e < PER; e++) {
-                            if constexpr (!WIDE) {
-                                mma_f16(acc[e], reinterpret_cast<const uint32_t(&)[4]>(pf[u]), b0[e], b1[e]);
-                            } else {
-                                const uint32_t hi[4] = {pf[u][0], pf[u][1], pf[u][2], pf[u][3]}, lo[4] = {pf[u][4], pf[u][5], pf[u][6], pf[u][7]};
-                                mma_f16(acc[e], lo, b0[e], b1[e]);
-                                mma_f16(acc[e], hi, b0[e], b1[e]);
+                            for (int e = 0; e < PER; e++) {
+                                if (u == 0) mma_f16_from0(acc[e], p, b0[e], b1[e]);
+                                else mma_f16(acc[e], p, b0[e], b1[e]);
                             }
+                        } else {
+                            const uint32_t hi[4] = {pf[u][0], pf[u][1], pf[u][2], pf[u][3]}, lo[4] = {pf[u][4], pf[u][5], pf[u][6], pf[u][7]};
+#pragma unroll
+                            for (int e = 0; e < PER; e++) {
+                                if (u == 0) mma_f16_from0(acc[e], lo, b0[e], b1[e]);
+                                else mma_f16(acc[e], lo, b0[e], b1[e]);
+                            }
+#pragma unroll
+                            for (int e = 0; e < PER; e++) mma_f16(acc[e], hi, b0[e], b1[e]);
                         }
                     }
 #pragma unroll
@@ -703,14 +809,8 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
                     }
                 }
             }
-            const uint32_t sf = d.seq_first, sr = d.seq_rows, r0 = d.row0, hd_ = d.head;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[worker * stages + stage]);
-            if (++stage == stages) {
-                stage = 0;
-                phase ^= 1u;
-            }
-            if (!(flags & PA_END)) continue;
+            const uint32_t flags = d.flags;
+            if (flags & PA_END) {
             // the segment's end: the row sums of four threads meet
 #pragma unroll
             for (int i = 0; i < RW; i++) {
@@ -720,21 +820,21 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
             if (flags & PA_WHOLE) {
 #pragma unroll
                 for (int i = 0; i < RW; i++) {
-                    const uint32_t r = r0 + wi * S::ROWS + g + 8u * i, tk = r / A.group;
-                    if (r >= sr * A.group) continue;
+                    const uint32_t r = it_row0 + wi * S::ROWS + g + 8u * i, tk = by_group(A, r);
+                    if (r >= it_rows * A.group) continue;
                     const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
-                    float *dst = A.out + (size_t)(sf + tk) * A.ld_out + (size_t)(hd_ * A.group + r - tk * A.group) * HD;
+                    float *dst = A.out + (size_t)(it_first + tk) * A.ld_out + (size_t)(it_head * A.group + r - tk * A.group) * HD;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {  // columns 2 t and 2 t + 1 of the products: dimensions (2 t + e) NO..
-                        float *q = dst + (2u * t + e) * NO;
+                    for (int e = 0; e < 2; e++) {  // columns 2 t and 2 t + 1 of the products
+                        float *q = dst + (2u * t + e) * WD;
                         if (A.vec) {
 #pragma unroll
                             for (int k = 0; k < NO; k += 4)
-                                *reinterpret_cast<float4 *>(q + k) = make_float4(o[k][2 * i + e] * inv, o[k + 1][2 * i + e] * inv,
+                                *reinterpret_cast<float4 *>(q + tile_dim(k)) = make_float4(o[k][2 * i + e] * inv, o[k + 1][2 * i + e] * inv,
                                                                                  o[k + 2][2 * i + e] * inv, o[k + 3][2 * i + e] * inv);
                         } else {
 #pragma unroll
-                            for (int k = 0; k < NO; k++) q[k] = o[k][2 * i + e] * inv;
+                            for (int k = 0; k < NO; k++) q[tile_dim(k)] = o[k][2 * i + e] * inv;
                         }
                     }
                 }
@@ -743,9 +843,9 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
                 for (int i = 0; i < RW; i++) {
                     float *dst = slots + (size_t)(warp * S::ROWS + g + 8u * i) * PS;
 #pragma unroll
-                    for (int k = 0; k < NO; k++) {
-                        dst[2u * t * NO + k] = o[k][2 * i];
-                        dst[(2u * t + 1u) * NO + k] = o[k][2 * i + 1];
+                    for (int k = 0; k < NO; k += 2) {
+                        *reinterpret_cast<float2 *>(dst + 2u * t * WD + tile_dim(k)) = make_float2(o[k][2 * i], o[k + 1][2 * i]);
+                        *reinterpret_cast<float2 *>(dst + (2u * t + 1u) * WD + tile_dim(k)) = make_float2(o[k][2 * i + 1], o[k + 1][2 * i + 1]);
                     }
                     if (t == 0) {
                         dst[HD] = m[i];
@@ -755,21 +855,40 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
             } else {
                 open_tail = true;
             }
+            }
+        }
+        __syncwarp();  // the half is done with
+        if (wm > 1u && lane == 0) mbar_arrive(&empty[half]);
+        if (++half == halves) {
+            half = 0;
+            phase ^= 1u;
+        }
+        }
+        // refill: alone, a warp refills the half it has just used; with others, the one before, which they have mostly left as well
+        if (wi == 0 && is_left && (step < 0 || wm == 1u || step > 0)) {
+            if (step > 0 && wm > 1u) {
+                mbar_wait_bounded(&empty[e_half], e_phase, V.status);
+                if (++e_half == halves) {
+                    e_half = 0;
+                    e_phase ^= 1u;
+                }
+            }
+            issue();
         }
     }
+    report_bad(V, bad);
 
     // ---- parts of items that more than one worker has: tails go where the rings were
     __syncthreads();
     float *tails = reinterpret_cast<float *>(rings);
     if (open_tail) {
-        const uint32_t g = lane >> 2, t = lane & 3u;
 #pragma unroll
         for (int i = 0; i < RW; i++) {
             float *dst = tails + (size_t)(warp * S::ROWS + g + 8u * i) * PS;
 #pragma unroll
-            for (int k = 0; k < NO; k++) {
-                dst[2u * t * NO + k] = o[k][2 * i];
-                dst[(2u * t + 1u) * NO + k] = o[k][2 * i + 1];
+            for (int k = 0; k < NO; k += 2) {
+                *reinterpret_cast<float2 *>(dst + 2u * t * WD + tile_dim(k)) = make_float2(o[k][2 * i], o[k + 1][2 * i]);
+                *reinterpret_cast<float2 *>(dst + (2u * t + 1u) * WD + tile_dim(k)) = make_float2(o[k][2 * i + 1], o[k + 1][2 * i + 1]);
             }
             if (t == 0) {
                 dst[HD] = m[i];
@@ -779,101 +898,139 @@ __global__ void __launch_bounds__((PaShape<HD, TYPE, WIDE>::NW + 1) * 32, 1) pag
     }
     __syncthreads();
     if (n_block == 0u) return;
-    if (warp == NW && lane == 0) range[0] = total, range[1] = blocks;
-    __syncthreads();
-    const uint32_t line = range[0], line_blocks = range[1];
-    constexpr uint32_t THREADS = (NW + 1) * 32;
-
-    // one chain of parts: [tail of worker a,] heads of the workers behind it; `front` / `back`: it goes on in other blocks
-    auto emit = [&](int a_tail, uint32_t h0, uint32_t h1, const PaWorker::Part &it, bool front, bool back) {
-        const uint32_t R = it.seq_rows * A.group;
-        // weight of each part, row by row: 2^(its maximum - the largest)
-        float *slot = A.part + ((size_t)blockIdx.x * 2u + (front ? 0u : 1u)) * rb * PS;
-        for (uint32_t i = threadIdx.x; i < rb * PS; i += THREADS) {
-            const uint32_t row = i / PS, col = i - row * PS;
-            if (it.row0 + row >= R) continue;
-            const float *tp = a_tail >= 0 ? tails + ((size_t)a_tail * rb + row) * PS : nullptr;
-            float M = tp ? tp[HD] : -INFINITY;
-            for (uint32_t w = h0; w < h1; w++) M = info[w].has_head ? fmaxf(M, slots[((size_t)w * rb + row) * PS + HD]) : M;
-            const float b = M == -INFINITY ? 0.f : M;
-            float sum = 0.f, wsum = 0.f;
-            auto add = [&](const float *p) {
-                const float f = ex2(p[HD] - b);
-                sum = fmaf(f, p[col == HD ? 0 : col], sum);
-                wsum = fmaf(f, p[HD + 1], wsum);
-            };
-            if (tp) add(tp);
-            for (uint32_t w = h0; w < h1; w++)
-                if (info[w].has_head) add(slots + ((size_t)w * rb + row) * PS);
-            if (front || back) {
-                __stcg(slot + i, col == HD ? M : col == HD + 1 ? wsum : sum);
-            } else if (col < HD) {
-                const uint32_t r = it.row0 + row, tk = r / A.group;
-                A.out[(size_t)(it.seq_first + tk) * A.ld_out + (size_t)(it.head * A.group + r - tk * A.group) * HD + col] =
-                    wsum == 0.f ? 0.f : sum * (1.0f / wsum);
-            }
-        }
-        if (!front && !back) return;
-        // blocks that have a part: those whose cut lies inside the item, and the one in front of the first such cut
-        const uint32_t i0 = it.item0, i1 = it.item0 + it.item_tiles;
-        const uint32_t c_lo = (uint32_t)(((uint64_t)(i0 + 1u) * line_blocks - 1u) / line);   // block that holds the item's first tile
-        const uint32_t c_hi = (uint32_t)(((uint64_t)i1 * line_blocks - 1u) / line);          // ... and its last
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const uint32_t n = atomicAdd(&A.ticket[c_lo], 1u);
-            last_here = n == c_hi - c_lo;
-            if (last_here) A.ticket[c_lo] = 0u;
-        }
-        __syncthreads();
-        if (!last_here) return;
-        __threadfence();
-        for (uint32_t i = threadIdx.x; i < rb * HD; i += THREADS) {
-            const uint32_t row = i / HD, col = i - row * HD;
-            if (it.row0 + row >= R) continue;
-            auto part = [&](uint32_t c) { return A.part + (((size_t)c * 2u + (c == c_lo ? 1u : 0u)) * rb + row) * PS; };
-            float M = -INFINITY;
-            for (uint32_t c = c_lo; c <= c_hi; c++) M = fmaxf(M, __ldcg(part(c) + HD));
-            const float b = M == -INFINITY ? 0.f : M;
-            float sum = 0.f, wsum = 0.f;
-            for (uint32_t c = c_lo; c <= c_hi; c++) {
-                const float *p = part(c);
-                const float f = ex2(__ldcg(p + HD) - b);
-                sum = fmaf(f, __ldcg(p + col), sum);
-                wsum = fmaf(f, __ldcg(p + HD + 1), wsum);
-            }
-            const uint32_t r = it.row0 + row, tk = r / A.group;
-            A.out[(size_t)(it.seq_first + tk) * A.ld_out + (size_t)(it.head * A.group + r - tk * A.group) * HD + col] =
-                wsum == 0.f ? 0.f : sum * (1.0f / wsum);
-        }
+    // Chains of parts: [the tail of worker a and] heads of the workers behind it up to the one where the item ends. One without a
+    // tail comes from the block in front, one without an end goes on in the next. A warp joins a row at a time.
+    uint32_t heads, ends, tail_set;
+    {
+        const bool on = lane < workers;
+        heads = __ballot_sync(0xffffffffu, on && info[min(lane, workers - 1u)].has_head);
+        ends = __ballot_sync(0xffffffffu, on && info[min(lane, workers - 1u)].head_ended);
+        tail_set = __ballot_sync(0xffffffffu, on && info[min(lane, workers - 1u)].has_tail);
+    }
+    const bool front = heads && (tail_set == 0u || __ffs(heads) <= __ffs(tail_set));
+    const uint32_t chains = __popc(tail_set) + front;
+    auto row_out = [&](const PaWorker::Part &it, uint32_t row) {
+        const uint32_t r = it.row0 + row, tk = by_group(A, r);
+        return A.out + (size_t)(it.seq_first + tk) * A.ld_out + (size_t)(it.head * A.group + r - tk * A.group) * HD;
     };
-    int a_tail = -1;
-    uint32_t h0 = 0;
-    bool open = false, front = false;
-    PaWorker::Part it{};
-    for (uint32_t w = 0; w < workers; w++) {
-        const PaWorker &I = info[w];
-        if (I.has_head) {
-            if (!open) {
-                open = front = true;
-                a_tail = -1;
-                h0 = w;
-                it = I.head;
-            }
-            if (I.head_ended) {
-                emit(a_tail, h0, w + 1u, it, front, false);
-                open = front = false;
-            }
+    constexpr int DL = (HD / 2 + 31) / 32;  // pairs of a row in a lane
+    const PaWorker::Part *cross[2] = {nullptr, nullptr};  // the item that goes on in front, and behind
+    for (uint32_t c = 0, left = tail_set; c < chains; c++) {
+        int a = -1;
+        if (c > 0u || !front) {
+            a = __ffs(left) - 1;
+            left &= left - 1u;
         }
-        if (I.has_tail) {
-            open = true;
-            front = false;
-            a_tail = (int)w;
-            h0 = w + 1u;
-            it = I.tail;
+        const uint32_t behind = a < 0 ? 0xffffffffu : a == 31 ? 0u : ~0u << (a + 1);
+        const uint32_t stop = ends & behind;
+        const uint32_t members = heads & behind & (stop ? (stop & -stop) | ((stop & -stop) - 1u) : 0xffffffffu);
+        const PaWorker::Part &it = a < 0 ? info[__ffs(members) - 1].head : info[a].tail;
+        const bool out = a < 0 || stop == 0u;
+        if (out) cross[a < 0 ? 0 : 1] = &it;
+        const uint32_t R = min(rb, it.seq_rows * A.group - it.row0);
+        for (uint32_t row = (warp + NW - c % NW) % NW; row < R; row += NW) {
+            const bool tl = (int)lane == a, mine = tl || ((members >> lane) & 1u);
+            const float *p = (tl ? tails : slots) + (size_t)((mine ? lane : 0u) * rb + row) * PS;
+            const float pm = mine ? p[HD] : -INFINITY;
+            float M = pm;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+            const float f = pm == -INFINITY ? 0.f : ex2(pm - M);
+            const float L = warp_sum(mine ? f * p[HD + 1] : 0.f);
+            float2 acc[DL];
+#pragma unroll
+            for (int k = 0; k < DL; k++) acc[k] = make_float2(0.f, 0.f);
+            for (uint32_t set = members | (a >= 0 ? 1u << a : 0u); set; set &= set - 1u) {
+                const uint32_t w = __ffs(set) - 1u;
+                const float fw = __shfl_sync(0xffffffffu, f, w);
+                const float2 *src = reinterpret_cast<const float2 *>(((int)w == a ? tails : slots) + (size_t)(w * rb + row) * PS);
+#pragma unroll
+                for (int k = 0; k < DL; k++)
+                    if (k * 32 + lane < HD / 2) {
+                        const float2 v = src[k * 32 + lane];
+                        acc[k].x = fmaf(fw, v.x, acc[k].x);
+                        acc[k].y = fmaf(fw, v.y, acc[k].y);
+                    }
+            }
+            if (out) {
+                float *dst = A.part + (((size_t)blockIdx.x * 2u + (a < 0 ? 0u : 1u)) * rb + row) * PS;
+#pragma unroll
+                for (int k = 0; k < DL; k++)
+                    if (k * 32 + lane < HD / 2) __stcg(reinterpret_cast<float2 *>(dst) + k * 32 + lane, acc[k]);
+                if (lane == 0) __stcg(reinterpret_cast<float2 *>(dst + HD), make_float2(M, L));
+            } else {
+                const float inv = L == 0.f ? 0.f : 1.0f / L;
+                float *dst = row_out(it, row);
+#pragma unroll
+                for (int k = 0; k < DL; k++)
+                    if (k * 32 + lane < HD / 2) {
+                        dst[2 * (k * 32 + lane)] = acc[k].x * inv;
+                        dst[2 * (k * 32 + lane) + 1] = acc[k].y * inv;
+                    }
+            }
         }
     }
-    if (open) emit(a_tail, h0, workers, it, front, true);
+    if (!cross[0] && !cross[1]) return;
+    // ---- items that several blocks have: the last of them to come here joins their parts
+    const PaCuts line(total, line_blocks);
+    __threadfence();
+    __syncthreads();
+    if (warp < 2u && lane == 0) {
+        last_here[warp] = 0u;
+        if (const PaWorker::Part *it = cross[warp]) {
+            const uint32_t lo = line.part_of(it->item0), hi = line.part_of(it->item0 + it->item_tiles - 1u);
+            if (atomicAdd(&A.ticket[lo], 1u) == hi - lo) {
+                A.ticket[lo] = 0u;
+                last_here[warp] = 1u;
+            }
+        }
+    }
+    __syncthreads();
+    for (int e = 0; e < 2; e++) {
+        if (!last_here[e]) continue;
+        __threadfence();
+        const PaWorker::Part &it = *cross[e];
+        const uint32_t lo = line.part_of(it.item0), n = line.part_of(it.item0 + it.item_tiles - 1u) - lo + 1u;
+        const uint32_t R = min(rb, it.seq_rows * A.group - it.row0);
+        for (uint32_t row = warp; row < R; row += NW) {
+            auto part = [&](uint32_t i) { return A.part + (((size_t)(lo + i) * 2u + (i == 0u ? 1u : 0u)) * rb + row) * PS; };
+            float M = -INFINITY, L = 0.f;
+            for (uint32_t i = lane; i < n; i += 32u) M = fmaxf(M, __ldcg(part(i) + HD));
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+            float2 acc[DL];
+#pragma unroll
+            for (int k = 0; k < DL; k++) acc[k] = make_float2(0.f, 0.f);
+            for (uint32_t base = 0; base < n; base += 32u) {
+                const uint32_t cnt = min(32u, n - base);
+                float2 ml = make_float2(-INFINITY, 0.f);
+                if (lane < cnt) ml = __ldcg(reinterpret_cast<const float2 *>(part(base + lane) + HD));
+                const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+                L += f * ml.y;
+#pragma unroll 4
+                for (uint32_t i = 0; i < cnt; i++) {
+                    const float fw = __shfl_sync(0xffffffffu, f, i);
+                    const float2 *src = reinterpret_cast<const float2 *>(part(base + i));
+#pragma unroll
+                    for (int k = 0; k < DL; k++)
+                        if (k * 32 + lane < HD / 2) {
+                            const float2 v = __ldcg(src + k * 32 + lane);
+                            acc[k].x = fmaf(fw, v.x, acc[k].x);
+                            acc[k].y = fmaf(fw, v.y, acc[k].y);
+                        }
+                }
+            }
+            L = warp_sum(L);
+            const float inv = L == 0.f ? 0.f : 1.0f / L;
+            float *dst = row_out(it, row);
+#pragma unroll
+            for (int k = 0; k < DL; k++)
+                if (k * 32 + lane < HD / 2) {
+                    dst[2 * (k * 32 + lane)] = acc[k].x * inv;
+                    dst[2 * (k * 32 + lane) + 1] = acc[k].y * inv;
+                }
+        }
+    }
 }
 
 // Blocks that the launch may have: one on each SM.
@@ -883,12 +1040,10 @@ static uint32_t attn_blocks(const strix_cuda *h) { return (uint32_t)std::min<int
 // 16 rows a warp and as many warps to a worker as cover them (at most all of a block).
 static void attn_form(const PagedView &V, uint32_t group, bool &wide, uint32_t &wm) {
     const uint64_t rows = ((uint64_t)V.n_rows * group + V.n_seq - 1) / std::max(V.n_seq, 1u);
-    const bool f16 = V.type == STRIX_KV_F16;
     wide = rows > 8;
     const uint32_t most = V.head_dim >= 192 ? 4u : 8u;
     wm = 1;
     while (wide && wm < most && 16ull * wm < rows) wm *= 2;
-    if (wide && V.head_dim >= 192 && f16 && wm < 2) wm = 2;  // (the rings of four workers do not fit)
 }
 
 static size_t attn_work_bytes(const strix_cuda *h, const PagedView &V, uint32_t group) {
@@ -900,17 +1055,52 @@ static size_t attn_work_bytes(const strix_cuda *h, const PagedView &V, uint32_t 
     return (PA_MAX_BLOCKS * 4 + part + 255) & ~(size_t)255;
 }
 
+typedef CUresult (*AttnEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static AttnEncodeFn attn_encode_fn() {
+    static AttnEncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<AttnEncodeFn>(p);
+    }();
+    return fn;
+}
+// A cache as [page][KV head and slot][element], copied in boxes of `rows` slots by `box` elements.
+static bool attn_map(CUtensorMap *map, const PagedView &V, void *base, uint32_t box, uint32_t rows, bool swizzled) {
+    AttnEncodeFn fn = attn_encode_fn();
+    if (!fn) return false;
+    const bool f16 = V.type == STRIX_KV_F16;
+    const cuuint64_t dims[3] = {V.head_dim, (cuuint64_t)V.n_kv * V.page_tokens, V.n_pages};
+    const cuuint64_t strides[2] = {(cuuint64_t)V.head_dim * (f16 ? 2 : 1), V.page_bytes};
+    const cuuint32_t boxes[3] = {box, rows, 1}, one[3] = {1, 1, 1};
+    return fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, boxes, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int HD, int TYPE, bool WIDE>
 static cudaError_t attn_launch(const strix_cuda *h, PagedAttnArgs &A, cudaStream_t stream) {
     using S = PaShape<HD, TYPE, WIDE>;
     const int workers = S::NW / (int)A.wm;
-    const int stages = S::stages_for((int)A.wm, h->smem_optin - PA_STATIC);
-    const size_t smem = (size_t)workers * stages * S::STAGE + S::fixed(workers, stages);
-    if (smem + PA_STATIC > h->smem_optin || (size_t)stages * S::STAGE < (size_t)S::ROWS * A.wm * S::PSTRIDE * 4) return cudaErrorInvalidConfiguration;
-    cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<HD, TYPE, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    A.stages = (uint32_t)stages;
-    paged_attn_kernel<HD, TYPE, WIDE><<<attn_blocks(h), (S::NW + 1) * 32, smem, stream>>>(A);
+    const int halves = S::halves_for((int)A.wm, h->smem_optin - PA_STATIC);
+    const size_t smem = S::rings(workers, halves) + S::fixed(workers, halves) + 1024;
+    if (halves < 2 || smem + PA_STATIC - 1024 > h->smem_optin) return cudaErrorInvalidConfiguration;
+    const uint32_t sub = std::min<uint32_t>(S::TT, A.V.page_tokens);
+    if (!attn_map(&A.k_map, A.V, A.V.k, S::BOXB / S::EL, sub, S::SWZ) || !attn_map(&A.v_map, A.V, A.V.v, S::BOXB / S::EL, sub, S::SWZ))
+        return cudaErrorInvalidValue;
+    static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic shared memory is raised for this kernel
+    const uint64_t bit = 1ull << (h->device & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<HD, TYPE, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)(h->smem_optin - 512));
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    A.halves = (uint32_t)halves;
+    paged_attn_kernel<HD, TYPE, WIDE><<<attn_blocks(h), S::NW * 32, smem, stream>>>(A);
     return cudaGetLastError();
 }
 
@@ -922,6 +1112,7 @@ static int attn_check(strix_cuda *h, const char *who, const strix_kv_pages *cach
     const int rc = serve_check(h, who, cache, batch, &V);
     if (rc != 1) return rc;
     if (n_heads == 0 || n_heads > 65535u || n_heads % V.n_kv) return 0;
+    if (V.n_seq > PA_MAX_SEQ) return serve_fail(h, who, "at most 8192 sequences in one call");
     // the line of tiles is counted in 31 bits
     const uint64_t rb = 8, group = n_heads / V.n_kv;
     const uint64_t blocks = ((uint64_t)V.n_rows * group + rb - 1) / rb + V.n_seq, tiles = (uint64_t)V.pages_ld * V.page_tokens / 16 + 1;
@@ -957,6 +1148,8 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     if (!d_q || !d_out) return serve_fail(h, who, "d_q or d_out missing");
     if (!d_work || (reinterpret_cast<uintptr_t>(d_work) & 255u)) return serve_fail(h, who, "d_work must be 256-byte aligned");
     A.group = n_heads / A.V.n_kv;
+    while ((1u << A.g_shift) < A.group) A.g_shift++;
+    A.g_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << A.g_shift) - A.group)) / A.group + 1u);
     if (work_bytes < attn_work_bytes(h, A.V, A.group)) return serve_fail(h, who, "work_bytes too small");
     A.q = d_q;
     A.out = d_out;
