@@ -21,7 +21,7 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <algorithm>
+#include <atomic>
 
 #include "kv_pages.cuh"
 
@@ -31,11 +31,11 @@ namespace strix {
 
 typedef unsigned long long u64;
 
-constexpr int SAMPLE_THREADS = 1024;
+constexpr int SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr uint32_t SAMPLE_BINS = 2048, SAMPLE_CAP = 2048;
+constexpr int SAMPLE_BPT = SAMPLE_BINS / SAMPLE_THREADS;  // bins, or list entries, of a thread
 constexpr float SAMPLE_ORDERS = 41.f;       // weights below 2^-41 round to no step of 2^-40
-constexpr float SAMPLE_DELTA = 0.008f;      // half a bin: 41 ln 2 / 2047 / 2 = 0.0069, and f32 sums over 2048 bins
-constexpr uint32_t SAMPLE_MAX_CLUSTER = 16;
+constexpr float SAMPLE_DELTA = 0.008f;      // half a bin: 41 ln 2 / 2048 / 2 = 0.0069, and f32 sums over 2048 bins
 
 struct SampleArgs {
     const float *x;
@@ -56,7 +56,7 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
 __device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct SampleShared {
-    uint32_t hist[SAMPLE_BINS];
+    uint32_t hist[SAMPLE_BINS / 2];  // two counts to a word: a block has fewer than 2^16 logits
     union {
         struct {
             u64 mass[SAMPLE_BINS];
@@ -67,67 +67,118 @@ struct SampleShared {
             u64 sorted[SAMPLE_CAP / 2];
         } list;
     };
-    u64 warp_sum[SAMPLE_THREADS / 32];
-    u64 xch[2][4];                  // what the cluster's blocks tell each other, in turns
-    uint32_t n_list, first, second, rank[256];
+    u64 ws[2][2][SAMPLE_WARPS];     // sums of the warps, in turns
+    float wf[SAMPLE_WARPS];
+    u64 xch[2][2];                  // what the cluster's blocks tell each other, in turns
+    uint32_t n_list, first, second, fmax, rank[256];
     u64 found[2];
-    float fred[SAMPLE_THREADS / 32];
 };
-
 static_assert(sizeof(SampleShared) % 16 == 0, "the logits behind it are read in 16-byte words");
 
-// One block's view of its row.
+struct OpAdd {
+    __device__ u64 operator()(u64 p, u64 q) const { return p + q; }
+};
+struct OpMin {
+    __device__ u64 operator()(u64 p, u64 q) const { return p < q ? p : q; }
+};
+struct OpMax {
+    __device__ u64 operator()(u64 p, u64 q) const { return p > q ? p : q; }
+};
+
+// f(logit, its place in the block) for every logit of a thread's stretch; the loads of eight go ahead of their use
+template <typename F>
+__device__ __forceinline__ void each_logit(const float *xs, uint32_t i0, uint32_t i1, F f) {
+    uint32_t i = i0;
+    for (; i + 8u <= i1; i += 8u) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = xs[i + j];
+#pragma unroll
+        for (int j = 0; j < 8; j++) f(v[j], i + j);
+    }
+    for (; i < i1; i++) f(xs[i], i);
+}
+
+// One block's view of its row, which C blocks share. Two rules keep the cluster together: what a block shows to the others
+// (hist, fine, list, xch, found, fmax) is not written again before a cluster barrier behind their reads, and every branch
+// that a barrier depends on is taken on values that all blocks compute from the same data in the same order.
+template <int C>
 struct SampleRow {
     SampleShared &S;
-    const float *xs;               // this block's logits
-    uint32_t cnt, base, seg, i0, i1;  // how many, index of the first; this thread's stretch (an odd length: no bank conflicts)
-    float m, c, min_p;
-    uint32_t turn;
-    cg::cluster_group cl;
+    const float *xs;                // this block's logits
+    uint32_t base, i0, i1;          // index of the first; this thread's stretch (of an odd length: no bank conflicts)
+    float m, c, cb, min_p;          // maximum; log2(e) / T; bins to a unit of logit
+    uint32_t turn, wturn;
 
-    __device__ float order(float x) const {  // log2 of the weight
-        return x == m ? 0.f : m == INFINITY || !(x > -INFINITY) ? -INFINITY : (x - m) * c;
+    __device__ static uint32_t me() { return C > 1 ? cg::this_cluster().block_rank() : 0u; }
+    __device__ static void csync() {
+        if constexpr (C > 1) cg::this_cluster().sync();
+        else __syncthreads();
     }
-    __device__ static u64 steps(float y) { return y < -SAMPLE_ORDERS ? 0ull : __float2ull_rn(exp2f(y) * 1099511627776.f); }
-    __device__ static uint32_t bin(float y) {  // SAMPLE_BINS = no weight
-        return y < -SAMPLE_ORDERS ? SAMPLE_BINS : (uint32_t)(y * -((float)(SAMPLE_BINS - 1u) / SAMPLE_ORDERS));
+    template <typename T>
+    __device__ static T far(const T *p, uint32_t r) {
+        if constexpr (C > 1) return *cg::this_cluster().map_shared_rank(p, r);
+        else return *p;
     }
+    // log2 of a weight: NaN or far below -SAMPLE_ORDERS where there is none
+    __device__ float order(float x) const { return (x - m) * c; }
+    __device__ static bool weighs(float y) { return y >= -SAMPLE_ORDERS; }
+    // the weight in steps of 2^-40 (rounded to nearest), as units of 2^20 and the rest
+    __device__ static void split(float y, uint32_t &hi, uint32_t &lo) {
+        const float w = exp2f(y) * 1048576.f, h = __fadd_rd(w, 8388608.f);
+        hi = __float_as_uint(h) & 0x7fffffu;
+        lo = __float_as_uint(fmaf(w - (h - 8388608.f), 1048576.f, 8388608.f)) & 0x7fffffu;
+    }
+    __device__ static u64 steps(float y) {
+        if (!weighs(y)) return 0ull;
+        uint32_t hi, lo;
+        split(y, hi, lo);
+        return ((u64)hi << 20) + lo;
+    }
+    // place in the histogram, a number below SAMPLE_BINS where there is weight
+    __device__ float bin_of(float x) const { return (m - x) * cb; }
+    __device__ static uint32_t bin(float b) { return __float_as_uint(__fadd_rd(b, 8388608.f)) & 0x7fffffu; }
 
-    // Sums (or with op a maximum / minimum) of up to four values over the block, then over the cluster; all threads get them.
+    // folds up to two values over the cluster
     template <int N, typename F>
-    __device__ void block_fold(u64 (&v)[N], F op) {
+    __device__ void fold(u64 (&v)[N], F op) {
+        u64(&ws)[2][SAMPLE_WARPS] = S.ws[wturn];
+        wturn ^= 1u;
+        const uint32_t lane = threadIdx.x & 31u;
 #pragma unroll
         for (int k = 0; k < N; k++) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) v[k] = op(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
-            __syncthreads();
-            if ((threadIdx.x & 31u) == 0) S.warp_sum[threadIdx.x >> 5] = v[k];
-            __syncthreads();
-            v[k] = S.warp_sum[threadIdx.x & 31u];
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v[k] = op(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
+            if (lane == 0) ws[k][threadIdx.x >> 5] = v[k];
         }
-    }
-    template <int N, typename F>
-    __device__ void fold(u64 (&v)[N], F op) {
-        block_fold(v, op);
-        if (threadIdx.x == 0)
-            for (int k = 0; k < N; k++) S.xch[turn][k] = v[k];
-        cl.sync();
-        for (int k = 0; k < N; k++)
-            for (uint32_t r = 0; r < cl.num_blocks(); r++) {
-                const u64 w = *cl.map_shared_rank(&S.xch[turn][k], r);
-                v[k] = r ? op(v[k], w) : w;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            v[k] = ws[k][lane & (SAMPLE_WARPS - 1)];
+#pragma unroll
+            for (int o = SAMPLE_WARPS / 2; o > 0; o >>= 1) v[k] = op(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
+            if (C > 1 && threadIdx.x == 0) S.xch[turn][k] = v[k];
+        }
+        if constexpr (C > 1) {
+            csync();
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                v[k] = far(&S.xch[turn][k], lane & (C - 1));
+#pragma unroll
+                for (int o = C / 2; o > 0; o >>= 1) v[k] = op(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
             }
-        turn ^= 1u;
+            turn ^= 1u;
+        }
     }
     __device__ u64 sum(u64 v) {
         u64 a[1] = {v};
-        fold(a, [](u64 p, u64 q) { return p + q; });
+        fold(a, OpAdd());
         return a[0];
     }
-    // this thread's place in the block: the sum over the threads before it, and over all
+    // the sum over the block's threads before this one, and over all
     __device__ u64 before(u64 v, u64 &all) {
+        u64 *ws = S.ws[wturn][0];
+        wturn ^= 1u;
         const uint32_t lane = threadIdx.x & 31u, w = threadIdx.x >> 5;
         u64 incl = v;
 #pragma unroll
@@ -135,32 +186,39 @@ struct SampleRow {
             const u64 p = __shfl_up_sync(0xffffffffu, incl, o);
             if ((int)lane >= o) incl += p;
         }
+        if (lane == 31u) ws[w] = incl;
         __syncthreads();
-        if (lane == 31u) S.warp_sum[w] = incl;
-        __syncthreads();
-        u64 ws = S.warp_sum[lane];
-        u64 wi = ws;
+        const u64 mine = ws[lane & (SAMPLE_WARPS - 1)];
+        u64 wi = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
+        for (int o = 1; o < SAMPLE_WARPS; o <<= 1) {
             const u64 p = __shfl_up_sync(0xffffffffu, wi, o);
-            if ((int)lane >= o) wi += p;
+            if ((int)(lane & (SAMPLE_WARPS - 1)) >= o) wi += p;
         }
-        all = __shfl_sync(0xffffffffu, wi, 31);
-        return __shfl_sync(0xffffffffu, wi - ws, w) + incl - v;
+        all = __shfl_sync(0xffffffffu, wi, SAMPLE_WARPS - 1);
+        return __shfl_sync(0xffffffffu, wi - mine, w) + incl - v;
     }
-    // the same over the cluster's blocks, in rank order
+    // the same over the cluster, blocks in rank order
     __device__ u64 before_all(u64 v, u64 &all) {
         u64 mine;
         u64 b = before(v, mine);
-        if (threadIdx.x == 0) S.xch[turn][0] = mine;
-        cl.sync();
-        all = 0;
-        for (uint32_t r = 0; r < cl.num_blocks(); r++) {
-            const u64 w = *cl.map_shared_rank(&S.xch[turn][0], r);
-            if (r < cl.block_rank()) b += w;
-            all += w;
+        if constexpr (C > 1) {
+            if (threadIdx.x == 0) S.xch[turn][0] = mine;
+            csync();
+            const uint32_t lane = threadIdx.x & 31u, r = me();
+            const u64 w = lane < C ? far(&S.xch[turn][0], lane & (C - 1)) : 0ull;
+            u64 a = w, l = lane < r ? w : 0ull;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                a += __shfl_xor_sync(0xffffffffu, a, o);
+                l += __shfl_xor_sync(0xffffffffu, l, o);
+            }
+            all = a;
+            b += l;
+            turn ^= 1u;
+        } else {
+            all = mine;
         }
-        turn ^= 1u;
         return b;
     }
 
@@ -192,8 +250,8 @@ struct SampleRow {
         __syncthreads();
         for (uint32_t k = 2; k <= np; k *= 2)
             for (uint32_t j = k / 2; j > 0; j /= 2) {
-                if (t < np / 2) {
-                    const uint32_t a = 2 * t - (t & (j - 1u)), b = a + j;
+                for (uint32_t h = t; h < np / 2; h += SAMPLE_THREADS) {
+                    const uint32_t a = 2 * h - (h & (j - 1u)), b = a + j;
                     const u64 p = S.list.e[a], q = S.list.e[b];
                     if ((p > q) == ((a & k) == 0u)) {
                         S.list.e[a] = q;
@@ -203,30 +261,42 @@ struct SampleRow {
                 __syncthreads();
             }
     }
-    // Gathers the tokens that `want` names, from all blocks, into rank 0's list: (descending key, index). Ends behind a cluster
-    // barrier after which only rank 0 has the list; the others' lists stay until the next barrier.
+    // Puts the tokens that `want` names into this block's list (descending key, index), ends behind a cluster barrier, and
+    // brings the other blocks' lists into rank 0's. Returns how many there are (to rank 0 only). `told` is what the block
+    // tells the others by the same barrier: their sum comes back through it.
     template <typename F>
-    __device__ uint32_t gather(F want) {
-        __syncthreads();
-        if (threadIdx.x == 0) S.n_list = 0u;
-        __syncthreads();
-        for (uint32_t i = i0; i < i1; i++) {
-            const float x = xs[i];
-            if (!want(x)) continue;
+    __device__ uint32_t gather(F want, u64 &told) {
+        each_logit(xs, i0, i1, [&](float x, uint32_t i) {
+            if (!want(x, base + i)) return;
             const uint32_t at = atomicAdd(&S.n_list, 1u);
             if (at < SAMPLE_CAP) S.list.e[at] = (u64)(~logit_key(x)) << 32 | (base + i);
-        }
-        cl.sync();
-        uint32_t n = S.n_list;
-        if (cl.block_rank() == 0) {
-            for (uint32_t r = 1; r < cl.num_blocks(); r++) {
-                const uint32_t k = *cl.map_shared_rank(&S.n_list, r);
-                const u64 *src = cl.map_shared_rank(&S.list.e[0], r);
-                for (uint32_t i = threadIdx.x; i < k && n + i < SAMPLE_CAP; i += SAMPLE_THREADS) S.list.e[n + i] = src[i];
-                n += k;
+        });
+        if (threadIdx.x == 0) S.xch[turn][0] = told;
+        csync();
+        uint32_t n = min(S.n_list, SAMPLE_CAP);
+        if constexpr (C > 1) {
+            if (me() == 0) {
+                const uint32_t lane = threadIdx.x & 31u, w = threadIdx.x >> 5, r = w & (C - 1), part = w / C;
+                const uint32_t k = far(&S.n_list, lane & (C - 1));
+                told = far(&S.xch[turn][0], lane & (C - 1));
+                uint32_t upto = k;
+#pragma unroll
+                for (int o = 1; o < C; o <<= 1) {
+                    const uint32_t p = __shfl_up_sync(0xffffffffu, upto, o);
+                    if ((int)(lane & (C - 1)) >= o) upto += p;
+                }
+#pragma unroll
+                for (int o = C / 2; o > 0; o >>= 1) told += __shfl_xor_sync(0xffffffffu, told, o);
+                n = __shfl_sync(0xffffffffu, upto, C - 1);
+                const uint32_t kr = __shfl_sync(0xffffffffu, k, r), at = __shfl_sync(0xffffffffu, upto, r) - kr;
+                if (r > 0u) {
+                    const u64 *src = cg::this_cluster().map_shared_rank(&S.list.e[0], r);
+                    for (uint32_t i = part * 32u + lane; i < kr && at + i < SAMPLE_CAP; i += (SAMPLE_WARPS / C) * 32u) S.list.e[at + i] = src[i];
+                }
+                n = min(n, SAMPLE_CAP);
+                __syncthreads();
             }
-            n = min(n, SAMPLE_CAP);
-            __syncthreads();
+            turn ^= 1u;
         }
         return n;
     }
@@ -238,18 +308,19 @@ struct Cut {
     __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
 };
 
-__global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs A) {
+template <int C>
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs A) {
+    using Row = SampleRow<C>;
     extern __shared__ __align__(16) uint8_t raw[];
     SampleShared &S = *reinterpret_cast<SampleShared *>(raw);
     float *xs = reinterpret_cast<float *>(raw + sizeof(SampleShared));
-    cg::cluster_group cl = cg::this_cluster();
-    const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), t = threadIdx.x, row = blockIdx.x / C;
+    const uint32_t rank = Row::me(), t = threadIdx.x, lane = t & 31u, row = blockIdx.x / C;
     const uint32_t base = min(A.n, rank * A.per), cnt = min(A.n, base + A.per) - base;
     const float *x = A.x + (size_t)row * A.stride + base;
     const float temp = A.p.d_temperature ? A.p.d_temperature[row] : 1.f;
     const int top_k = A.p.d_top_k ? A.p.d_top_k[row] : 0;
-    const float top_p = A.p.d_top_p ? A.p.d_top_p[row] : 1.f;
-    float u = A.u[row];
+    const float top_p = A.p.d_top_p ? A.p.d_top_p[row] : 1.f, min_p = A.p.d_min_p ? A.p.d_min_p[row] : 0.f;
+    const float u = A.u[row];
     const bool greedy = !(temp > 0.f);
 
     // the row into shared memory, its maximum
@@ -258,7 +329,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
         const uint32_t n4 = cnt / 4;
         const float4 *x4 = reinterpret_cast<const float4 *>(x);
         float4 *s4 = reinterpret_cast<float4 *>(xs);
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t i = t; i < n4; i += SAMPLE_THREADS) {
             const float4 v = __ldcs(x4 + i);
             s4[i] = v;
@@ -277,36 +348,46 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
             m = fmaxf(m, v);
         }
     }
-    for (uint32_t i = t; i < SAMPLE_BINS; i += SAMPLE_THREADS) S.hist[i] = 0u;
+    for (uint32_t i = t; i < SAMPLE_BINS / 2; i += SAMPLE_THREADS) S.hist[i] = 0u;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((t & 31u) == 0) S.fred[t >> 5] = m;
+    if (lane == 0) S.wf[t >> 5] = m;
+    if (t == 0) {
+        S.n_list = 0u;
+        S.first = S.second = SAMPLE_BINS - 1u;
+    }
     __syncthreads();
-    m = S.fred[t & 31u];
+    m = S.wf[lane & (SAMPLE_WARPS - 1)];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (t == 0) S.xch[1][0] = __float_as_uint(m);
-    cl.sync();
-    for (uint32_t r = 0; r < C; r++) m = fmaxf(m, __uint_as_float((uint32_t)*cl.map_shared_rank(&S.xch[1][0], r)));
-    const uint32_t seg = ((cnt + SAMPLE_THREADS - 1) / SAMPLE_THREADS) | 1u, i0 = min(cnt, t * seg);
-    SampleRow R{S, xs, cnt, base, seg, i0, min(cnt, i0 + seg), m, 1.4426950408889634f / temp, A.p.d_min_p ? A.p.d_min_p[row] : 0.f, 0u, cl};
-    const uint32_t i1 = R.i1;
-    if (greedy) R.c = INFINITY;  // nothing but the maximum has weight
+    for (int o = SAMPLE_WARPS / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if constexpr (C > 1) {
+        if (t == 0) S.fmax = __float_as_uint(m);
+        Row::csync();
+        m = __uint_as_float(Row::far(&S.fmax, lane & (C - 1)));
+#pragma unroll
+        for (int o = C / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
+    const uint32_t seg = ((cnt + SAMPLE_THREADS - 1) / SAMPLE_THREADS) | 1u, i0 = min(cnt, t * seg), i1 = min(cnt, i0 + seg);
+    if (m == INFINITY) {  // only the infinite ones have weight: as if they were the only ones
+        for (uint32_t i = i0; i < i1; i++) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
+        m = 0.f;
+    }
+    const float c = fminf(1.4426950408889634f / temp, 1.0e36f);
+    Row R{S, xs, base, i0, i1, m, c, c * (SAMPLE_BINS / SAMPLE_ORDERS), min_p, 0u, 0u};
 
     if (m == -INFINITY || greedy) {  // no token, or the first of the largest
         u64 best[1] = {0xffffffffull};
         if (m > -INFINITY)
             for (uint32_t i = i1; i-- > i0;)
                 if (xs[i] == m) best[0] = base + i;
-        R.fold(best, [](u64 p, u64 q) { return p < q ? p : q; });
+        R.fold(best, OpMin());
         if (rank == 0 && t == 0) {
             A.ids[row] = m > -INFINITY ? (uint32_t)best[0] : 0u;
             if (A.probs) A.probs[row] = m > -INFINITY ? 1.f : 0.f;
         }
-        cl.sync();  // (nobody leaves while others read its shared memory)
+        Row::csync();  // (nobody leaves while others read its shared memory)
         return;
     }
-    auto add = [](u64 p, u64 q) { return p + q; };
     auto write = [&](uint32_t id, u64 w, u64 total) {
         A.ids[row] = id;
         if (A.probs) A.probs[row] = (float)((double)w / (double)total);
@@ -320,109 +401,234 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
     const bool nucleus = top_p < 1.f;
     if ((top_k > 0 && (uint32_t)top_k < A.n) || nucleus) {
         // ---- histogram of log2 weight
-        for (uint32_t i = i0; i < i1; i++) {
-            const uint32_t b = R.bin(R.order(xs[i]));
-            if (b < SAMPLE_BINS) atomicAdd(&S.hist[b], 1u);
+        each_logit(xs, i0, i1, [&](float v, uint32_t) {
+            const float b = R.bin_of(v);
+            if (b < (float)SAMPLE_BINS) {
+                const uint32_t k = Row::bin(b);
+                atomicAdd(&S.hist[k / 2u], 1u << (k % 2u * 16u));
+            }
+        });
+        Row::csync();
+        // a thread's bins: counts and middle masses up to each (f32 sums in a fixed order: they only bound)
+        uint32_t h[SAMPLE_BPT] = {};
+#pragma unroll
+        for (int r = 0; r < C; r++) {
+            const uint2 q = Row::far(reinterpret_cast<const uint2 *>(&S.hist[0]) + t, r);
+            h[0] += q.x & 0xffffu;
+            h[1] += q.x >> 16;
+            h[2] += q.y & 0xffffu;
+            h[3] += q.y >> 16;
         }
-        cl.sync();
-        // thread t: bins 2 t and 2 t + 1 over the cluster; counts and middle masses up to each
-        uint32_t h0 = 0, h1 = 0;
-        for (uint32_t r = 0; r < C; r++) {
-            const uint2 h = reinterpret_cast<const uint2 *>(cl.map_shared_rank(&S.hist[0], r))[t];
-            h0 += h.x;
-            h1 += h.y;
+        uint32_t cc[SAMPLE_BPT];
+        float sm[SAMPLE_BPT];
+        const float mid = SAMPLE_ORDERS / SAMPLE_BINS;
+        uint32_t n_weight, c_all = 0;
+        float a_total, s_all = 0.f;
+#pragma unroll
+        for (int j = 0; j < SAMPLE_BPT; j++) {
+            c_all += h[j];
+            s_all = fmaf((float)h[j], exp2f(-((float)(SAMPLE_BPT * t + j) + 0.5f) * mid), s_all);
+            cc[j] = c_all;
+            sm[j] = s_all;
         }
-        u64 n_weight;
-        const u64 c_before = R.before(h0 + h1, n_weight), c0 = c_before + h0, c1 = c0 + h1;
-        const float mid = SAMPLE_ORDERS / (SAMPLE_BINS - 1u);
-        const float a0 = (float)h0 * exp2f(-(2.f * t + 0.5f) * mid), a1 = (float)h1 * exp2f(-(2.f * t + 1.5f) * mid);
-        // (in steps of 2^-32: at least 2^18 tokens of weight 1 fit, and smaller ones do not count here)
-        u64 a_total;
-        const u64 a_before = R.before((u64)__float2ull_rn(a0 * 4294967296.f) + (u64)__float2ull_rn(a1 * 4294967296.f), a_total);
-        const double s0 = (double)(a_before + (u64)__float2ull_rn(a0 * 4294967296.f)),
-                     s1 = s0 + (double)(u64)__float2ull_rn(a1 * 4294967296.f);
-        const bool by_k = top_k > 0 && (u64)top_k < n_weight;
-        const u64 k = by_k ? (u64)top_k : n_weight;
-        // S.first: bin of the k-th token; S.second: the last bin that may matter
-        if (t == 0) S.first = S.second = SAMPLE_BINS - 1u;
+        {
+            uint32_t ci = c_all;
+            float si = s_all;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t p = __shfl_up_sync(0xffffffffu, ci, o);
+                const float q = __shfl_up_sync(0xffffffffu, si, o);
+                if ((int)lane >= o) {
+                    ci += p;
+                    si += q;
+                }
+            }
+            u64 *ws = S.ws[R.wturn][0];
+            R.wturn ^= 1u;
+            if (lane == 31u) {
+                ws[t >> 5] = ci;
+                S.wf[t >> 5] = si;
+            }
+            __syncthreads();
+            const uint32_t cw = (uint32_t)ws[lane & (SAMPLE_WARPS - 1)];
+            const float sw = S.wf[lane & (SAMPLE_WARPS - 1)];
+            uint32_t cu = cw;
+            float su = sw;
+#pragma unroll
+            for (int o = 1; o < SAMPLE_WARPS; o <<= 1) {
+                const uint32_t p = __shfl_up_sync(0xffffffffu, cu, o);
+                const float q = __shfl_up_sync(0xffffffffu, su, o);
+                if ((int)(lane & (SAMPLE_WARPS - 1)) >= o) {
+                    cu += p;
+                    su += q;
+                }
+            }
+            n_weight = __shfl_sync(0xffffffffu, cu, SAMPLE_WARPS - 1);
+            a_total = __shfl_sync(0xffffffffu, su, SAMPLE_WARPS - 1);
+            const float s_up = __shfl_up_sync(0xffffffffu, su, 1), s_in = __shfl_up_sync(0xffffffffu, si, 1);
+            const uint32_t cb4 = __shfl_sync(0xffffffffu, cu - cw, t >> 5) + ci - c_all;
+            const float sb = ((t >> 5) ? __shfl_sync(0xffffffffu, s_up, t >> 5) : 0.f) + (lane ? s_in : 0.f);
+#pragma unroll
+            for (int j = 0; j < SAMPLE_BPT; j++) {
+                cc[j] += cb4;
+                sm[j] += sb;
+            }
+        }
+        const bool by_k = top_k > 0 && (uint32_t)top_k < n_weight;
+        const uint32_t k = by_k ? (uint32_t)top_k : n_weight;
+        // S.first: the bin of the k-th token; S.second: the first bin up to which the masses surely reach top_p of all of them
+        // (without top-k, where all is all); and the tokens up to either
+        const float sure = top_p * a_total * ((1.f + SAMPLE_DELTA) / (1.f - SAMPLE_DELTA));
+        if (t == 0) S.found[0] = n_weight;
         __syncthreads();
-        if (by_k) {
-            if (c_before < k && k <= c0) S.first = 2u * t;
-            if (c0 < k && k <= c1) S.first = 2u * t + 1u;
-        }
-        // the first bin up to which the masses surely reach top_p of all of them (only without top-k, where all is all)
-        const double sure = (double)top_p * (double)a_total * (1.0 + SAMPLE_DELTA) / (1.0 - SAMPLE_DELTA) + SAMPLE_BINS;
-        if (!by_k && nucleus) {
-            if ((double)a_before < sure && sure <= s0) S.second = 2u * t;
-            if (s0 < sure && sure <= s1) S.second = 2u * t + 1u;
+#pragma unroll
+        for (int j = 0; j < SAMPLE_BPT; j++) {
+            const uint32_t c_prev = cc[j] - h[j];
+            if (by_k) {
+                if (c_prev < k && k <= cc[j]) {
+                    S.first = SAMPLE_BPT * t + j;
+                    S.found[0] = cc[j];
+                    S.found[1] = c_prev;
+                }
+            } else if (h[j] && sm[j] >= sure) {
+                atomicMin(&S.second, SAMPLE_BPT * t + j);
+            }
         }
         __syncthreads();
         const uint32_t bk = S.first, b_last = by_k ? bk : S.second;
-        // tokens up to b_last
-        __syncthreads();
-        if (b_last / 2u == t) S.found[0] = b_last & 1u ? c1 : c0;
-        __syncthreads();
-        const u64 n_last = S.found[0];
+        if (!by_k) {
+            if (b_last / SAMPLE_BPT == t) S.found[0] = cc[b_last % SAMPLE_BPT];
+            __syncthreads();
+        }
+        const uint32_t n_last = (uint32_t)S.found[0], above_k = (uint32_t)S.found[1];
 
         if (n_last <= SAMPLE_CAP) {
             // ---- few candidates: the whole draw in one block
             u64 all = 0;
             if (!by_k) {  // top-p of the whole row
-                for (uint32_t i = i0; i < i1; i++) all += R.steps(R.order(xs[i]));
-                all = R.sum(all);
+                uint32_t hs = 0, ls = 0;  // (at most 97 tokens to a thread: their halves fit 32 bits)
+                each_logit(xs, i0, i1, [&](float v, uint32_t) {
+                    const float y = R.order(v);
+                    uint32_t hi, lo;
+                    Row::split(Row::weighs(y) ? y : -200.f, hi, lo);
+                    hs += hi;
+                    ls += lo;
+                });
+                all = ((u64)hs << 20) + ls;
+                (void)R.before(all, all);
             }
-            const uint32_t n = R.gather([&](float v) { return R.bin(R.order(v)) <= b_last; });
+            const float stop = (float)(b_last + 1u);
+            const uint32_t n = R.gather([&](float v, uint32_t) { return R.bin_of(v) < stop; }, all);
             if (rank == 0) {
-                R.sort_list(n);
-                const uint32_t keep = by_k ? min(n, (uint32_t)k) : n;
-                // two neighbours to a thread
-                u64 e[2], w[2];
-                for (int j = 0; j < 2; j++) {
-                    const uint32_t i = 2u * t + j;
-                    e[j] = i < keep ? S.list.e[i] : ~0ull;
-                    w[j] = i < keep ? R.steps(R.order(key_logit(~(uint32_t)(e[j] >> 32)))) : 0ull;
-                }
-                u64 sum_k;
-                const u64 b0 = R.before(w[0] + w[1], sum_k);
-                if (by_k) all = sum_k;
-                const double need = (double)top_p * (double)all;
-                u64 kept = 0;
-                for (int j = 0; j < 2; j++) {
-                    const uint32_t i = 2u * t + j;
-                    const u64 bef = j ? b0 + w[0] : b0;
-                    bool on = i < keep && (!nucleus || i == 0u || (double)bef < need);
-                    if (on) {
-                        const float v = key_logit(~(uint32_t)(e[j] >> 32));
-                        on = v == m || exp2f(R.order(v)) >= R.min_p;
+                const uint32_t kk = by_k ? min(n, k) : n;
+                if (n <= 64u) {
+                    // ---- one warp, two tokens to a lane; ranks and sums in index order by counting
+                    if (t < 32u) {
+                        u64 e[2];
+                        uint32_t rk[2] = {0u, 0u};
+                        for (int j = 0; j < 2; j++) e[j] = lane + 32u * j < n ? S.list.e[lane + 32u * j] : ~0ull;
+                        for (uint32_t i = 0; i < n; i++) {
+                            const u64 o = S.list.e[i];
+                            rk[0] += o < e[0];
+                            rk[1] += o < e[1];
+                        }
+                        u64 w[2], bef[2] = {0ull, 0ull};
+                        for (int j = 0; j < 2; j++) {
+                            w[j] = rk[j] < kk && lane + 32u * j < n ? Row::steps(R.order(key_logit(~(uint32_t)(e[j] >> 32)))) : 0ull;
+                            S.list.sorted[lane + 32u * j] = w[j];
+                        }
+                        u64 of_k = w[0] + w[1];
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) of_k += __shfl_xor_sync(0xffffffffu, of_k, o);
+                        if (by_k) all = of_k;
+                        __syncwarp();
+                        if (nucleus) {
+                            for (uint32_t i = 0; i < n; i++) {
+                                const u64 o = S.list.e[i], wo = S.list.sorted[i];
+                                bef[0] += o < e[0] ? wo : 0ull;
+                                bef[1] += o < e[1] ? wo : 0ull;
+                            }
+                        }
+                        __syncwarp();
+                        const double need = (double)top_p * (double)all;
+                        for (int j = 0; j < 2; j++) {
+                            const float v = key_logit(~(uint32_t)(e[j] >> 32));
+                            const bool on = w[j] && (!nucleus || rk[j] == 0u || (double)bef[j] < need) && (v == m || exp2f(R.order(v)) >= min_p);
+                            if (!on) w[j] = 0ull;
+                            S.list.sorted[lane + 32u * j] = w[j];
+                        }
+                        __syncwarp();
+                        u64 upto[2] = {0ull, 0ull}, total = 0;
+                        for (uint32_t i = 0; i < n; i++) {
+                            const uint32_t o = (uint32_t)S.list.e[i];
+                            const u64 wo = S.list.sorted[i];
+                            total += wo;
+                            upto[0] += o <= (uint32_t)e[0] ? wo : 0ull;
+                            upto[1] += o <= (uint32_t)e[1] ? wo : 0ull;
+                        }
+                        const u64 target = target_of(total);
+                        for (int j = 0; j < 2; j++)
+                            if (w[j] && upto[j] > target && upto[j] - w[j] <= target) write((uint32_t)e[j], w[j], total);
                     }
-                    // kept tokens by index for the draw; the others go to the end
-                    if (i < keep) S.list.e[i] = on ? (e[j] & 0xffffffffull) << 32 | (uint32_t)(e[j] >> 32) : ~0ull;
-                    kept += on;
+                } else {
+                    R.sort_list(n);
+                    u64 e[SAMPLE_BPT], w[SAMPLE_BPT], mine = 0;  // neighbours
+#pragma unroll
+                    for (int j = 0; j < SAMPLE_BPT; j++) {
+                        const uint32_t i = SAMPLE_BPT * t + j;
+                        e[j] = i < kk ? S.list.e[i] : ~0ull;
+                        w[j] = i < kk ? Row::steps(R.order(key_logit(~(uint32_t)(e[j] >> 32)))) : 0ull;
+                        mine += w[j];
+                    }
+                    u64 of_k;
+                    u64 b = R.before(mine, of_k);
+                    if (by_k) all = of_k;
+                    const double need = (double)top_p * (double)all;
+                    u64 kept = 0;
+#pragma unroll
+                    for (int j = 0; j < SAMPLE_BPT; j++) {
+                        const uint32_t i = SAMPLE_BPT * t + j;
+                        bool on = i < kk && (!nucleus || i == 0u || (double)b < need);
+                        if (on) {
+                            const float v = key_logit(~(uint32_t)(e[j] >> 32));
+                            on = v == m || exp2f(R.order(v)) >= min_p;
+                        }
+                        // kept tokens by index for the draw; the others go to the end
+                        if (i < kk) S.list.e[i] = on ? (e[j] & 0xffffffffull) << 32 | (uint32_t)(e[j] >> 32) : ~0ull;
+                        kept += on;
+                        b += w[j];
+                    }
+                    u64 n_kept;
+                    (void)R.before(kept, n_kept);
+                    R.sort_list(kk);
+                    mine = 0;
+#pragma unroll
+                    for (int j = 0; j < SAMPLE_BPT; j++) {
+                        const uint32_t i = SAMPLE_BPT * t + j;
+                        e[j] = i < (uint32_t)n_kept ? S.list.e[i] : ~0ull;
+                        w[j] = i < (uint32_t)n_kept ? Row::steps(R.order(key_logit(~(uint32_t)e[j]))) : 0ull;
+                        mine += w[j];
+                    }
+                    u64 total;
+                    b = R.before(mine, total);
+                    const u64 target = target_of(total);
+#pragma unroll
+                    for (int j = 0; j < SAMPLE_BPT; j++) {
+                        if (b <= target && b + w[j] > target) write((uint32_t)(e[j] >> 32), w[j], total);
+                        b += w[j];
+                    }
                 }
-                u64 n_kept;
-                (void)R.before(kept, n_kept);
-                __syncthreads();
-                R.sort_list(keep);
-                for (int j = 0; j < 2; j++) {
-                    const uint32_t i = 2u * t + j;
-                    e[j] = i < (uint32_t)n_kept ? S.list.e[i] : ~0ull;
-                    w[j] = i < (uint32_t)n_kept ? R.steps(R.order(key_logit(~(uint32_t)e[j]))) : 0ull;
-                }
-                u64 total;
-                const u64 bef = R.before(w[0] + w[1], total), target = target_of(total);
-                if (bef <= target && bef + w[0] > target) write((uint32_t)(e[0] >> 32), w[0], total);
-                else if (bef + w[0] <= target && bef + w[0] + w[1] > target) write((uint32_t)(e[1] >> 32), w[1], total);
             }
-            cl.sync();
+            Row::csync();
             return;
         }
 
         // ---- many: cuts by the uncertain bins. A cut is told to all blocks through rank 0's S.found.
         auto told = [&](bool mine, uint32_t key, uint32_t last) {
             if (mine) S.found[1] = (u64)key << 32 | last;
-            cl.sync();
-            const u64 f = *cl.map_shared_rank(&S.found[1], 0);
-            cl.sync();
+            Row::csync();
+            const u64 f = Row::far(&S.found[1], 0);
+            Row::csync();
             return Cut{(uint32_t)(f >> 32), (uint32_t)f};
         };
         // the index of the quota-th kept token with this key
@@ -439,7 +645,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
                         break;
                     }
             }
-            R.fold(at, add);
+            R.fold(at, OpAdd());
             return (uint32_t)at[0];
         };
         // smallest and largest key among the tokens `in` names
@@ -451,20 +657,23 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
                     r[0] = max(r[0], (u64)~key);
                     r[1] = max(r[1], (u64)key);
                 }
-            R.fold(r, [](u64 p, u64 q) { return p > q ? p : q; });
+            R.fold(r, OpMax());
             lo = ~(uint32_t)r[0];
             hi = (uint32_t)r[1];
         };
+        u64 nothing = 0;
         if (by_k) {
-            if (bk / 2u == t) S.found[0] = bk & 1u ? c0 : c_before;  // tokens above the bin
-            __syncthreads();
-            const u64 above = S.found[0], quota = k - above;
-            auto in = [&](float v, uint32_t) { return R.bin(R.order(v)) == bk; };
-            if (n_last - above <= SAMPLE_CAP) {
-                const uint32_t n = R.gather([&](float v) { return in(v, 0u); });
+            const uint32_t quota = k - above_k;  // tokens of the bin that stay
+            auto in = [&](float v, uint32_t) {
+                const float b = R.bin_of(v);
+                return b < (float)SAMPLE_BINS && Row::bin(b) == bk;
+            };
+            if (n_last - above_k <= SAMPLE_CAP) {
+                const uint32_t n = R.gather(in, nothing);
                 if (rank == 0) R.sort_list(n);
                 const u64 e = rank == 0 ? S.list.e[quota - 1] : 0ull;
                 cut = told(rank == 0 && t == 0, ~(uint32_t)(e >> 32), (uint32_t)e);
+                if (t == 0) S.n_list = 0u;
             } else {  // the largest key that `quota` tokens of the bin reach
                 uint32_t lo, hi;
                 key_range(in, lo, hi);
@@ -482,115 +691,116 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
         }
         if (nucleus) {
             u64 all = 0;
-            for (uint32_t i = i0; i < i1; i++)
-                if (cut.keeps(logit_key(xs[i]), base + i)) all += R.steps(R.order(xs[i]));
+            each_logit(xs, i0, i1, [&](float v, uint32_t i) {
+                const float y = R.order(v);
+                if (!by_k || cut.keeps(logit_key(v), base + i)) all += Row::steps(y);
+            });
             all = R.sum(all);
             const double need = (double)top_p * (double)all;
-            // bins that are surely kept, and from where on surely nothing is: masses in steps of 2^-32 against `need` in 2^-40
-            const double n32 = need * 0.00390625;
+            // bins that are surely kept, and from where on surely nothing is
             if (t == 0) {
                 S.first = 0u;
                 S.second = bk;
             }
             __syncthreads();
-            const double lo_d = n32 / (1.0 + SAMPLE_DELTA) - SAMPLE_BINS, hi_d = n32 / (1.0 - SAMPLE_DELTA) + SAMPLE_BINS;
-            if (s0 < lo_d) atomicMax(&S.first, 2u * t + 1u);  // (bins up to 2 t stay)
-            if (s1 < lo_d) atomicMax(&S.first, 2u * t + 2u);
-            if (s0 >= hi_d) atomicMin(&S.second, 2u * t);
-            if (s1 >= hi_d) atomicMin(&S.second, 2u * t + 1u);
+            const float n1 = (float)(need * (1.0 / 1099511627776.0)), lo_d = n1 / (1.f + SAMPLE_DELTA), hi_d = n1 / (1.f - SAMPLE_DELTA);
+#pragma unroll
+            for (int j = 0; j < SAMPLE_BPT; j++) {
+                if (h[j] && sm[j] < lo_d) atomicMax(&S.first, SAMPLE_BPT * t + j + 1u);  // (the bin stays)
+                if (h[j] && sm[j] >= hi_d) atomicMin(&S.second, SAMPLE_BPT * t + j);
+            }
             __syncthreads();
-            const uint32_t b_lo = min(S.first, S.second), b_hi = S.second;  // the uncertain bins
+            const uint32_t b_hi = S.second, b_lo = min(S.first, b_hi);  // the uncertain bins
             // exact masses: of what lies above them, and of 2048 finer bins
             __syncthreads();
             for (uint32_t i = t; i < SAMPLE_BINS; i += SAMPLE_THREADS) {
                 S.fine.mass[i] = 0ull;
                 S.fine.count[i] = 0u;
             }
+            if (t == 0) S.first = 0u;
             __syncthreads();
-            const float f_lo = (float)b_lo * mid, f_scale = (SAMPLE_BINS - 1u) / ((float)(b_hi + 1u - b_lo) * mid);
-            auto fine = [&](float y) { return (uint32_t)fminf(fmaxf((-y - f_lo) * f_scale, 0.f), (float)(SAMPLE_BINS - 1u)); };
+            const float f_lo = (float)b_lo, f_hi = (float)(b_hi + 1u), f_scale = (float)SAMPLE_BINS / (f_hi - f_lo);
+            auto fine = [&](float b) { return Row::bin(fminf((b - f_lo) * f_scale, (float)(SAMPLE_BINS - 1u))); };
             u64 above = 0;
-            for (uint32_t i = i0; i < i1; i++) {
-                const float y = R.order(xs[i]);
-                const uint32_t b = R.bin(y);
-                if (b > b_hi || !cut.keeps(logit_key(xs[i]), base + i)) continue;
-                const u64 w = R.steps(y);
-                if (b < b_lo) {
+            each_logit(xs, i0, i1, [&](float v, uint32_t i) {
+                const float b = R.bin_of(v);
+                if (!(b < f_hi) || (by_k && !cut.keeps(logit_key(v), base + i))) return;
+                const u64 w = Row::steps(R.order(v));
+                if (b < f_lo) {
                     above += w;
                 } else {
-                    const uint32_t f = fine(y);
+                    const uint32_t f = fine(b);
                     atomicAdd(&S.fine.count[f], 1u);
                     uint32_t *half = reinterpret_cast<uint32_t *>(&S.fine.mass[f]);
                     const uint32_t low = (uint32_t)w, was = atomicAdd(half, low);
                     const uint32_t high = (uint32_t)(w >> 32) + (was + low < was);  // (two adds that carry: exact in any order)
                     if (high) atomicAdd(half + 1, high);
                 }
-            }
-            above = R.sum(above);  // (its barrier also ends the histogram)
-            u64 g0 = 0, g1 = 0;
-            uint32_t q0 = 0, q1 = 0;
-            for (uint32_t r = 0; r < C; r++) {
-                const ulonglong2 g = reinterpret_cast<const ulonglong2 *>(cl.map_shared_rank(&S.fine.mass[0], r))[t];
-                const uint2 q = reinterpret_cast<const uint2 *>(cl.map_shared_rank(&S.fine.count[0], r))[t];
-                g0 += g.x;
-                g1 += g.y;
-                q0 += q.x;
-                q1 += q.y;
+            });
+            above = R.sum(above);
+            if constexpr (C == 1) __syncthreads();  // (in a cluster, the sum's barrier ends the histogram)
+            u64 g[SAMPLE_BPT] = {}, bef[SAMPLE_BPT];
+            uint32_t q[SAMPLE_BPT] = {};
+#pragma unroll
+            for (int r = 0; r < C; r++) {
+                const ulonglong2 ga = Row::far(reinterpret_cast<const ulonglong2 *>(&S.fine.mass[0]) + 2 * t, r);
+                const ulonglong2 gb = Row::far(reinterpret_cast<const ulonglong2 *>(&S.fine.mass[0]) + 2 * t + 1, r);
+                const uint4 qa = Row::far(reinterpret_cast<const uint4 *>(&S.fine.count[0]) + t, r);
+                g[0] += ga.x;
+                g[1] += ga.y;
+                g[2] += gb.x;
+                g[3] += gb.y;
+                q[0] += qa.x;
+                q[1] += qa.y;
+                q[2] += qa.z;
+                q[3] += qa.w;
             }
             u64 g_all;
-            const u64 m0 = above + R.before(g0 + g1, g_all), m1 = m0 + g0;
+            bef[0] = above + R.before(g[0] + g[1] + g[2] + g[3], g_all);
             // the last finer bin with tokens before which the mass is below `need`
-            if (t == 0) S.first = 0u;
+#pragma unroll
+            for (int j = 0; j < SAMPLE_BPT; j++) {
+                if (j) bef[j] = bef[j - 1] + g[j - 1];
+                if (q[j] && ((double)bef[j] < need || bef[j] == 0ull)) atomicMax(&S.first, SAMPLE_BPT * t + j + 1u);
+            }
             __syncthreads();
-            if (q0 && ((double)m0 < need || m0 == 0ull)) atomicMax(&S.first, 2u * t + 1u);
-            if (q1 && ((double)m1 < need || m1 == 0ull)) atomicMax(&S.first, 2u * t + 2u);
-            __syncthreads();
-            if (S.first > 0u) {  // (0: no token in the uncertain bins, nothing to cut)
-                const uint32_t fb = S.first - 1u;
-                __syncthreads();
-                if (fb / 2u == t) {
-                    S.found[0] = fb & 1u ? m1 : m0;
-                    S.second = fb & 1u ? q1 : q0;
-                }
-                cl.sync();  // every block has read the others' masses: the lists may take their place
+            const uint32_t fb1 = S.first;
+            if (fb1 > 0u) {  // (0: no token in the uncertain bins, nothing to cut)
+                const uint32_t fb = fb1 - 1u;
+#pragma unroll
+                for (int j = 0; j < SAMPLE_BPT; j++)
+                    if (fb == SAMPLE_BPT * t + j) {
+                        S.found[0] = bef[j];
+                        S.second = q[j];
+                    }
+                Row::csync();  // every block has read the others' masses: the lists may take their place
                 const u64 mass_above = S.found[0];
                 const uint32_t n_fine = S.second;
                 const Cut old = cut;
                 auto in = [&](float v, uint32_t i) {
-                    const float y = R.order(v);
-                    const uint32_t b = R.bin(y);
-                    return b >= b_lo && b <= b_hi && fine(y) == fb && old.keeps(logit_key(v), i);
+                    const float b = R.bin_of(v);
+                    return b >= f_lo && b < f_hi && fine(b) == fb && (!by_k || old.keeps(logit_key(v), i));
                 };
                 if (n_fine <= SAMPLE_CAP) {
-                    __syncthreads();
-                    if (t == 0) S.n_list = 0u;
-                    __syncthreads();
-                    for (uint32_t i = i0; i < i1; i++)
-                        if (in(xs[i], base + i)) S.list.e[atomicAdd(&S.n_list, 1u)] = (u64)(~logit_key(xs[i])) << 32 | (base + i);
-                    cl.sync();
+                    const uint32_t n = R.gather(in, nothing);
                     if (rank == 0) {
-                        uint32_t n = S.n_list;
-                        for (uint32_t r = 1; r < C; r++) {
-                            const uint32_t kk = *cl.map_shared_rank(&S.n_list, r);
-                            const u64 *src = cl.map_shared_rank(&S.list.e[0], r);
-                            for (uint32_t i = t; i < kk && n + i < SAMPLE_CAP; i += SAMPLE_THREADS) S.list.e[n + i] = src[i];
-                            n += kk;
-                        }
-                        n = min(n, SAMPLE_CAP);
-                        __syncthreads();
                         R.sort_list(n);
-                        u64 e[2], w[2], dummy;
-                        for (int j = 0; j < 2; j++) {
-                            const uint32_t i = 2u * t + j;
-                            e[j] = i < n ? S.list.e[i] : 0ull;
-                            w[j] = i < n ? R.steps(R.order(key_logit(~(uint32_t)(e[j] >> 32)))) : 0ull;
+                        u64 w[SAMPLE_BPT], mine = 0, dummy;
+#pragma unroll
+                        for (int j = 0; j < SAMPLE_BPT; j++) {
+                            const uint32_t i = SAMPLE_BPT * t + j;
+                            w[j] = i < n ? Row::steps(R.order(key_logit(~(uint32_t)(S.list.e[i] >> 32)))) : 0ull;
+                            mine += w[j];
                         }
-                        const u64 p0 = mass_above + R.before(w[0] + w[1], dummy), p1 = p0 + w[0];
-                        // the last token before which the mass is below `need`
                         if (t == 0) S.first = 0u;
-                        __syncthreads();
-                        if (2u * t < n && ((double)p0 < need || p0 == 0ull)) atomicMax(&S.first, 2u * t);
-                        if (2u * t + 1u < n && (double)p1 < need) atomicMax(&S.first, 2u * t + 1u);
+                        u64 b = mass_above + R.before(mine, dummy);
+                        // the last token before which the mass is below `need`
+#pragma unroll
+                        for (int j = 0; j < SAMPLE_BPT; j++) {
+                            const uint32_t i = SAMPLE_BPT * t + j;
+                            if (i < n && ((double)b < need || b == 0ull)) atomicMax(&S.first, i);
+                            b += w[j];
+                        }
                         __syncthreads();
                     }
                     const u64 e = rank == 0 ? S.list.e[S.first] : 0ull;
@@ -602,18 +812,18 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
                         const uint32_t mid_key = lo + (hi - lo) / 2u;
                         u64 w = 0;
                         for (uint32_t i = i0; i < i1; i++)
-                            if (logit_key(xs[i]) > mid_key && in(xs[i], base + i)) w += R.steps(R.order(xs[i]));
+                            if (logit_key(xs[i]) > mid_key && in(xs[i], base + i)) w += Row::steps(R.order(xs[i]));
                         if ((double)(mass_above + R.sum(w)) < need) hi = mid_key; else lo = mid_key + 1u;
                     }
                     u64 v[2] = {0ull, 0ull};
                     for (uint32_t i = i0; i < i1; i++)
                         if (in(xs[i], base + i)) {
                             const uint32_t key = logit_key(xs[i]);
-                            if (key > lo) v[0] += R.steps(R.order(xs[i]));
+                            if (key > lo) v[0] += Row::steps(R.order(xs[i]));
                             v[1] += key == lo;
                         }
-                    R.fold(v, add);
-                    const u64 w1 = R.steps(R.order(key_logit(lo))), s = mass_above + v[0];
+                    R.fold(v, OpAdd());
+                    const u64 w1 = Row::steps(R.order(key_logit(lo))), s = mass_above + v[0];
                     // the j-th equal (from 0) stays if s + j w1 < need
                     double j = w1 ? ceil((need - (double)s) / (double)w1) : (double)v[1];
                     j = fmin(fmax(j, 1.0), (double)v[1]);
@@ -624,19 +834,20 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
     }
 
     // ---- the draw, in index order
-    auto value = [&](uint32_t i) -> u64 {
-        const float v = xs[i], y = R.order(v);
-        if (y < -SAMPLE_ORDERS || !cut.keeps(logit_key(v), base + i)) return 0ull;
-        if (R.min_p > 0.f && v != m && exp2f(y) < R.min_p) return 0ull;
-        return R.steps(y);
+    const bool cuts = cut.key != 0u;
+    auto value = [&](float v, uint32_t i) -> u64 {
+        const float y = R.order(v);
+        if (!Row::weighs(y) || (cuts && !cut.keeps(logit_key(v), base + i))) return 0ull;
+        if (min_p > 0.f && v != m && !(exp2f(y) >= min_p)) return 0ull;
+        return Row::steps(y);
     };
     u64 mine = 0, total;
-    for (uint32_t i = i0; i < i1; i++) mine += value(i);
+    each_logit(xs, i0, i1, [&](float v, uint32_t i) { mine += value(v, i); });
     const u64 bef = R.before_all(mine, total), target = target_of(total);
     if (bef <= target && bef + mine > target) {
         u64 s = bef;
         for (uint32_t i = i0; i < i1; i++) {
-            const u64 w = value(i);
+            const u64 w = value(xs[i], i);
             s += w;
             if (s > target) {
                 write(base + i, w, total);
@@ -644,40 +855,53 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
             }
         }
     }
-    cl.sync();
+    Row::csync();
 }
 
-// Blocks to a row. More blocks shorten every pass, a cluster barrier costs the same; the row has to fit their shared memory.
+// Blocks to a row. More blocks shorten every pass, a cluster barrier costs the same; the row has to fit their shared memory, and
+// with many rows two blocks to an SM hide each other's barriers.
 static uint32_t sample_cluster(uint32_t n, uint32_t rows, size_t smem_optin) {
     const size_t room = (smem_optin - sizeof(SampleShared) - 1024) / 4;
     uint32_t c = 1;
     while (c < 8 && (size_t)(n + c - 1) / c > (rows * c >= 296 ? room : 4096)) c *= 2;
-    while (c < SAMPLE_MAX_CLUSTER && (size_t)((n + c - 1) / c + 3) > room) c *= 2;
     return c;
 }
 
-cudaError_t launch_sample(strix_cuda *h, const float *d_x, uint32_t n, size_t stride, uint32_t rows, const strix_sample_params &p,
-                          const float *d_u, uint32_t *d_ids, float *d_probs, cudaStream_t stream) {
-    const uint32_t c = sample_cluster(n, rows, h->smem_optin);
-    const uint32_t per = ((n + c - 1) / c + 3u) & ~3u;
-    const SampleArgs A{d_x, stride, n, per, p, d_u, d_ids, d_probs};
-    const size_t smem = sizeof(SampleShared) + (size_t)per * 4;
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess && c > 8) e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
+template <int C>
+static cudaError_t sample_launch(strix_cuda *h, const SampleArgs &A, uint32_t rows, cudaStream_t stream) {
+    const size_t smem = sizeof(SampleShared) + (size_t)A.per * 4;
+    static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic shared memory is raised for this kernel
+    const uint64_t bit = 1ull << (h->device & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(h->smem_optin - 512));
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(rows * c);
+    cfg.gridDim = dim3(rows * C);
     cfg.blockDim = dim3(SAMPLE_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = c;
+    at[0].val.clusterDim.x = C;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, sample_kernel<C>, A);
+}
+
+cudaError_t launch_sample(strix_cuda *h, const float *d_x, uint32_t n, size_t stride, uint32_t rows, const strix_sample_params &p,
+                          const float *d_u, uint32_t *d_ids, float *d_probs, cudaStream_t stream) {
+    const uint32_t c = sample_cluster(n, rows, h->smem_optin);
+    const SampleArgs A{d_x, stride, n, ((n + c - 1) / c + 3u) & ~3u, p, d_u, d_ids, d_probs};
     ProfScope prof(h, stream, "sample");
-    return cudaLaunchKernelEx(&cfg, sample_kernel, A);
+    switch (c) {
+        case 1: return sample_launch<1>(h, A, rows, stream);
+        case 2: return sample_launch<2>(h, A, rows, stream);
+        case 4: return sample_launch<4>(h, A, rows, stream);
+        default: return sample_launch<8>(h, A, rows, stream);
+    }
 }
 
 }  // namespace strix
