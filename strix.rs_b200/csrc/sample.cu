@@ -47,11 +47,15 @@ struct SampleArgs {
     float *probs;
 };
 
-// Unsigned keys in the order of the logits; NaN ranks as -inf, -0 equals +0.
+// Unsigned keys in the order of the logits (no NaN here: they become -inf on their way into shared memory); -0 equals +0.
 __device__ __forceinline__ uint32_t logit_key(float x) {
-    if (x != x) x = -INFINITY;
     const uint32_t b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float ex2(float y) {
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(y));
+    return w;
 }
 __device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
@@ -85,18 +89,17 @@ struct OpMax {
     __device__ u64 operator()(u64 p, u64 q) const { return p > q ? p : q; }
 };
 
-// f(logit, its place in the block) for every logit of a thread's stretch; the loads of eight go ahead of their use
+// f(logit, its place in the block) for every logit of the block, shared out in words of four (xs is padded to one with -inf)
 template <typename F>
-__device__ __forceinline__ void each_logit(const float *xs, uint32_t i0, uint32_t i1, F f) {
-    uint32_t i = i0;
-    for (; i + 8u <= i1; i += 8u) {
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = xs[i + j];
-#pragma unroll
-        for (int j = 0; j < 8; j++) f(v[j], i + j);
+__device__ __forceinline__ void each_logit(const float *xs, uint32_t cnt, F f) {
+#pragma unroll 4
+    for (uint32_t i = 4u * threadIdx.x; i < cnt; i += 4u * SAMPLE_THREADS) {
+        const float4 v = *reinterpret_cast<const float4 *>(xs + i);
+        f(v.x, i);
+        f(v.y, i + 1u);
+        f(v.z, i + 2u);
+        f(v.w, i + 3u);
     }
-    for (; i < i1; i++) f(xs[i], i);
 }
 
 // One block's view of its row, which C blocks share. Two rules keep the cluster together: what a block shows to the others
@@ -106,7 +109,7 @@ template <int C>
 struct SampleRow {
     SampleShared &S;
     const float *xs;                // this block's logits
-    uint32_t base, i0, i1;          // index of the first; this thread's stretch (of an odd length: no bank conflicts)
+    uint32_t base, cnt;             // index of the first, how many
     float m, c, cb, min_p;          // maximum; log2(e) / T; bins to a unit of logit
     uint32_t turn, wturn;
 
@@ -120,12 +123,12 @@ struct SampleRow {
         if constexpr (C > 1) return *cg::this_cluster().map_shared_rank(p, r);
         else return *p;
     }
-    // log2 of a weight: NaN or far below -SAMPLE_ORDERS where there is none
+    // log2 of a weight, below -SAMPLE_ORDERS where there is none (NaN for -inf at an infinite temperature: no weight either)
     __device__ float order(float x) const { return (x - m) * c; }
     __device__ static bool weighs(float y) { return y >= -SAMPLE_ORDERS; }
     // the weight in steps of 2^-40 (rounded to nearest), as units of 2^20 and the rest
     __device__ static void split(float y, uint32_t &hi, uint32_t &lo) {
-        const float w = exp2f(y) * 1048576.f, h = __fadd_rd(w, 8388608.f);
+        const float w = ex2(y) * 1048576.f, h = __fadd_rd(w, 8388608.f);
         hi = __float_as_uint(h) & 0x7fffffu;
         lo = __float_as_uint(fmaf(w - (h - 8388608.f), 1048576.f, 8388608.f)) & 0x7fffffu;
     }
@@ -266,7 +269,7 @@ struct SampleRow {
     // tells the others by the same barrier: their sum comes back through it.
     template <typename F>
     __device__ uint32_t gather(F want, u64 &told) {
-        each_logit(xs, i0, i1, [&](float x, uint32_t i) {
+        each_logit(xs, cnt, [&](float x, uint32_t i) {
             if (!want(x, base + i)) return;
             const uint32_t at = atomicAdd(&S.n_list, 1u);
             if (at < SAMPLE_CAP) S.list.e[at] = (u64)(~logit_key(x)) << 32 | (base + i);
@@ -331,23 +334,25 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         float4 *s4 = reinterpret_cast<float4 *>(xs);
 #pragma unroll 8
         for (uint32_t i = t; i < n4; i += SAMPLE_THREADS) {
-            const float4 v = __ldcs(x4 + i);
+            float4 v = __ldcs(x4 + i);
+            v = make_float4(fmaxf(v.x, -INFINITY), fmaxf(v.y, -INFINITY), fmaxf(v.z, -INFINITY), fmaxf(v.w, -INFINITY));  // NaN to -inf
             s4[i] = v;
             m = fmaxf(fmaxf(m, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
         }
         for (uint32_t i = n4 * 4 + t; i < cnt; i += SAMPLE_THREADS) {
-            const float v = x[i];
+            const float v = fmaxf(x[i], -INFINITY);
             xs[i] = v;
             m = fmaxf(m, v);
         }
     } else {
 #pragma unroll 8
         for (uint32_t i = t; i < cnt; i += SAMPLE_THREADS) {
-            const float v = __ldcs(x + i);
+            const float v = fmaxf(__ldcs(x + i), -INFINITY);
             xs[i] = v;
             m = fmaxf(m, v);
         }
     }
+    if (t < (-cnt & 3u)) xs[cnt + t] = -INFINITY;
     for (uint32_t i = t; i < SAMPLE_BINS / 2; i += SAMPLE_THREADS) S.hist[i] = 0u;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -367,13 +372,15 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
 #pragma unroll
         for (int o = C / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     }
+    // this thread's stretch where index order matters (of an odd length: no bank conflicts)
     const uint32_t seg = ((cnt + SAMPLE_THREADS - 1) / SAMPLE_THREADS) | 1u, i0 = min(cnt, t * seg), i1 = min(cnt, i0 + seg);
     if (m == INFINITY) {  // only the infinite ones have weight: as if they were the only ones
-        for (uint32_t i = i0; i < i1; i++) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
+        for (uint32_t i = t; i < cnt; i += SAMPLE_THREADS) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
         m = 0.f;
+        __syncthreads();
     }
     const float c = fminf(1.4426950408889634f / temp, 1.0e36f);
-    Row R{S, xs, base, i0, i1, m, c, c * (SAMPLE_BINS / SAMPLE_ORDERS), min_p, 0u, 0u};
+    Row R{S, xs, base, cnt, m, c, c * (SAMPLE_BINS / SAMPLE_ORDERS), min_p, 0u, 0u};
 
     if (m == -INFINITY || greedy) {  // no token, or the first of the largest
         u64 best[1] = {0xffffffffull};
@@ -401,12 +408,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     const bool nucleus = top_p < 1.f;
     if ((top_k > 0 && (uint32_t)top_k < A.n) || nucleus) {
         // ---- histogram of log2 weight
-        each_logit(xs, i0, i1, [&](float v, uint32_t) {
+        const uint32_t hist_at = smem_u32(&S.hist[0]);
+        each_logit(xs, cnt, [&](float v, uint32_t) {
+            // (in assembly for the predicated add: no branch around it)
             const float b = R.bin_of(v);
-            if (b < (float)SAMPLE_BINS) {
-                const uint32_t k = Row::bin(b);
-                atomicAdd(&S.hist[k / 2u], 1u << (k % 2u * 16u));
-            }
+            const uint32_t k = Row::bin(b);
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.f32 p, %0, %1;\n\t@p red.shared.add.u32 [%2], %3;\n\t}" ::"f"(b), "f"((float)SAMPLE_BINS),
+                         "r"(hist_at + (k / 2u) * 4u), "r"((k & 1u) ? 0x10000u : 1u)
+                         : "memory");
         });
         Row::csync();
         // a thread's bins: counts and middle masses up to each (f32 sums in a fixed order: they only bound)
@@ -504,72 +513,62 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
 
         if (n_last <= SAMPLE_CAP) {
             // ---- few candidates: the whole draw in one block
+            // (top-p of the whole row needs the sum of all weights: f32 over a thread's hundred or fewer, integers beyond)
             u64 all = 0;
-            if (!by_k) {  // top-p of the whole row
-                uint32_t hs = 0, ls = 0;  // (at most 97 tokens to a thread: their halves fit 32 bits)
-                each_logit(xs, i0, i1, [&](float v, uint32_t) {
-                    const float y = R.order(v);
-                    uint32_t hi, lo;
-                    Row::split(Row::weighs(y) ? y : -200.f, hi, lo);
-                    hs += hi;
-                    ls += lo;
-                });
-                all = ((u64)hs << 20) + ls;
-                (void)R.before(all, all);
-            }
             const float stop = (float)(b_last + 1u);
-            const uint32_t n = R.gather([&](float v, uint32_t) { return R.bin_of(v) < stop; }, all);
+            uint32_t n;
+            if (by_k) {
+                n = R.gather([&](float v, uint32_t) { return R.bin_of(v) < stop; }, all);
+            } else {
+                float sum = 0.f;
+                each_logit(xs, cnt, [&](float v, uint32_t) { sum += ex2(fmaxf(R.order(v), -200.f)); });
+                all = __float2ull_rn(sum * 1099511627776.f);
+                (void)R.before(all, all);
+                n = R.gather([&](float v, uint32_t) { return R.bin_of(v) < stop; }, all);
+            }
             if (rank == 0) {
                 const uint32_t kk = by_k ? min(n, k) : n;
                 if (n <= 64u) {
-                    // ---- one warp, two tokens to a lane; ranks and sums in index order by counting
-                    if (t < 32u) {
-                        u64 e[2];
-                        uint32_t rk[2] = {0u, 0u};
-                        for (int j = 0; j < 2; j++) e[j] = lane + 32u * j < n ? S.list.e[lane + 32u * j] : ~0ull;
-                        for (uint32_t i = 0; i < n; i++) {
-                            const u64 o = S.list.e[i];
-                            rk[0] += o < e[0];
-                            rk[1] += o < e[1];
+                    // ---- eight threads to a token; ranks, and sums in either order, by counting over all
+                    const uint32_t i = t / 8u, part = t % 8u;
+                    u64 *weight = S.list.sorted;
+                    const u64 e = i < n ? S.list.e[i] : ~0ull;
+                    const float v = key_logit(~(uint32_t)(e >> 32));
+                    const auto eight = [](u64 x) {
+                        x += __shfl_xor_sync(0xffffffffu, x, 1);
+                        x += __shfl_xor_sync(0xffffffffu, x, 2);
+                        return x + __shfl_xor_sync(0xffffffffu, x, 4);
+                    };
+                    u64 rk = 0;
+                    for (uint32_t j = part; j < n; j += 8u) rk += S.list.e[j] < e;
+                    rk = eight(rk);
+                    u64 w = i < n && rk < kk ? Row::steps(R.order(v)) : 0ull;
+                    if (part == 0u) weight[i] = w;
+                    __syncthreads();
+                    if (nucleus) {
+                        u64 bef = 0, of_k = 0;
+                        for (uint32_t j = part; j < n; j += 8u) {
+                            of_k += weight[j];
+                            bef += S.list.e[j] < e ? weight[j] : 0ull;
                         }
-                        u64 w[2], bef[2] = {0ull, 0ull};
-                        for (int j = 0; j < 2; j++) {
-                            w[j] = rk[j] < kk && lane + 32u * j < n ? Row::steps(R.order(key_logit(~(uint32_t)(e[j] >> 32)))) : 0ull;
-                            S.list.sorted[lane + 32u * j] = w[j];
-                        }
-                        u64 of_k = w[0] + w[1];
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) of_k += __shfl_xor_sync(0xffffffffu, of_k, o);
+                        bef = eight(bef);
+                        of_k = eight(of_k);
                         if (by_k) all = of_k;
-                        __syncwarp();
-                        if (nucleus) {
-                            for (uint32_t i = 0; i < n; i++) {
-                                const u64 o = S.list.e[i], wo = S.list.sorted[i];
-                                bef[0] += o < e[0] ? wo : 0ull;
-                                bef[1] += o < e[1] ? wo : 0ull;
-                            }
-                        }
-                        __syncwarp();
-                        const double need = (double)top_p * (double)all;
-                        for (int j = 0; j < 2; j++) {
-                            const float v = key_logit(~(uint32_t)(e[j] >> 32));
-                            const bool on = w[j] && (!nucleus || rk[j] == 0u || (double)bef[j] < need) && (v == m || exp2f(R.order(v)) >= min_p);
-                            if (!on) w[j] = 0ull;
-                            S.list.sorted[lane + 32u * j] = w[j];
-                        }
-                        __syncwarp();
-                        u64 upto[2] = {0ull, 0ull}, total = 0;
-                        for (uint32_t i = 0; i < n; i++) {
-                            const uint32_t o = (uint32_t)S.list.e[i];
-                            const u64 wo = S.list.sorted[i];
-                            total += wo;
-                            upto[0] += o <= (uint32_t)e[0] ? wo : 0ull;
-                            upto[1] += o <= (uint32_t)e[1] ? wo : 0ull;
-                        }
-                        const u64 target = target_of(total);
-                        for (int j = 0; j < 2; j++)
-                            if (w[j] && upto[j] > target && upto[j] - w[j] <= target) write((uint32_t)e[j], w[j], total);
+                        if (rk && !((double)bef < (double)top_p * (double)all)) w = 0ull;
                     }
+                    if (v != m && !(ex2(R.order(v)) >= min_p)) w = 0ull;
+                    __syncthreads();
+                    if (part == 0u) weight[i] = w;
+                    __syncthreads();
+                    u64 upto = 0, total = 0;
+                    for (uint32_t j = part; j < n; j += 8u) {
+                        total += weight[j];
+                        upto += (uint32_t)S.list.e[j] <= (uint32_t)e ? weight[j] : 0ull;
+                    }
+                    upto = eight(upto);
+                    total = eight(total);
+                    const u64 target = target_of(total);
+                    if (part == 0u && w && upto > target && upto - w <= target) write((uint32_t)e, w, total);
                 } else {
                     R.sort_list(n);
                     u64 e[SAMPLE_BPT], w[SAMPLE_BPT], mine = 0;  // neighbours
@@ -591,7 +590,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                         bool on = i < kk && (!nucleus || i == 0u || (double)b < need);
                         if (on) {
                             const float v = key_logit(~(uint32_t)(e[j] >> 32));
-                            on = v == m || exp2f(R.order(v)) >= min_p;
+                            on = v == m || ex2(R.order(v)) >= min_p;
                         }
                         // kept tokens by index for the draw; the others go to the end
                         if (i < kk) S.list.e[i] = on ? (e[j] & 0xffffffffull) << 32 | (uint32_t)(e[j] >> 32) : ~0ull;
@@ -691,7 +690,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         }
         if (nucleus) {
             u64 all = 0;
-            each_logit(xs, i0, i1, [&](float v, uint32_t i) {
+            each_logit(xs, cnt, [&](float v, uint32_t i) {
                 const float y = R.order(v);
                 if (!by_k || cut.keeps(logit_key(v), base + i)) all += Row::steps(y);
             });
@@ -722,7 +721,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             const float f_lo = (float)b_lo, f_hi = (float)(b_hi + 1u), f_scale = (float)SAMPLE_BINS / (f_hi - f_lo);
             auto fine = [&](float b) { return Row::bin(fminf((b - f_lo) * f_scale, (float)(SAMPLE_BINS - 1u))); };
             u64 above = 0;
-            each_logit(xs, i0, i1, [&](float v, uint32_t i) {
+            each_logit(xs, cnt, [&](float v, uint32_t i) {
                 const float b = R.bin_of(v);
                 if (!(b < f_hi) || (by_k && !cut.keeps(logit_key(v), base + i))) return;
                 const u64 w = Row::steps(R.order(v));
@@ -838,11 +837,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     auto value = [&](float v, uint32_t i) -> u64 {
         const float y = R.order(v);
         if (!Row::weighs(y) || (cuts && !cut.keeps(logit_key(v), base + i))) return 0ull;
-        if (min_p > 0.f && v != m && !(exp2f(y) >= min_p)) return 0ull;
+        if (min_p > 0.f && v != m && !(ex2(y) >= min_p)) return 0ull;
         return Row::steps(y);
     };
     u64 mine = 0, total;
-    each_logit(xs, i0, i1, [&](float v, uint32_t i) { mine += value(v, i); });
+    for (uint32_t i = i0; i < i1; i++) mine += value(xs[i], i);
     const u64 bef = R.before_all(mine, total), target = target_of(total);
     if (bef <= target && bef + mine > target) {
         u64 s = bef;
