@@ -2,20 +2,23 @@
 // number. Contract: include/strix_serve.h. Stands beside the greedy argmax (argmax.cu).
 //
 // A row lives in the shared memory of a cluster of blocks, so the logits are read from HBM once and every question about them
-// is a pass over on-chip data: what bounds a draw is the number of passes and cluster barriers (about a microsecond each), not the
-// 4 bytes a logit.
+// is a pass over on-chip data: what bounds a draw is the number of passes and cluster barriers (half a microsecond to a microsecond
+// each), not the 4 bytes a logit. (Reading the logits from L2 in every pass, so that more rows run at once, was slower: 58 against
+// 52 us at 64 rows of 151936, 60 against 45 at 16 of 262147.)
 //
 // Nothing as long as the row is sorted. What top-k and top-p keep is, in the order (logit, lower index first), everything down to
-// one cut (key, index). The cut is found from a histogram of log2 weight (y = (x - max) log2(e) / T; 2048 bins over the 41
-// binary orders that a weight in steps of 2^-40 can have; logits below that have no weight and no part in anything):
+// one cut (key, index). The cut is found from a histogram of log2 weight (y = (x - max) log2(e) / T; 2048 bins over the 16
+// binary orders below the maximum, which few tokens reach and where most cuts lie; over all 41 that a weight in steps of 2^-40
+// can have if the cut is not among those; logits below have no weight and no part in anything):
 //   top-k: the bin in which the count passes k;
-//   top-p: a bin's mass is its count times its middle weight to within SAMPLE_DELTA, so the counts bound where the mass
-//          passes top_p: mostly a few bins.
+//   top-p: a bin's mass is its count times its middle weight to within half a bin, so the counts bound where the mass passes
+//          top_p of the sum over all, which the same pass takes: mostly a few bins.
 // If all that the cut may leave is at most SAMPLE_CAP tokens, they are gathered in one block, sorted and the draw ends there.
 // Otherwise the uncertain bins alone are resolved: exact masses on 2048 finer bins, then the tokens of one of those are
 // sorted, or, where they are too many (logits that came from 16 bits have thousands of equal values), the cut is bisected
 // over their keys. The draw itself is a sum over the row in index order.
-// Weights are summed as 64-bit integers in steps of 2^-40, so no sum depends on its order, and neither does the draw.
+// Weights are summed as 64-bit integers in steps of 2^-40 (the sum over all as f32 within a thread's stretch, whose order is
+// fixed), so no sum depends on the order of atomics, and neither does the draw.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -35,7 +38,7 @@ constexpr int SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr uint32_t SAMPLE_BINS = 2048, SAMPLE_CAP = 2048;
 constexpr int SAMPLE_BPT = SAMPLE_BINS / SAMPLE_THREADS;  // bins, or list entries, of a thread
 constexpr float SAMPLE_ORDERS = 41.f;       // weights below 2^-41 round to no step of 2^-40
-constexpr float SAMPLE_DELTA = 0.008f;      // half a bin: 41 ln 2 / 2048 / 2 = 0.0069, and f32 sums over 2048 bins
+constexpr float SAMPLE_NEAR = 16.f;         // binary orders of the first histogram
 
 struct SampleArgs {
     const float *x;
@@ -89,18 +92,26 @@ struct OpMax {
     __device__ u64 operator()(u64 p, u64 q) const { return p > q ? p : q; }
 };
 
-// f(logit, its place in the block) for every logit of the block, shared out in words of four (xs is padded to one with -inf)
-template <typename F>
-__device__ __forceinline__ void each_logit(const float *xs, uint32_t cnt, F f) {
+// A block's logits in shared memory, padded with -inf to a multiple of four; no NaN among them.
+struct Logits {
+    const float *p;
+    uint32_t cnt;
+    __device__ float operator[](uint32_t i) const { return p[i]; }
+    // f(logit, its place) for those in [i0, i1) (i0 a multiple of four) that fall to this one of `takers`, in words of four
+    template <typename F>
+    __device__ __forceinline__ void each(uint32_t i0, uint32_t i1, uint32_t taker, uint32_t takers, F f) const {
 #pragma unroll 4
-    for (uint32_t i = 4u * threadIdx.x; i < cnt; i += 4u * SAMPLE_THREADS) {
-        const float4 v = *reinterpret_cast<const float4 *>(xs + i);
-        f(v.x, i);
-        f(v.y, i + 1u);
-        f(v.z, i + 2u);
-        f(v.w, i + 3u);
+        for (uint32_t i = i0 + 4u * taker; i < i1; i += 4u * takers) {
+            const float4 v = *reinterpret_cast<const float4 *>(p + i);
+            f(v.x, i);
+            f(v.y, i + 1u);
+            f(v.z, i + 2u);
+            f(v.w, i + 3u);
+        }
     }
-}
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const { each(0u, cnt, threadIdx.x, SAMPLE_THREADS, f); }
+};
 
 // One block's view of its row, which C blocks share. Two rules keep the cluster together: what a block shows to the others
 // (hist, fine, list, xch, found, fmax) is not written again before a cluster barrier behind their reads, and every branch
@@ -108,9 +119,9 @@ __device__ __forceinline__ void each_logit(const float *xs, uint32_t cnt, F f) {
 template <int C>
 struct SampleRow {
     SampleShared &S;
-    const float *xs;                // this block's logits
-    uint32_t base, cnt;             // index of the first, how many
-    float m, c, cb, min_p;          // maximum; log2(e) / T; bins to a unit of logit
+    const Logits xs;                // this block's
+    uint32_t base;                  // index of the first
+    float m, c, cb;                 // maximum; log2(e) / T; bins to a unit of logit
     uint32_t turn, wturn;
 
     __device__ static uint32_t me() { return C > 1 ? cg::this_cluster().block_rank() : 0u; }
@@ -125,6 +136,7 @@ struct SampleRow {
     }
     // log2 of a weight, below -SAMPLE_ORDERS where there is none (NaN for -inf at an infinite temperature: no weight either)
     __device__ float order(float x) const { return (x - m) * c; }
+    __device__ void bins_over(float orders) { cb = c * (SAMPLE_BINS / orders); }
     __device__ static bool weighs(float y) { return y >= -SAMPLE_ORDERS; }
     // the weight in steps of 2^-40 (rounded to nearest), as units of 2^20 and the rest
     __device__ static void split(float y, uint32_t &hi, uint32_t &lo) {
@@ -265,31 +277,26 @@ struct SampleRow {
             }
     }
     // Puts the tokens that `want` names into this block's list (descending key, index), ends behind a cluster barrier, and
-    // brings the other blocks' lists into rank 0's. Returns how many there are (to rank 0 only). `told` is what the block
-    // tells the others by the same barrier: their sum comes back through it.
+    // brings the other blocks' lists into rank 0's. Returns how many there are (to rank 0 only).
     template <typename F>
-    __device__ uint32_t gather(F want, u64 &told) {
-        each_logit(xs, cnt, [&](float x, uint32_t i) {
+    __device__ uint32_t gather(F want) {
+        xs.each([&](float x, uint32_t i) {
             if (!want(x, base + i)) return;
             const uint32_t at = atomicAdd(&S.n_list, 1u);
             if (at < SAMPLE_CAP) S.list.e[at] = (u64)(~logit_key(x)) << 32 | (base + i);
         });
-        if (threadIdx.x == 0) S.xch[turn][0] = told;
         csync();
         uint32_t n = min(S.n_list, SAMPLE_CAP);
         if constexpr (C > 1) {
             if (me() == 0) {
                 const uint32_t lane = threadIdx.x & 31u, w = threadIdx.x >> 5, r = w & (C - 1), part = w / C;
                 const uint32_t k = far(&S.n_list, lane & (C - 1));
-                told = far(&S.xch[turn][0], lane & (C - 1));
                 uint32_t upto = k;
 #pragma unroll
                 for (int o = 1; o < C; o <<= 1) {
                     const uint32_t p = __shfl_up_sync(0xffffffffu, upto, o);
                     if ((int)(lane & (C - 1)) >= o) upto += p;
                 }
-#pragma unroll
-                for (int o = C / 2; o > 0; o >>= 1) told += __shfl_xor_sync(0xffffffffu, told, o);
                 n = __shfl_sync(0xffffffffu, upto, C - 1);
                 const uint32_t kr = __shfl_sync(0xffffffffu, k, r), at = __shfl_sync(0xffffffffu, upto, r) - kr;
                 if (r > 0u) {
@@ -299,16 +306,16 @@ struct SampleRow {
                 n = min(n, SAMPLE_CAP);
                 __syncthreads();
             }
-            turn ^= 1u;
         }
         return n;
     }
 };
 
-// The cut: kept are the tokens with a larger key, and those with this key up to this index.
+// The cut: kept are the tokens with a larger logit, and those with this one up to this index.
 struct Cut {
-    uint32_t key, last;
-    __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
+    float x;
+    uint32_t last;
+    __device__ bool keeps(float v, uint32_t i) const { return v > x || (v == x && i <= last); }
 };
 
 template <int C>
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     using Row = SampleRow<C>;
     extern __shared__ __align__(16) uint8_t raw[];
     SampleShared &S = *reinterpret_cast<SampleShared *>(raw);
-    float *xs = reinterpret_cast<float *>(raw + sizeof(SampleShared));
+    float *own = reinterpret_cast<float *>(raw + sizeof(SampleShared));  // the block's logits
     const uint32_t rank = Row::me(), t = threadIdx.x, lane = t & 31u, row = blockIdx.x / C;
     const uint32_t base = min(A.n, rank * A.per), cnt = min(A.n, base + A.per) - base;
     const float *x = A.x + (size_t)row * A.stride + base;
@@ -326,33 +333,23 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     const float u = A.u[row];
     const bool greedy = !(temp > 0.f);
 
-    // the row into shared memory, its maximum
+    // the row into shared memory (NaN as -inf), its maximum
     float m = -INFINITY;
-    if ((reinterpret_cast<uintptr_t>(x) & 15u) == 0) {
-        const uint32_t n4 = cnt / 4;
-        const float4 *x4 = reinterpret_cast<const float4 *>(x);
-        float4 *s4 = reinterpret_cast<float4 *>(xs);
+    const uint32_t quads = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 ? cnt / 4u : 0u;
 #pragma unroll 8
-        for (uint32_t i = t; i < n4; i += SAMPLE_THREADS) {
-            float4 v = __ldcs(x4 + i);
-            v = make_float4(fmaxf(v.x, -INFINITY), fmaxf(v.y, -INFINITY), fmaxf(v.z, -INFINITY), fmaxf(v.w, -INFINITY));  // NaN to -inf
-            s4[i] = v;
-            m = fmaxf(fmaxf(m, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
-        }
-        for (uint32_t i = n4 * 4 + t; i < cnt; i += SAMPLE_THREADS) {
-            const float v = fmaxf(x[i], -INFINITY);
-            xs[i] = v;
-            m = fmaxf(m, v);
-        }
-    } else {
-#pragma unroll 8
-        for (uint32_t i = t; i < cnt; i += SAMPLE_THREADS) {
-            const float v = fmaxf(__ldcs(x + i), -INFINITY);
-            xs[i] = v;
-            m = fmaxf(m, v);
-        }
+    for (uint32_t i = t; i < quads; i += SAMPLE_THREADS) {
+        float4 v = __ldcs(reinterpret_cast<const float4 *>(x) + i);
+        v = make_float4(fmaxf(v.x, -INFINITY), fmaxf(v.y, -INFINITY), fmaxf(v.z, -INFINITY), fmaxf(v.w, -INFINITY));
+        reinterpret_cast<float4 *>(own)[i] = v;
+        m = fmaxf(fmaxf(m, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
     }
-    if (t < (-cnt & 3u)) xs[cnt + t] = -INFINITY;
+#pragma unroll 8
+    for (uint32_t i = 4u * quads + t; i < cnt; i += SAMPLE_THREADS) {
+        const float v = fmaxf(__ldcs(x + i), -INFINITY);
+        own[i] = v;
+        m = fmaxf(m, v);
+    }
+    if (t < (-cnt & 3u)) own[cnt + t] = -INFINITY;
     for (uint32_t i = t; i < SAMPLE_BINS / 2; i += SAMPLE_THREADS) S.hist[i] = 0u;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -375,12 +372,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     // this thread's stretch where index order matters (of an odd length: no bank conflicts)
     const uint32_t seg = ((cnt + SAMPLE_THREADS - 1) / SAMPLE_THREADS) | 1u, i0 = min(cnt, t * seg), i1 = min(cnt, i0 + seg);
     if (m == INFINITY) {  // only the infinite ones have weight: as if they were the only ones
-        for (uint32_t i = t; i < cnt; i += SAMPLE_THREADS) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
+        for (uint32_t i = t; i < cnt; i += SAMPLE_THREADS) own[i] = own[i] == INFINITY ? 0.f : -INFINITY;
         m = 0.f;
         __syncthreads();
     }
+    const Logits xs{own, cnt};
     const float c = fminf(1.4426950408889634f / temp, 1.0e36f);
-    Row R{S, xs, base, cnt, m, c, c * (SAMPLE_BINS / SAMPLE_ORDERS), min_p, 0u, 0u};
+    Row R{S, xs, base, m, c, 0.f, 0u, 0u};
 
     if (m == -INFINITY || greedy) {  // no token, or the first of the largest
         u64 best[1] = {0xffffffffull};
@@ -404,42 +402,62 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         const u64 g = f < 1.0e19 ? (u64)f : total;
         return g < total ? g : total - 1;
     };
-    Cut cut{0u, 0xffffffffu};
+    Cut cut{-INFINITY, 0xffffffffu};
     const bool nucleus = top_p < 1.f;
     if ((top_k > 0 && (uint32_t)top_k < A.n) || nucleus) {
-        // ---- histogram of log2 weight
+        // ---- histogram of log2 weight, near the maximum, or over all orders
         const uint32_t hist_at = smem_u32(&S.hist[0]);
-        each_logit(xs, cnt, [&](float v, uint32_t) {
-            // (in assembly for the predicated add: no branch around it)
-            const float b = R.bin_of(v);
-            const uint32_t k = Row::bin(b);
-            asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.f32 p, %0, %1;\n\t@p red.shared.add.u32 [%2], %3;\n\t}" ::"f"(b), "f"((float)SAMPLE_BINS),
-                         "r"(hist_at + (k / 2u) * 4u), "r"((k & 1u) ? 0x10000u : 1u)
-                         : "memory");
-        });
-        Row::csync();
-        // a thread's bins: counts and middle masses up to each (f32 sums in a fixed order: they only bound)
-        uint32_t h[SAMPLE_BPT] = {};
+        const bool want_k = top_k > 0 && (uint32_t)top_k < A.n;
+        uint32_t h[SAMPLE_BPT], cc[SAMPLE_BPT], n_weight = 0;
+        float sm[SAMPLE_BPT], a_total = 0.f, delta = 0.f, mid = 0.f;
+        u64 all = 0;  // the weights of the whole row
+        bool by_k = false;
+        for (float orders = SAMPLE_NEAR;; orders = SAMPLE_ORDERS) {
+            R.bins_over(orders);
+            mid = orders / SAMPLE_BINS;
+            delta = orders * (0.69314718f / (2 * SAMPLE_BINS)) * 1.1f + 1.0e-4f;  // half a bin, and f32 sums over the bins
+            float sum = 0.f;
+            auto count = [&](float v) {  // (in assembly for the predicated add: no branch around it)
+                const float b = R.bin_of(v);
+                const uint32_t k = Row::bin(b);
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.f32 p, %0, %1;\n\t@p red.shared.add.u32 [%2], %3;\n\t}" ::"f"(b), "f"((float)SAMPLE_BINS),
+                             "r"(hist_at + (k / 2u) * 4u), "r"((k & 1u) ? 0x10000u : 1u)
+                             : "memory");
+            };
+            if (nucleus && orders == SAMPLE_NEAR)
+                xs.each([&](float v, uint32_t) {
+                    count(v);
+                    sum += ex2(fmaxf(R.order(v), -200.f));
+                });
+            else
+                xs.each([&](float v, uint32_t) { count(v); });
+            if (nucleus && orders == SAMPLE_NEAR) {
+                all = __float2ull_rn(sum * 1099511627776.f);  // (at most 128 weights)
+                all = R.sum(all);                             // (its cluster barrier ends the histogram as well)
+                if (C == 1) __syncthreads();
+            } else {
+                Row::csync();
+            }
+            // a thread's bins: counts and middle masses up to each (f32 sums in a fixed order: they only bound)
 #pragma unroll
-        for (int r = 0; r < C; r++) {
-            const uint2 q = Row::far(reinterpret_cast<const uint2 *>(&S.hist[0]) + t, r);
-            h[0] += q.x & 0xffffu;
-            h[1] += q.x >> 16;
-            h[2] += q.y & 0xffffu;
-            h[3] += q.y >> 16;
-        }
-        uint32_t cc[SAMPLE_BPT];
-        float sm[SAMPLE_BPT];
-        const float mid = SAMPLE_ORDERS / SAMPLE_BINS;
-        uint32_t n_weight, c_all = 0;
-        float a_total, s_all = 0.f;
+            for (int j = 0; j < SAMPLE_BPT; j++) h[j] = 0u;
 #pragma unroll
-        for (int j = 0; j < SAMPLE_BPT; j++) {
-            c_all += h[j];
-            s_all = fmaf((float)h[j], exp2f(-((float)(SAMPLE_BPT * t + j) + 0.5f) * mid), s_all);
-            cc[j] = c_all;
-            sm[j] = s_all;
-        }
+            for (int r = 0; r < C; r++) {
+                const uint2 q = Row::far(reinterpret_cast<const uint2 *>(&S.hist[0]) + t, r);
+                h[0] += q.x & 0xffffu;
+                h[1] += q.x >> 16;
+                h[2] += q.y & 0xffffu;
+                h[3] += q.y >> 16;
+            }
+            uint32_t c_all = 0;
+            float s_all = 0.f;
+#pragma unroll
+            for (int j = 0; j < SAMPLE_BPT; j++) {
+                c_all += h[j];
+                s_all = fmaf((float)h[j], ex2(-((float)(SAMPLE_BPT * t + j) + 0.5f) * mid), s_all);
+                cc[j] = c_all;
+                sm[j] = s_all;
+            }
         {
             uint32_t ci = c_all;
             float si = s_all;
@@ -483,11 +501,17 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                 sm[j] += sb;
             }
         }
-        const bool by_k = top_k > 0 && (uint32_t)top_k < n_weight;
+            // is the cut within these bins?
+            by_k = want_k && (uint32_t)top_k < n_weight;
+            if (orders == SAMPLE_ORDERS || by_k || (!want_k && (double)a_total * (1.0 - delta) * 1099511627776.0 >= (double)top_p * (double)all)) break;
+            Row::csync();  // (all have read the counts)
+            for (uint32_t i = t; i < SAMPLE_BINS / 2; i += SAMPLE_THREADS) S.hist[i] = 0u;
+            __syncthreads();
+        }
         const uint32_t k = by_k ? (uint32_t)top_k : n_weight;
-        // S.first: the bin of the k-th token; S.second: the first bin up to which the masses surely reach top_p of all of them
-        // (without top-k, where all is all); and the tokens up to either
-        const float sure = top_p * a_total * ((1.f + SAMPLE_DELTA) / (1.f - SAMPLE_DELTA));
+        // S.first: the bin of the k-th token; S.second: the first bin up to which the masses surely reach top_p of all
+        // (without top-k); and the tokens up to either
+        const float sure = (float)((double)top_p * (double)all * (1.0 / 1099511627776.0)) / (1.f - delta);
         if (t == 0) S.found[0] = n_weight;
         __syncthreads();
 #pragma unroll
@@ -499,7 +523,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                     S.found[0] = cc[j];
                     S.found[1] = c_prev;
                 }
-            } else if (h[j] && sm[j] >= sure) {
+            } else if (nucleus && h[j] && sm[j] >= sure) {
                 atomicMin(&S.second, SAMPLE_BPT * t + j);
             }
         }
@@ -513,19 +537,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
 
         if (n_last <= SAMPLE_CAP) {
             // ---- few candidates: the whole draw in one block
-            // (top-p of the whole row needs the sum of all weights: f32 over a thread's hundred or fewer, integers beyond)
-            u64 all = 0;
             const float stop = (float)(b_last + 1u);
-            uint32_t n;
-            if (by_k) {
-                n = R.gather([&](float v, uint32_t) { return R.bin_of(v) < stop; }, all);
-            } else {
-                float sum = 0.f;
-                each_logit(xs, cnt, [&](float v, uint32_t) { sum += ex2(fmaxf(R.order(v), -200.f)); });
-                all = __float2ull_rn(sum * 1099511627776.f);
-                (void)R.before(all, all);
-                n = R.gather([&](float v, uint32_t) { return R.bin_of(v) < stop; }, all);
-            }
+            const uint32_t n = R.gather([&](float v, uint32_t) { return R.bin_of(v) < stop; });
             if (rank == 0) {
                 const uint32_t kk = by_k ? min(n, k) : n;
                 if (n <= 64u) {
@@ -628,18 +641,18 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             Row::csync();
             const u64 f = Row::far(&S.found[1], 0);
             Row::csync();
-            return Cut{(uint32_t)(f >> 32), (uint32_t)f};
+            return Cut{key_logit((uint32_t)(f >> 32)), (uint32_t)f};
         };
         // the index of the quota-th kept token with this key
         auto tie_index = [&](uint32_t key, const Cut &old, u64 quota) {
             u64 mine = 0, all;
-            for (uint32_t i = i0; i < i1; i++) mine += logit_key(xs[i]) == key && old.keeps(key, base + i);
+            for (uint32_t i = i0; i < i1; i++) mine += logit_key(xs[i]) == key && old.keeps(xs[i], base + i);
             const u64 bef = R.before_all(mine, all);
             u64 at[1] = {0};
             if (bef < quota && quota <= bef + mine) {
                 u64 q = bef;
                 for (uint32_t i = i0; i < i1; i++)
-                    if (logit_key(xs[i]) == key && old.keeps(key, base + i) && ++q == quota) {
+                    if (logit_key(xs[i]) == key && old.keeps(xs[i], base + i) && ++q == quota) {
                         at[0] = base + i;
                         break;
                     }
@@ -660,7 +673,6 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             lo = ~(uint32_t)r[0];
             hi = (uint32_t)r[1];
         };
-        u64 nothing = 0;
         if (by_k) {
             const uint32_t quota = k - above_k;  // tokens of the bin that stay
             auto in = [&](float v, uint32_t) {
@@ -668,7 +680,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                 return b < (float)SAMPLE_BINS && Row::bin(b) == bk;
             };
             if (n_last - above_k <= SAMPLE_CAP) {
-                const uint32_t n = R.gather(in, nothing);
+                const uint32_t n = R.gather(in);
                 if (rank == 0) R.sort_list(n);
                 const u64 e = rank == 0 ? S.list.e[quota - 1] : 0ull;
                 cut = told(rank == 0 && t == 0, ~(uint32_t)(e >> 32), (uint32_t)e);
@@ -685,16 +697,17 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                 u64 n = 0;
                 for (uint32_t i = i0; i < i1; i++) n += in(xs[i], 0u) && logit_key(xs[i]) > lo;
                 n = R.sum(n);
-                cut = Cut{lo, tie_index(lo, cut, quota - n)};
+                cut = Cut{key_logit(lo), tie_index(lo, cut, quota - n)};
             }
         }
         if (nucleus) {
-            u64 all = 0;
-            each_logit(xs, cnt, [&](float v, uint32_t i) {
-                const float y = R.order(v);
-                if (!by_k || cut.keeps(logit_key(v), base + i)) all += Row::steps(y);
-            });
-            all = R.sum(all);
+            if (by_k) {
+                float sum = 0.f;
+                xs.each([&](float v, uint32_t i) {
+                    if (cut.keeps(v, base + i)) sum += ex2(fmaxf(R.order(v), -200.f));
+                });
+                all = R.sum(__float2ull_rn(sum * 1099511627776.f));
+            }
             const double need = (double)top_p * (double)all;
             // bins that are surely kept, and from where on surely nothing is
             if (t == 0) {
@@ -702,7 +715,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                 S.second = bk;
             }
             __syncthreads();
-            const float n1 = (float)(need * (1.0 / 1099511627776.0)), lo_d = n1 / (1.f + SAMPLE_DELTA), hi_d = n1 / (1.f - SAMPLE_DELTA);
+            const float n1 = (float)(need * (1.0 / 1099511627776.0)), lo_d = n1 / (1.f + delta), hi_d = n1 / (1.f - delta);
 #pragma unroll
             for (int j = 0; j < SAMPLE_BPT; j++) {
                 if (h[j] && sm[j] < lo_d) atomicMax(&S.first, SAMPLE_BPT * t + j + 1u);  // (the bin stays)
@@ -720,14 +733,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             __syncthreads();
             const float f_lo = (float)b_lo, f_hi = (float)(b_hi + 1u), f_scale = (float)SAMPLE_BINS / (f_hi - f_lo);
             auto fine = [&](float b) { return Row::bin(fminf((b - f_lo) * f_scale, (float)(SAMPLE_BINS - 1u))); };
-            u64 above = 0;
-            each_logit(xs, cnt, [&](float v, uint32_t i) {
+            float above_f = 0.f;
+            xs.each([&](float v, uint32_t i) {
                 const float b = R.bin_of(v);
-                if (!(b < f_hi) || (by_k && !cut.keeps(logit_key(v), base + i))) return;
-                const u64 w = Row::steps(R.order(v));
                 if (b < f_lo) {
-                    above += w;
-                } else {
+                    above_f += ex2(R.order(v));
+                } else if (b < f_hi && (!by_k || cut.keeps(v, base + i))) {
+                    const u64 w = Row::steps(R.order(v));
                     const uint32_t f = fine(b);
                     atomicAdd(&S.fine.count[f], 1u);
                     uint32_t *half = reinterpret_cast<uint32_t *>(&S.fine.mass[f]);
@@ -736,7 +748,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                     if (high) atomicAdd(half + 1, high);
                 }
             });
-            above = R.sum(above);
+            const u64 above = R.sum(__float2ull_rn(above_f * 1099511627776.f));
             if constexpr (C == 1) __syncthreads();  // (in a cluster, the sum's barrier ends the histogram)
             u64 g[SAMPLE_BPT] = {}, bef[SAMPLE_BPT];
             uint32_t q[SAMPLE_BPT] = {};
@@ -778,10 +790,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                 const Cut old = cut;
                 auto in = [&](float v, uint32_t i) {
                     const float b = R.bin_of(v);
-                    return b >= f_lo && b < f_hi && fine(b) == fb && (!by_k || old.keeps(logit_key(v), i));
+                    return b >= f_lo && b < f_hi && fine(b) == fb && (!by_k || old.keeps(v, i));
                 };
                 if (n_fine <= SAMPLE_CAP) {
-                    const uint32_t n = R.gather(in, nothing);
+                    const uint32_t n = R.gather(in);
                     if (rank == 0) {
                         R.sort_list(n);
                         u64 w[SAMPLE_BPT], mine = 0, dummy;
@@ -826,44 +838,59 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                     // the j-th equal (from 0) stays if s + j w1 < need
                     double j = w1 ? ceil((need - (double)s) / (double)w1) : (double)v[1];
                     j = fmin(fmax(j, 1.0), (double)v[1]);
-                    cut = Cut{lo, tie_index(lo, old, (u64)j)};
+                    cut = Cut{key_logit(lo), tie_index(lo, old, (u64)j)};
                 }
             }
         }
     }
 
     // ---- the draw, in index order
-    const bool cuts = cut.key != 0u;
-    auto value = [&](float v, uint32_t i) -> u64 {
-        const float y = R.order(v);
-        if (!Row::weighs(y) || (cuts && !cut.keeps(logit_key(v), base + i))) return 0ull;
-        if (min_p > 0.f && v != m && !(ex2(y) >= min_p)) return 0ull;
-        return Row::steps(y);
+    const float low = min_p > 0.f ? min_p : 0.f;
+    auto value = [&](float v, uint32_t i) -> float {
+        const float w = ex2(fmaxf(R.order(v), -200.f));
+        return cut.keeps(v, base + i) && (w >= low || v == m) ? w : 0.f;
     };
-    u64 mine = 0, total;
-    for (uint32_t i = i0; i < i1; i++) mine += value(xs[i], i);
-    const u64 bef = R.before_all(mine, total), target = target_of(total);
-    if (bef <= target && bef + mine > target) {
-        u64 s = bef;
-        for (uint32_t i = i0; i < i1; i++) {
-            const u64 w = value(xs[i], i);
-            s += w;
-            if (s > target) {
-                write(base + i, w, total);
-                break;
+    // a warp sums a stretch of neighbours (f32 within a lane, integers beyond); the block that has the target goes over the stretch
+    // that has it once more, a few neighbours to a thread. What f32 rounds differently there moves the end of the stretch by
+    // 2^-24 of it: a target beyond that end is the stretch's last kept token.
+    const uint32_t w = t >> 5, len = ((cnt + SAMPLE_WARPS - 1) / SAMPLE_WARPS + 3u) & ~3u, w0 = min(cnt, w * len), w1 = min(cnt, w0 + len);
+    float lane_sum = 0.f;
+    xs.each(w0, w1, lane, 32u, [&](float v, uint32_t i) { lane_sum += value(v, i); });
+    u64 mine = __float2ull_rn(lane_sum * 1099511627776.f), total;
+    u64 b = R.before_all(mine, total);  // (threads are in warp order, so this is where the warp's stretch begins, at its first lane)
+    const u64 target = target_of(total);
+    u64 sum = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    b = __shfl_sync(0xffffffffu, b, 0);
+    if (t == 0) S.first = SAMPLE_WARPS;
+    __syncthreads();
+    if (lane == 0 && b <= target && b + sum > target) {
+        S.first = w;
+        S.found[0] = b;
+    }
+    __syncthreads();
+    if (S.first < SAMPLE_WARPS) {  // (in one block of the cluster)
+        const uint32_t s0 = min(cnt, S.first * len), s1 = min(cnt, s0 + len), part = (len + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
+        const uint32_t j0 = min(s1, s0 + t * part), j1 = min(s1, j0 + part);
+        auto steps = [](float w) { return w > 0.f ? max(1ull, __float2ull_rn(w * 1099511627776.f)) : 0ull; };  // (something is kept here)
+        mine = 0;
+        for (uint32_t i = j0; i < j1; i++) mine += steps(value(xs[i], i));
+        u64 of_part;
+        u64 at = S.found[0] + R.before(mine, of_part);
+        const u64 end = S.found[0] + of_part, goal = target < end ? target : end - 1u;
+        if (at <= goal && at + mine > goal) {
+            for (uint32_t i = j0; i < j1; i++) {
+                const u64 v = steps(value(xs[i], i));
+                at += v;
+                if (at > goal) {
+                    write(base + i, v, total);
+                    break;
+                }
             }
         }
     }
     Row::csync();
-}
-
-// Blocks to a row. More blocks shorten every pass, a cluster barrier costs the same; the row has to fit their shared memory, and
-// with many rows two blocks to an SM hide each other's barriers.
-static uint32_t sample_cluster(uint32_t n, uint32_t rows, size_t smem_optin) {
-    const size_t room = (smem_optin - sizeof(SampleShared) - 1024) / 4;
-    uint32_t c = 1;
-    while (c < 8 && (size_t)(n + c - 1) / c > (rows * c >= 296 ? room : 4096)) c *= 2;
-    return c;
 }
 
 template <int C>
@@ -890,10 +917,14 @@ static cudaError_t sample_launch(strix_cuda *h, const SampleArgs &A, uint32_t ro
     return cudaLaunchKernelEx(&cfg, sample_kernel<C>, A);
 }
 
+// A row takes as many blocks as make it 4096 logits or fewer to a block, at most 8: more blocks shorten every pass, a barrier among
+// them costs the same (4 instead of 8 for 151936 logits: 18.7 against 15.8 us a row, 80 against 69 for 64, in an earlier form).
 cudaError_t launch_sample(strix_cuda *h, const float *d_x, uint32_t n, size_t stride, uint32_t rows, const strix_sample_params &p,
                           const float *d_u, uint32_t *d_ids, float *d_probs, cudaStream_t stream) {
-    const uint32_t c = sample_cluster(n, rows, h->smem_optin);
+    uint32_t c = 1;
+    while (c < 8 && (n + c - 1) / c > 4096) c *= 2;
     const SampleArgs A{d_x, stride, n, ((n + c - 1) / c + 3u) & ~3u, p, d_u, d_ids, d_probs};
+    static_assert(sizeof(SampleShared) + (STRIX_SAMPLE_MAX_N / 8 + 4) * 4 <= 231000, "the longest row fits eight blocks");
     ProfScope prof(h, stream, "sample");
     switch (c) {
         case 1: return sample_launch<1>(h, A, rows, stream);

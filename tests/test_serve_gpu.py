@@ -461,6 +461,21 @@ def test_sample_all_parameters(torch, accel, n):
     check_sample(x, u, ids, probs, TP=TP)
 
 
+@pytest.mark.parametrize("rows,n", [(31, 33000), (67, 20001), (70, 140000), (150, 5000), (300, 1500), (3, 393216), (32, 300000)])
+def test_sample_many_rows(torch, accel, rows, n):
+    """More rows than run at once, unaligned ones too (odd n), and the longest."""
+    rng = np.random.RandomState(rows)
+    x = (rng.randn(rows, n) * 2.5).astype(np.float32)
+    x[0, ::7] = np.nan
+    x[1, [3, n - 1]] = np.inf
+    x[2] = np.float32(0.25) * np.round(x[2] * 4)          # ties
+    u = rng.rand(rows).astype(np.float32)
+    T, K = rng.choice([0.0, 0.5, 1.0, 1.5], rows), rng.choice([0, 0, 50, 3000, n // 2], rows)
+    TP, MP = rng.choice([0.5, 0.9, 1.0], rows), rng.choice([0.0, 0.02], rows)
+    ids, probs = sample(torch, accel, x, u, T, K, TP, MP)
+    check_sample(x, u, ids, probs, T, K, TP, MP)
+
+
 def test_sample_ties(torch, accel):
     """Logits from a few values only (whole rows of ties): top-k and top-p cut inside the ties, lower indices first."""
     rng = np.random.RandomState(1)
