@@ -5,7 +5,8 @@
 // a decode step is one launch and a chain of four dependent loads (row0, ctx, page id, old scale).
 //
 // Work split. The cache side goes by pages, because a page and head share one scale: a block takes one (page, head) of k
-// or v, holds its new rows in registers, reduces their largest magnitude and stores codes. Which page a block has follows
+// or v (four heads of it in turn, where sequences bring many rows), holds its new rows in registers, reduces their largest
+// magnitude and stores codes. Which page a block has follows
 // from a row: a unit is RU consecutive rows and owns the pages whose first new row lies among them. RU = page_tokens when
 // sequences bring many rows (a block for each page), 1 when they bring few (a block for each row, most of them one-row pages).
 // The q side has no scale to share: a warp takes one row and a few heads, so that the angles of a row are computed once
@@ -34,7 +35,7 @@ struct AppendArgs {
     double turn[8];  // (theta^(-2/hd))^(2^b), b = 0..7; angles in turns start from 1 / (2 pi)
     float eps;
     int rope, norm_v;
-    uint32_t n_heads, kv_blocks, unit_rows, heads_per_warp, q_chunks, vec;  // vec: every f32 row starts on 16 bytes
+    uint32_t n_heads, kv_blocks, unit_rows, kv_group, heads_per_warp, q_chunks, vec;  // vec: every f32 row starts on 16 bytes
 };
 
 // The lanes that share a row: HD / 2 pairs, four to a lane, in a power-of-two group of lanes.
@@ -72,7 +73,9 @@ __device__ __forceinline__ float inv_rms(const Eight &x, float eps) {
     for (int i = 0; i < 4; i++) ss = fmaf(x.a[i], x.a[i], fmaf(x.b[i], x.b[i], ss));
 #pragma unroll
     for (int o = RowLanes<HD>::GROUP / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    return 1.0f / sqrtf(ss / (float)HD + eps);
+    // (the approximate root and one step of Newton's: within 2^-23)
+    const float s = ss * (1.0f / (float)HD) + eps, r = rsqrtf(s);
+    return s > 0.f && s < 3.0e38f ? r * fmaf(-0.5f * s * r, r, 1.5f) : r;
 }
 
 struct Turn {
@@ -152,62 +155,71 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
     if (blockIdx.x >= A.kv_blocks) {  // ---- q: one row and heads_per_warp heads for each warp
         const uint32_t w = (blockIdx.x - A.kv_blocks) * WARPS + warp, row = w / A.q_chunks, chunk = w - row * A.q_chunks;
         if (row >= V.n_rows) return;
-        frequencies();
+        constexpr int NB = WARPS >= 16 ? 4 : 1;  // heads of a lane group on their way at once: what is in flight bounds a prompt
+        const uint32_t h1 = min(A.n_heads, (chunk + 1u) * A.heads_per_warp);
+        const float *src = A.src_q + (size_t)row * A.ld_q;
+        float *dst = A.dst_q + (size_t)row * A.ld_qo;
+        Eight x[NB];
+        auto fetch = [&](uint32_t h0) {
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const uint32_t hh = h0 + i * R::ROWS + sub;
+                x[i] = {};
+                if (on && hh < h1) load_eight(x[i], src + hh * HD, o0, o1, A.vec);
+            }
+        };
+        uint32_t h0 = chunk * A.heads_per_warp;
+        fetch(h0);
         uint32_t first, end;
         const uint32_t s = seq_of_row(V, row, first, end, bad);
-        if (s < V.n_seq) {
-            const int ctx = V.ctx[s];
-            if (ctx >= 0) {
-                const uint32_t pos = (uint32_t)ctx + (row - first);
-                Turn t;
-                if (A.rope != STRIX_ROPE_NONE) turn_of(t, inv, pos);
-                float4 wa = make_float4(1.f, 1.f, 1.f, 1.f), wb = wa;
-                if (A.q_norm && on) {
-                    Eight n;
-                    load_eight(n, A.q_norm, o0, o1, false);
-                    wa = make_float4(n.a[0], n.a[1], n.a[2], n.a[3]);
-                    wb = make_float4(n.b[0], n.b[1], n.b[2], n.b[3]);
-                }
-                const uint32_t h1 = min(A.n_heads, (chunk + 1u) * A.heads_per_warp);
-                for (uint32_t h0 = chunk * A.heads_per_warp; h0 < h1; h0 += R::ROWS) {
-                    const uint32_t hh = h0 + sub;
-                    const bool mine = on && hh < h1;
-                    Eight x = {};
-                    if (mine) load_eight(x, A.src_q + (size_t)row * A.ld_q + (size_t)hh * HD, o0, o1, A.vec);
-                    if (A.q_norm) {
-                        const float r = inv_rms<HD>(x, A.eps);
-                        const float w8[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+        report_bad(V, bad && lane == 0);
+        if (s >= V.n_seq) return;
+        const int ctx = V.ctx[s];
+        if (ctx < 0) return;
+        frequencies();
+        Turn t;
+        if (A.rope != STRIX_ROPE_NONE) turn_of(t, inv, (uint32_t)ctx + (row - first));
+        Eight n = {};
+        if (A.q_norm && on) load_eight(n, A.q_norm, o0, o1, false);
+        for (;;) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            x.a[i] = x.a[i] * r * w8[i];
-                            x.b[i] = x.b[i] * r * w8[4 + i];
-                        }
+            for (int i = 0; i < NB; i++) {
+                const uint32_t hh = h0 + i * R::ROWS + sub;
+                Eight y = x[i];
+                if (A.q_norm) {
+                    const float r = inv_rms<HD>(y, A.eps);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        y.a[e] = y.a[e] * r * n.a[e];
+                        y.b[e] = y.b[e] * r * n.b[e];
                     }
-                    rotate(x, t, A.rope);
-                    if (!mine) continue;
-                    float *o = A.dst_q + (size_t)row * A.ld_qo + (size_t)hh * HD;
-                    if (A.vec) {
-                        *reinterpret_cast<float4 *>(o + o0) = make_float4(x.a[0], x.a[1], x.a[2], x.a[3]);
-                        *reinterpret_cast<float4 *>(o + o1) = make_float4(x.b[0], x.b[1], x.b[2], x.b[3]);
-                    } else {
+                }
+                rotate(y, t, A.rope);
+                if (!(on && hh < h1)) continue;
+                float *o = dst + hh * HD;
+                if (A.vec) {
+                    *reinterpret_cast<float4 *>(o + o0) = make_float4(y.a[0], y.a[1], y.a[2], y.a[3]);
+                    *reinterpret_cast<float4 *>(o + o1) = make_float4(y.b[0], y.b[1], y.b[2], y.b[3]);
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            o[o0 + i] = x.a[i];
-                            o[o1 + i] = x.b[i];
-                        }
+                    for (int e = 0; e < 4; e++) {
+                        o[o0 + e] = y.a[e];
+                        o[o1 + e] = y.b[e];
                     }
                 }
             }
+            h0 += NB * R::ROWS;
+            if (h0 >= h1) return;
+            fetch(h0);
         }
-        report_bad(V, bad && lane == 0);
-        return;
     }
 
-    // ---- k or v: the pages whose first new row lies in this unit, one head
-    const uint32_t per = 2u * V.n_kv, unit = blockIdx.x / per, which = blockIdx.x - unit * per;
-    const bool is_v = which >= V.n_kv;
-    const uint32_t hh = is_v ? which - V.n_kv : which;
-    const float *src = (is_v ? A.src_v : A.src_k) + (size_t)hh * HD;
+    // ---- k or v: the pages whose first new row lies in this unit, kv_group heads one after the other
+    const uint32_t groups = (V.n_kv + A.kv_group - 1u) / A.kv_group;
+    const uint32_t per = 2u * groups, unit = blockIdx.x / per, which = blockIdx.x - unit * per;
+    const bool is_v = which >= groups;
+    const uint32_t g0 = (is_v ? which - groups : which) * A.kv_group, g1 = min(V.n_kv, g0 + A.kv_group);
+    constexpr bool KEEP = MAXIT <= 4;  // the rows' sines and cosines stay in registers from head to head
     const size_t ld = is_v ? A.ld_v : A.ld_k;
     uint8_t *cache = is_v ? V.v : V.k;
     float *scales = is_v ? V.v_scale : V.k_scale;
@@ -252,6 +264,9 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
             row += cnt;
             continue;
         }
+        Turn turns[KEEP ? MAXIT : 1];
+        for (uint32_t hh = g0; hh < g1; hh++) {
+        const float *src = (is_v ? A.src_v : A.src_k) + (size_t)hh * HD;
         uint8_t *dst = cache + (size_t)page * V.page_bytes + (size_t)hh * V.head_bytes;
         float *scale = TYPE == STRIX_KV_E4M3 ? scales + (size_t)page * V.n_kv + hh : nullptr;
         const float s_old = TYPE == STRIX_KV_E4M3 && slot ? *scale : 0.f;
@@ -260,12 +275,15 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
         auto fetch = [&](uint32_t base) {  // rows base .. base + CHUNK - 1 of the page's new rows into registers
             float m = 0.f;
 #pragma unroll
+            for (int it = 0; it < MAXIT; it++) {  // all on their way before the first is used
+                const uint32_t i = base + it * (WARPS * R::ROWS) + warp * R::ROWS + sub;
+                x[it] = {};
+                if (on && i < cnt) load_eight(x[it], src + (size_t)(row + i) * ld, o0, o1, A.vec);
+            }
+#pragma unroll
             for (int it = 0; it < MAXIT; it++) {
                 const uint32_t i = base + it * (WARPS * R::ROWS) + warp * R::ROWS + sub;
                 if (base + it * (WARPS * R::ROWS) + warp * R::ROWS >= cnt) break;  // (the same for the whole warp)
-                const bool mine = on && i < cnt;
-                x[it] = {};
-                if (mine) load_eight(x[it], src + (size_t)(row + i) * ld, o0, o1, A.vec);
                 if (norm) {
                     const float r = inv_rms<HD>(x[it], A.eps);
 #pragma unroll
@@ -275,8 +293,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
                     }
                 }
                 if (rope != STRIX_ROPE_NONE) {
-                    Turn t;
-                    turn_of(t, inv, (uint32_t)pos + i);
+                    Turn &t = turns[KEEP ? it : 0];
+                    if (!KEEP || hh == g0 || cnt > CHUNK) turn_of(t, inv, (uint32_t)pos + i);
                     rotate(x[it], t, rope);
                 }
 #pragma unroll
@@ -349,7 +367,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
                 fetch(base);
                 store(base, inv_s);
             }
-            __syncthreads();  // `red` is free for the next page
+            __syncthreads();  // `red` is free for the next head or page
+        }
         }
         row += cnt;
     }
@@ -486,11 +505,12 @@ extern "C" int strix_cuda_kv_append_dev(strix_cuda *h, const strix_kv_pages *cac
     const uint64_t n_rows = A.V.n_rows;
     const bool by_page = n_rows > 8ull * A.V.n_seq;
     A.unit_rows = by_page ? A.V.page_tokens : 1u;
-    const uint64_t kvb = (n_rows + A.unit_rows - 1) / A.unit_rows * 2ull * A.V.n_kv;
+    A.kv_group = by_page ? 4u : 1u;
+    const uint64_t kvb = (n_rows + A.unit_rows - 1) / A.unit_rows * 2ull * ((A.V.n_kv + A.kv_group - 1) / A.kv_group);
     const uint32_t hd = A.V.head_dim, rows_at_once = hd == 64 ? 4u : hd <= 128 ? 2u : 1u, warps = by_page ? 16u : 4u;
     uint64_t qb = 0;
     if (d_q) {
-        A.heads_per_warp = rows_at_once * (by_page ? 4u : 1u);
+        A.heads_per_warp = rows_at_once * (by_page ? 8u : 1u);
         A.q_chunks = (n_heads + A.heads_per_warp - 1) / A.heads_per_warp;
         qb = (n_rows * A.q_chunks + warps - 1) / warps;
     }
