@@ -24,35 +24,15 @@
 // parts of the others meet in shared memory at the block's end, and where an item goes on in another block, in the workspace:
 // the last block to arrive joins the parts, in the order of the line. Cuts that would fall into an item of at most PA_SNAP
 // tiles move to its nearer end.
-#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
 #include <atomic>
 
-#include "kv_pages.cuh"
+#include "kv_line.cuh"
 
 namespace strix {
-
-constexpr uint32_t PA_MAX_BLOCKS = 1024;  // tickets at the start of the workspace
-constexpr uint32_t PA_MAX_SEQ = 8192;     // their running tile counts lie in shared memory while a block finds its place
-constexpr uint32_t PA_SNAP = 16;
-constexpr size_t PA_STATIC = 2048;  // 1024 to align the rings, the rest static shared memory and what the system keeps
-
-struct PagedAttnArgs {
-    CUtensorMap k_map, v_map;  // [page][KV head and slot][element]
-    PagedView V;
-    const float *q;
-    float *out;
-    size_t ld_q, ld_out;
-    uint32_t n_heads, group, window, cap;  // cap: tokens a row of the page table can hold
-    uint32_t g_mul, g_shift;               // division by group
-    float scale;
-    uint32_t wm, halves, vec;  // warps of a worker; half tiles of a ring; q and out rows start on 16 bytes
-    uint32_t *ticket;          // [PA_MAX_BLOCKS]
-    float *part;               // [blocks][2][rows of a worker][HD + 2]
-};
 
 // Sizes that follow from the head size, the cache type and the row form (WIDE: 16 rows a warp, else 8).
 template <int HD, int TYPE, bool WIDE>
@@ -87,14 +67,6 @@ struct PaShape {
     }
 };
 
-// What the first warp tells a worker about a tile.
-struct __align__(16) PaTile {
-    uint32_t tile, flags, valid, row0;        // tile of the item; PA_*; one bit for each page of the tile; first row of the block
-    uint32_t seq_first, seq_rows, ctx, head;  // with PA_NEW: first row of the sequence, its new rows, tokens before them, KV head
-    float ks[4], vs[4];                       // the scales of the tile's pages
-};
-enum : uint32_t { PA_NEW = 1, PA_END = 2, PA_WHOLE = 4, PA_HEAD = 8 };  // first / last tile of the segment here; item complete here; begun elsewhere
-
 // What the joins need to know about a worker's open parts.
 struct __align__(16) PaWorker {
     struct Part {
@@ -114,32 +86,6 @@ __device__ __forceinline__ void mma_f16_from0(float (&c)[4], const uint32_t (&a)
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// x0, x1 as f16 (packed) and what that rounding left of them
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
-    hi = f32_to_f16x2(x0, x1);
-    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-    lo = f32_to_f16x2(x0 - h.x, x1 - h.y);
-}
-__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-                     smem_u32(dst)),
-                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-// true in one lane of the warp, in a form that lets the compiler know it is one
-__device__ __forceinline__ bool elect_lane() {
-    uint32_t one;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
-    return one != 0u;
-}
 template <int BYTES>
 __device__ __forceinline__ void lds_words(uint32_t *w, const uint8_t *p) {
     if constexpr (BYTES == 16) {
@@ -151,110 +97,6 @@ __device__ __forceinline__ void lds_words(uint32_t *w, const uint8_t *p) {
     } else {
         w[0] = *reinterpret_cast<const uint32_t *>(p);
     }
-}
-
-// n / group for n < 2^31
-__device__ __forceinline__ uint32_t by_group(const PagedAttnArgs &A, uint32_t n) { return (__umulhi(n, A.g_mul) + n) >> A.g_shift; }
-
-// Tiles of row block mb of a sequence: [lo_tile, lo_tile + n). rb: rows of a block, a power of two.
-template <int TT>
-__device__ __forceinline__ uint32_t block_tiles(const PagedAttnArgs &A, uint32_t rb, uint32_t rows, uint32_t ctx, uint32_t mb,
-                                                uint32_t &lo_tile) {
-    const uint32_t R = rows * A.group, r0 = mb * rb, r1 = min(R, r0 + rb) - 1u;
-    const uint32_t p0 = ctx + by_group(A, r0), p1 = ctx + by_group(A, r1);  // positions of the first and last row (below 2^32)
-    const uint32_t hi = min(A.cap, p1 + 1u);
-    const uint32_t lo = A.window && p0 >= A.window ? p0 + 1u - A.window : 0u;
-    lo_tile = lo / TT;
-    return hi > lo ? (hi + TT - 1u) / TT - lo_tile : 0u;
-}
-
-// A place in the line of tiles.
-struct __align__(16) PaPlace {
-    uint32_t s, first, rows, ctx, mb, head, lo_tile, tiles, at;  // item: tiles of it, `at` the place within
-    uint32_t item0;                                              // the line's index of the item's first tile
-    uint32_t left, pad;                                          // tiles of the worker from here on
-};
-
-__device__ __forceinline__ void load_seq(const PagedAttnArgs &A, uint32_t s, PaPlace &P) {
-    uint32_t end;
-    bool bad = false;
-    P.s = s;
-    seq_rows(A.V, s, P.first, end, bad);
-    P.rows = end - P.first;
-    P.ctx = (uint32_t)A.V.ctx[s];
-}
-// All tiles of a sequence.
-template <int TT>
-__device__ __forceinline__ uint32_t seq_tiles(const PagedAttnArgs &A, uint32_t rb, uint32_t s) {
-    PaPlace P;
-    load_seq(A, s, P);
-    if ((int)P.ctx < 0 || P.rows == 0u) return 0u;
-    uint32_t n = 0, lo;
-    const uint32_t blocks = (P.rows * A.group + rb - 1u) / rb;
-    for (uint32_t mb = 0; mb < blocks; mb++) n += block_tiles<TT>(A, rb, P.rows, P.ctx, mb, lo);
-    return n * A.V.n_kv;
-}
-// The place of line index x; upto[s]: tiles of the sequences up to and including s.
-template <int TT>
-__device__ __forceinline__ void find_place(const PagedAttnArgs &A, uint32_t rb, const uint32_t *upto, uint32_t x, PaPlace &P) {
-    uint32_t lo = 0, hi = A.V.n_seq - 1u;  // the first sequence with upto > x
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2u;
-        if (upto[mid] > x) hi = mid; else lo = mid + 1u;
-    }
-    load_seq(A, lo, P);
-    uint32_t off = x - (lo ? upto[lo - 1u] : 0u), n = 0, first_tile = 0;
-    const uint32_t blocks = (P.rows * A.group + rb - 1u) / rb;
-    for (P.mb = 0;; P.mb++) {
-        n = block_tiles<TT>(A, rb, P.rows, P.ctx, P.mb, first_tile);
-        if (off < n * A.V.n_kv || P.mb + 1u >= blocks) break;
-        off -= n * A.V.n_kv;
-    }
-    P.lo_tile = first_tile;
-    P.tiles = n;
-    P.head = n ? off / n : 0u;
-    P.at = n ? off - P.head * n : 0u;
-    P.item0 = x - P.at;
-}
-// The next item with tiles; the caller knows that there is one.
-template <int TT>
-__device__ __forceinline__ void next_item(const PagedAttnArgs &A, uint32_t rb, PaPlace &P) {
-    P.item0 += P.tiles;
-    P.at = 0;
-    if (++P.head < A.V.n_kv) return;
-    P.head = 0;
-    for (;;) {
-        const uint32_t blocks = (P.rows * A.group + rb - 1u) / rb;
-        if ((int)P.ctx >= 0 && ++P.mb < blocks) {
-            P.tiles = block_tiles<TT>(A, rb, P.rows, P.ctx, P.mb, P.lo_tile);
-            if (P.tiles) return;
-            continue;
-        }
-        if (P.s + 1u >= A.V.n_seq) {
-            P.tiles = 0;
-            return;
-        }
-        load_seq(A, P.s + 1u, P);
-        P.mb = 0xffffffffu;
-        if (P.rows == 0u) P.ctx = 0xffffffffu;
-    }
-}
-
-// The line's division among blocks: equal to within a tile.
-struct PaCuts {
-    uint32_t per, rem;
-    __device__ PaCuts(uint32_t total, uint32_t parts) : per(total / parts), rem(total - per * parts) {}
-    __device__ uint32_t cut(uint32_t c) const { return c * per + min(c, rem); }
-    __device__ uint32_t part_of(uint32_t x) const {  // the part that holds index x
-        const uint32_t big = rem * (per + 1u);
-        return x < big ? x / (per + 1u) : rem + (x - big) / per;
-    }
-};
-
-// Where cut x of the line falls: cuts inside a short item move to its nearer end.
-__device__ __forceinline__ uint32_t snapped(const PaPlace &P, uint32_t x) {
-    if (P.at == 0u || P.tiles > PA_SNAP) return x;
-    return 2u * P.at < P.tiles ? P.item0 : P.item0 + P.tiles;
 }
 
 template <int HD, int TYPE, bool WIDE>
@@ -287,24 +129,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
 
     // ---- running tile counts of the sequences (where the rings will be)
     uint32_t *upto = reinterpret_cast<uint32_t *>(rings);
-    uint32_t total = 0;
-    for (uint32_t c = 0; c < V.n_seq; c += NW * 32) {
-        uint32_t n = c + threadIdx.x < V.n_seq ? seq_tiles<TT>(A, rb, c + threadIdx.x) : 0u;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, n, d);
-            if ((int)lane >= d) n += v;
-        }
-        if (lane == 31u) scan[warp] = n;
-        __syncthreads();
-        uint32_t before = total;
-        for (uint32_t w = 0; w < NW; w++) {
-            if (w < warp) before += scan[w];
-            total += scan[w];
-        }
-        if (c + threadIdx.x < V.n_seq) upto[c + threadIdx.x] = before + n;
-        __syncthreads();
-    }
+    const uint32_t total = count_tiles<TT, NW * 32>(A, rb, upto, scan);
     for (uint32_t i = threadIdx.x; i < workers * halves; i += NW * 32) {
         mbar_init(&full[i], 1);
         mbar_init(&empty[i], wm);
@@ -323,7 +148,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         uint32_t x = line.cut(blockIdx.x + (lane & 1u));
         if (x < total) {
             find_place<TT>(A, rb, upto, x, place);
-            x = snapped(place, x);
+            x = snapped(place, x, PA_SNAP);
         }
         const uint32_t lo = __shfl_sync(0xffffffffu, x, 0), hi = __shfl_sync(0xffffffffu, x, 1);
         n_block = hi - lo;
@@ -448,27 +273,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         is_left--;
     };
 
-    // ---- rows that see nothing, and lengths beyond the table: each sequence is looked at by one warp of the grid
-    for (uint32_t s = blockIdx.x * NW + warp; s < V.n_seq; s += gridDim.x * NW) {
-        uint32_t first, end;
-        seq_rows(V, s, first, end, bad);
-        const int ctx = V.ctx[s];
-        const uint32_t rows = end - first;
-        const bool over = ctx >= 0 && rows && (uint64_t)(uint32_t)ctx + rows > A.cap;
-        bad |= over;
-        if (ctx < 0 || over) {
-            const uint32_t R = rows * A.group, nb = (R + rb - 1u) / rb;
-            for (uint32_t mb = 0; mb < nb; mb++) {
-                uint32_t lo;
-                if (ctx >= 0 && block_tiles<TT>(A, rb, rows, (uint32_t)ctx, mb, lo)) continue;
-                for (uint32_t r = mb * rb; r < min(R, (mb + 1u) * rb); r++)
-                    for (uint32_t h = 0; h < V.n_kv; h++) {
-                        float *dst = A.out + (size_t)(first + by_group(A, r)) * A.ld_out + (size_t)(h * A.group + r - by_group(A, r) * A.group) * HD;
-                        for (uint32_t i = lane; i < HD; i += 32u) dst[i] = 0.f;
-                    }
-            }
-        }
-    }
+    bad |= empty_rows<HD, TT>(A, rb, warp, NW);
 
     // ---- the loop over half tiles: k to weights, v to sums. The worker's first warp runs ahead by a ring.
     float o[NO][2 * RW], m[RW], l[RW];
@@ -909,10 +714,6 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     }
     const bool front = heads && (tail_set == 0u || __ffs(heads) <= __ffs(tail_set));
     const uint32_t chains = __popc(tail_set) + front;
-    auto row_out = [&](const PaWorker::Part &it, uint32_t row) {
-        const uint32_t r = it.row0 + row, tk = by_group(A, r);
-        return A.out + (size_t)(it.seq_first + tk) * A.ld_out + (size_t)(it.head * A.group + r - tk * A.group) * HD;
-    };
     constexpr int DL = (HD / 2 + 31) / 32;  // pairs of a row in a lane
     const PaWorker::Part *cross[2] = {nullptr, nullptr};  // the item that goes on in front, and behind
     for (uint32_t c = 0, left = tail_set; c < chains; c++) {
@@ -960,7 +761,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
                 if (lane == 0) __stcg(reinterpret_cast<float2 *>(dst + HD), make_float2(M, L));
             } else {
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
-                float *dst = row_out(it, row);
+                float *dst = item_row(A, HD, it.seq_first, it.row0, it.head, row);
 #pragma unroll
                 for (int k = 0; k < DL; k++)
                     if (k * 32 + lane < HD / 2) {
@@ -992,65 +793,33 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         const PaWorker::Part &it = *cross[e];
         const uint32_t lo = line.part_of(it.item0), n = line.part_of(it.item0 + it.item_tiles - 1u) - lo + 1u;
         const uint32_t R = min(rb, it.seq_rows * A.group - it.row0);
-        for (uint32_t row = warp; row < R; row += NW) {
-            auto part = [&](uint32_t i) { return A.part + (((size_t)(lo + i) * 2u + (i == 0u ? 1u : 0u)) * rb + row) * PS; };
-            float M = -INFINITY, L = 0.f;
-            for (uint32_t i = lane; i < n; i += 32u) M = fmaxf(M, __ldcg(part(i) + HD));
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-            float2 acc[DL];
-#pragma unroll
-            for (int k = 0; k < DL; k++) acc[k] = make_float2(0.f, 0.f);
-            for (uint32_t base = 0; base < n; base += 32u) {
-                const uint32_t cnt = min(32u, n - base);
-                float2 ml = make_float2(-INFINITY, 0.f);
-                if (lane < cnt) ml = __ldcg(reinterpret_cast<const float2 *>(part(base + lane) + HD));
-                const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-                L += f * ml.y;
-#pragma unroll 4
-                for (uint32_t i = 0; i < cnt; i++) {
-                    const float fw = __shfl_sync(0xffffffffu, f, i);
-                    const float2 *src = reinterpret_cast<const float2 *>(part(base + i));
-#pragma unroll
-                    for (int k = 0; k < DL; k++)
-                        if (k * 32 + lane < HD / 2) {
-                            const float2 v = __ldcg(src + k * 32 + lane);
-                            acc[k].x = fmaf(fw, v.x, acc[k].x);
-                            acc[k].y = fmaf(fw, v.y, acc[k].y);
-                        }
-                }
-            }
-            L = warp_sum(L);
-            const float inv = L == 0.f ? 0.f : 1.0f / L;
-            float *dst = row_out(it, row);
-#pragma unroll
-            for (int k = 0; k < DL; k++)
-                if (k * 32 + lane < HD / 2) {
-                    dst[2 * (k * 32 + lane)] = acc[k].x * inv;
-                    dst[2 * (k * 32 + lane) + 1] = acc[k].y * inv;
-                }
-        }
+        for (uint32_t row = warp; row < R; row += NW) join_row<HD>(A, rb, lo, n, row, item_row(A, HD, it.seq_first, it.row0, it.head, row));
     }
 }
+
+constexpr uint64_t ROWS_FROM = 16;
 
 // Blocks that the launch may have: one on each SM.
 static uint32_t attn_blocks(const strix_cuda *h) { return (uint32_t)std::min<int>(std::max(h->num_sms, 1), (int)PA_MAX_BLOCKS); }
 
-// Rows of a KV head that a sequence brings on average decide the form: up to 8, one product for values and remainders; beyond,
-// 16 rows a warp and as many warps to a worker as cover them (at most all of a block).
-static void attn_form(const PagedView &V, uint32_t group, bool &wide, uint32_t &wm) {
+// Rows of a KV head that a sequence brings on average decide the form: up to 8, one product for values and remainders; beyond, on
+// tcgen05 with blocks of 128 rows (head sizes 64 and 128), else 16 rows a warp and as many warps to a worker as cover them (at
+// most all of a block).
+enum : int { FORM_NARROW, FORM_WIDE, FORM_ROWS };
+static int attn_form(const PagedView &V, uint32_t group, uint32_t &wm) {
     const uint64_t rows = ((uint64_t)V.n_rows * group + V.n_seq - 1) / std::max(V.n_seq, 1u);
-    wide = rows > 8;
-    const uint32_t most = V.head_dim >= 192 ? 4u : 8u;
     wm = 1;
-    while (wide && wm < most && 16ull * wm < rows) wm *= 2;
+    if (rows <= 8) return FORM_NARROW;
+    if (rows > ROWS_FROM && (V.head_dim == 64 || V.head_dim == 128)) return FORM_ROWS;
+    const uint32_t most = V.head_dim >= 192 ? 4u : 8u;
+    while (wm < most && 16ull * wm < rows) wm *= 2;
+    return FORM_WIDE;
 }
 
 static size_t attn_work_bytes(const strix_cuda *h, const PagedView &V, uint32_t group) {
-    bool wide;
     uint32_t wm;
-    attn_form(V, group, wide, wm);
-    const size_t rb = wide ? 16u * wm : 8u;
+    const int form = attn_form(V, group, wm);
+    const size_t rb = form == FORM_ROWS ? 128u : form == FORM_WIDE ? 16u * wm : 8u;
     const size_t part = (size_t)attn_blocks(h) * 2 * rb * (V.head_dim + 2) * 4;
     return (PA_MAX_BLOCKS * 4 + part + 255) & ~(size_t)255;
 }
@@ -1068,8 +837,7 @@ static AttnEncodeFn attn_encode_fn() {
     }();
     return fn;
 }
-// A cache as [page][KV head and slot][element], copied in boxes of `rows` slots by `box` elements.
-static bool attn_map(CUtensorMap *map, const PagedView &V, void *base, uint32_t box, uint32_t rows, bool swizzled) {
+bool attn_map(CUtensorMap *map, const PagedView &V, void *base, uint32_t box, uint32_t rows, bool swizzled) {
     AttnEncodeFn fn = attn_encode_fn();
     if (!fn) return false;
     const bool f16 = V.type == STRIX_KV_F16;
@@ -1160,8 +928,8 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     A.vec = ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15u) == 0 && ((A.ld_q | A.ld_out) & 3u) == 0;
     A.ticket = static_cast<uint32_t *>(d_work);
     A.part = reinterpret_cast<float *>(static_cast<uint8_t *>(d_work) + PA_MAX_BLOCKS * 4);
-    bool wide;
-    attn_form(A.V, A.group, wide, A.wm);
+    const int form = attn_form(A.V, A.group, A.wm);
+    const bool wide = form == FORM_WIDE;
     DeviceGuard dev(h->device);
     if (dev.err != cudaSuccess) return serve_fail(h, who, cudaGetErrorString(dev.err));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1174,7 +942,8 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
         e = f16 ? (wide ? attn_launch<HD, STRIX_KV_F16, true>(h, A, s) : attn_launch<HD, STRIX_KV_F16, false>(h, A, s))             \
                 : (wide ? attn_launch<HD, STRIX_KV_E4M3, true>(h, A, s) : attn_launch<HD, STRIX_KV_E4M3, false>(h, A, s));          \
         break;
-        switch (hd) {
+        if (form == FORM_ROWS) e = launch_attn_rows(h, A, attn_blocks(h), s);
+        else switch (hd) {
             STRIX_ATTN(64)
             STRIX_ATTN(96)
             STRIX_ATTN(128)
