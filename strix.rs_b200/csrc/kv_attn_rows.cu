@@ -24,7 +24,7 @@
 
 namespace strix {
 
-constexpr uint32_t RA_ROWS = 128, RA_TT = 64, RA_THREADS = 384, RA_DESCS = 16, RA_QBUF = 4;
+constexpr uint32_t RA_ROWS = 128, RA_TT = 64, RA_THREADS = 640, RA_DESCS = 16, RA_QBUF = 4, RA_STATS = 8;
 constexpr uint32_t RA_SNAP = 4;   // cuts inside an item of at most this many tiles move to its end (256 tokens, as PA_SNAP tiles are)
 constexpr uint32_t RA_LEAST = 4;  // tiles a block takes at least
 
@@ -39,8 +39,8 @@ struct RowsShape {
     static constexpr int NR = EL == 1 ? 2 : 0;        // tiles of codes of k, and of v
     static constexpr int NL = EL == 1 ? NR : NS;      // tiles that copies land in
     static constexpr bool RAWSWZ = HD == 128;         // rows of 128 codes are swizzled on their way, rows of 64 lie as they are
-    static constexpr int BARS = 4 * NL + 4 * NS + 2 + 5 * 2;
-    static constexpr size_t SMEM = 2 * QB + 2 * NS * OPB + 2 * NR * RAWB + RA_DESCS * sizeof(PaTile) + RA_QBUF * 128 * 4 + BARS * 8 + 1024;
+    static constexpr int BARS = 4 * NL + 4 * NS + 2 + 5 * 2 + (int)RA_STATS;
+    static constexpr size_t SMEM = 2 * QB + 2 * NS * OPB + 2 * NR * RAWB + RA_DESCS * sizeof(PaTile) + RA_QBUF * 128 * 4 + 2 * RA_STATS * 128 * 4 + BARS * 8 + 1024;
     // TMEM columns: S 2 x 64, P 2 x (32 + 32), O 2 x HD
     static constexpr uint32_t COL_P = 128, COL_O = 256;
 };
@@ -73,12 +73,17 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t *r) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *r) {
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t *r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::STRIX_W8(r, 0),
-        STRIX_W8(r, 8), STRIX_W8(r, 16), STRIX_W8(r, 24), "r"(taddr)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : STRIX_R8(r, 0), STRIX_R8(r, 8)
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::STRIX_W8(r, 0), "r"(taddr)
         : "memory");
 }
 #undef STRIX_R8
@@ -104,11 +109,12 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
     uint8_t *q_smem = smem, *op = smem + 2 * S::QB, *raw = op + 2 * NS * S::OPB;  // op, raw: the tiles of k, then those of v
     PaTile *desc = reinterpret_cast<PaTile *>(raw + 2 * S::NR * S::RAWB);
     float *q_factor = reinterpret_cast<float *>(desc + RA_DESCS);  // [RA_QBUF][128]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(q_factor + RA_QBUF * 128);
+    float *tile_m = q_factor + RA_QBUF * 128, *tile_l = tile_m + RA_STATS * 128;  // [RA_STATS][128]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(tile_l + RA_STATS * 128);
     uint64_t *land_full = bars, *land_empty = land_full + 2 * NL;  // [k, v][NL]
     uint64_t *op_full = land_empty + 2 * NL, *op_empty = op_full + 2 * NS;
     uint64_t *q_full = op_empty + 2 * NS, *q_empty = q_full + 1;
-    uint64_t *s_full = q_empty + 1, *s_empty = s_full + 2, *p_full = s_empty + 2, *o_full = p_full + 2, *o_empty = o_full + 2;
+    uint64_t *s_full = q_empty + 1, *s_empty = s_full + 2, *p_full = s_empty + 2, *o_full = p_full + 2, *o_empty = o_full + 2, *m_full = o_empty + 2;
     __shared__ uint32_t scan[RA_THREADS / 32], tmem_slot, last_here[2];
     __shared__ volatile uint32_t gave_up;
     __shared__ PaWorkerParts parts;
@@ -135,12 +141,13 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             mbar_init(&o_full[i], 1);
             mbar_init(&o_empty[i], 4);
         }
+        for (uint32_t i = 0; i < RA_STATS; i++) mbar_init(&m_full[i], 4);
         mbar_fence_init();
         gave_up = 0u;
         parts.has_front = parts.has_back = 0u;
     }
     for (uint32_t i = threadIdx.x; i < RA_DESCS * 4u; i += RA_THREADS) desc[i / 4u].ks[i & 3u] = desc[i / 4u].vs[i & 3u] = 0.f;
-    if (warp == 9) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -171,120 +178,137 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
     const bool mixed = V.page_tokens < RA_TT;
     const uint32_t sub = min(RA_TT, V.page_tokens), n_sub = RA_TT / sub;
 
-    if (warp < 4) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        // ---- softmax: the thread has row 32 warp + lane of the block
-        const uint32_t row = threadIdx.x;
-        const uint32_t t_row = tmem + ((warp * 32u) << 16);
-        float o[HD], m = -INFINITY, l = 0.f, f_q = 0.f, v_prev = 0.f;
-        uint32_t pos = 0, pos_lo = 0, pos_hi = 0, items = 0;
-        uint32_t it_first = 0, it_rows = 0, it_row0 = 0, it_head = 0;
-        bool wrote = false;
-        // adds the product of tile n, scaled, to the running sums
-        auto add_tile = [&](uint32_t n, float scale) {
-            wait(&o_full[n & 1u], (n >> 1) & 1u);
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < HD / 32; c++) {
-                uint32_t r[32];
-                tc_ld32(t_row + S::COL_O + (n & 1u) * HD + c * 32, r);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; i++) o[c * 32 + i] = fmaf(__uint_as_float(r[i]), scale, o[c * 32 + i]);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_empty[n & 1u]);
-        };
-        for (uint32_t n = 0; n < n_tiles; n++) {
-            const uint32_t b = n & 1u;
+    if (warp < 8) {
+        // ---- softmax: warps 0-3 take the even tiles, 4-7 the odd ones; the thread has row 32 (warp & 3) + lane of the block
+        const uint32_t b = warp >> 2, row = threadIdx.x & 127u;
+        const uint32_t t_row = tmem + (((warp & 3u) * 32u) << 16);
+        float f_q = 0.f;
+        uint32_t pos = 0, pos_lo = 0, pos_hi = 0, item = ~0u;
+        for (uint32_t n = b; n < n_tiles; n += 2u) {
             wait(&s_full[b], (n >> 1) & 1u);
             tc_fence_after();
             const PaTile &d = desc[n % RA_DESCS];
-            const uint32_t flags = d.flags, valid = d.valid, tok = d.tile * RA_TT;
-            const bool fresh = flags & PA_NEW;
-            if (fresh) {
+            const uint32_t valid = d.valid, tok = d.tile * RA_TT;
+            if (d.flags >> PA_ITEM != item) {
+                item = d.flags >> PA_ITEM;
+                const uint32_t R = d.seq_rows * A.group, ctx = d.ctx, row0 = d.row0;
+                pos = ctx + by_group(A, min(row0 + row, R - 1u));
+                pos_lo = ctx + by_group(A, min(row0 + (row & 96u), R - 1u));
+                pos_hi = ctx + by_group(A, min(row0 + (row | 31u), R - 1u));
+                f_q = q_factor[(item % RA_QBUF) * 128u + row];
+            }
+            float vref = d.vs[0];
+            if (mixed) vref = fmaxf(fmaxf(vref, d.vs[1]), fmaxf(d.vs[2], d.vs[3]));
+            const float rvref = vref > 0.f ? 1.0f / vref : 0.f;
+            uint64_t sees = ~0ull;  // one bit for each token that the row sees
+            if (tok + RA_TT - 1u > pos_lo || valid != (1u << n_sub) - 1u || (A.window && pos_hi >= A.window && tok <= pos_hi - A.window)) {
+                const uint32_t last = pos - tok, from = A.window && pos >= A.window && pos - A.window >= tok ? pos - A.window - tok + 1u : 0u;
+                sees = pos < tok || from > 63u ? 0ull : ~0ull >> (63u - min(last, 63u)) & ~0ull << from;
+                for (uint32_t j = 0; j < n_sub; j++)
+                    if (!((valid >> j) & 1u)) sees &= ~((~0ull >> (64u - sub)) << (j * sub));
+            }
+            auto masked16 = [&](uint32_t *s, uint32_t c) {  // the sums of sixteen tokens, which are of one page
+                tc_ld16(t_row + b * 64u + c, s);
+                const uint32_t bits = (uint32_t)(sees >> c) & 0xffffu;
+                tc_wait_ld();
+                if (__any_sync(0xffffffffu, bits != 0xffffu)) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[i] = (bits >> i) & 1u ? s[i] : 0xff800000u;
+                }
+            };
+            // the factor to exponents of two is positive (the sign of the caller's scale went into q), so the largest product is the
+            // largest score; it multiplies inside the exponent's subtraction
+            auto factor = [&](uint32_t c) { return fmaxf(d.ks[mixed ? c >> pshift : 0u] * f_q, 1.0e-30f); };
+            float top = -INFINITY;
+#pragma unroll 1
+            for (uint32_t c = 0; c < RA_TT; c += 16u) {
+                uint32_t s[16];
+                masked16(s, c);
+                float t0 = __uint_as_float(s[0]), t1 = __uint_as_float(s[1]);
+#pragma unroll
+                for (int i = 2; i < 16; i += 2) {
+                    t0 = fmaxf(t0, __uint_as_float(s[i]));
+                    t1 = fmaxf(t1, __uint_as_float(s[i + 1]));
+                }
+                top = fmaxf(top, fmaxf(t0, t1) * factor(c));
+            }
+            const float base = top == -INFINITY ? 0.f : 15.f - top;
+            if (n >= 2u) wait(&o_full[b], ((n >> 1) & 1u) ^ 1u);  // the product of tile n - 2, which read this buffer of P
+            tc_fence_after();
+            float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+            for (uint32_t c = 0; c < RA_TT; c += 16u) {
+                uint32_t s[16], hi[8], lo[8];
+                const float f = factor(c), w = mixed ? d.vs[c >> pshift] * rvref : 1.f;
+                masked16(s, c);
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float p0 = ex2(fmaf(__uint_as_float(s[i]), f, base)), p1 = ex2(fmaf(__uint_as_float(s[i + 1]), f, base));
+                    l0 += p0;
+                    l1 += p1;
+                    split2(p0 * w, p1 * w, hi[i / 2], lo[i / 2]);
+                }
+                tc_st8(t_row + S::COL_P + b * 64u + c / 2u, hi);
+                tc_st8(t_row + S::COL_P + b * 64u + 32u + c / 2u, lo);
+            }
+            tile_m[(n % RA_STATS) * 128u + row] = top;
+            tile_l[(n % RA_STATS) * 128u + row] = l0 + l1;
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&s_empty[b]);
+                mbar_arrive(&m_full[n % RA_STATS]);
+                mbar_arrive(&p_full[b]);
+            }
+        }
+    } else if (warp < 12) {
+        // ---- sums: warps 8-11 add the tiles' products to O, whose row is kept by a thread, and write the finished items
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        const uint32_t row = threadIdx.x & 127u, t_row = tmem + (((warp & 3u) * 32u) << 16);
+        float o[HD], m = -INFINITY, l = 0.f;
+        uint32_t it_first = 0, it_rows = 0, it_row0 = 0, it_head = 0;
+        bool wrote = false;
+        for (uint32_t n = 0; n < n_tiles; n++) {
+            const uint32_t b = n & 1u;
+            const PaTile &d = desc[n % RA_DESCS];
+            wait(&m_full[n % RA_STATS], (n / RA_STATS) & 1u);
+            const uint32_t flags = d.flags;
+            if (flags & PA_NEW) {
                 it_first = d.seq_first;
                 it_rows = d.seq_rows;
                 it_row0 = d.row0;
                 it_head = d.head;
-                const uint32_t R = it_rows * A.group, ctx = d.ctx;
-                pos = ctx + by_group(A, min(it_row0 + row, R - 1u));
-                pos_lo = ctx + by_group(A, min(it_row0 + warp * 32u, R - 1u));
-                pos_hi = ctx + by_group(A, min(it_row0 + warp * 32u + 31u, R - 1u));
-                f_q = q_factor[(items++ % RA_QBUF) * 128u + row];
                 m = -INFINITY;
                 l = 0.f;
 #pragma unroll
                 for (int i = 0; i < HD; i++) o[i] = 0.f;
             }
-            uint32_t s[64];
-            tc_ld32(t_row + b * 64u, s);
-            tc_ld32(t_row + b * 64u + 32u, s + 32);
-            tc_wait_ld();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[b]);
-            float k0 = d.ks[0], vref = d.vs[0];
-            if (mixed) {  // the largest scales of the tile's pages; scores and weights take what another page's differs by
-                k0 = fmaxf(fmaxf(k0, d.ks[1]), fmaxf(d.ks[2], d.ks[3]));
-                vref = fmaxf(fmaxf(vref, d.vs[1]), fmaxf(d.vs[2], d.vs[3]));
-                const float rk0 = k0 > 0.f ? 1.0f / k0 : 0.f;
-#pragma unroll
-                for (int i = 0; i < 64; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * (d.ks[(uint32_t)i >> pshift] * rk0));
-            }
-            if (tok + RA_TT - 1u > pos_lo || valid != (1u << n_sub) - 1u || (A.window && pos_hi >= A.window && tok <= pos_hi - A.window)) {
-#pragma unroll
-                for (int i = 0; i < 64; i++) {
-                    const uint32_t tk = tok + i;
-                    const bool see = tk <= pos && (!A.window || pos < A.window || tk > pos - A.window) && ((valid >> (mixed ? (uint32_t)i >> pshift : 0u)) & 1u);
-                    if (!see) s[i] = 0xff800000u;
-                }
-            }
-            const float f = k0 * f_q;  // (not negative unless the caller's scale is: the largest score has the largest product then)
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 64; i++) {
-                const float x = __uint_as_float(s[i]);
-                const float y = x == -INFINITY ? -INFINITY : x * f;
-                s[i] = __float_as_uint(y);
-                top = fmaxf(top, y);
-            }
-            const float m_new = fmaxf(m, top), alpha = m_new == m ? 1.f : ex2(m - m_new);
-            const float base = m_new == -INFINITY ? 0.f : m_new - 15.f;
-            l *= alpha;
-            const float rvref = mixed && vref > 0.f ? 1.0f / vref : 1.f;
-            uint32_t hi[32], lo[32];
-            float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-                float p0 = ex2(__uint_as_float(s[2 * i]) - base), p1 = ex2(__uint_as_float(s[2 * i + 1]) - base);
-                l0 += p0;
-                l1 += p1;
-                if (mixed) {
-                    const float w = d.vs[(2u * i) >> pshift] * rvref;
-                    p0 *= w;
-                    p1 *= w;
-                }
-                split2(p0, p1, hi[i], lo[i]);
-            }
-            l += l0 + l1;
-            // (the product of tile n - 2, which read this buffer, was waited for when its sums were added)
-            tc_st32(t_row + S::COL_P + b * 64u, hi);
-            tc_st32(t_row + S::COL_P + b * 64u + 32u, lo);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[b]);
-            if (!fresh) add_tile(n - 1u, v_prev);
+            const float m_tile = tile_m[(n % RA_STATS) * 128u + row], m_new = fmaxf(m, m_tile);
+            const float alpha = m_new == m ? 1.f : ex2(m - m_new), beta = m_new == m_tile ? 1.f : ex2(m_tile - m_new);
+            float vref = d.vs[0];
+            if (mixed) vref = fmaxf(fmaxf(vref, d.vs[1]), fmaxf(d.vs[2], d.vs[3]));
+            const float w = beta * vref;
+            l = fmaf(tile_l[(n % RA_STATS) * 128u + row], beta, l * alpha);
+            m = m_new;
             if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
                 for (int i = 0; i < HD; i++) o[i] *= alpha;
             }
-            m = m_new;
-            v_prev = vref;
+            wait(&o_full[b], (n >> 1) & 1u);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) {
+                uint32_t r[32];
+                tc_ld32(t_row + S::COL_O + b * HD + c * 32, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[c * 32 + i] = fmaf(__uint_as_float(r[i]), w, o[c * 32 + i]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[b]);
             if (!(flags & PA_END)) continue;
-            add_tile(n, vref);
             if (it_row0 + row < it_rows * A.group) {
                 if (flags & PA_WHOLE) {
                     const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -311,14 +335,15 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             const PaCuts line(total, line_blocks);
             __threadfence();
             asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (warp < 2u && lane == 0) {
-                last_here[warp] = 0u;
-                if (warp == 0 ? parts.has_front : parts.has_back) {
-                    const PaPart &it = warp == 0 ? parts.front : parts.back;
+            if (warp < 10u && lane == 0) {
+                const uint32_t e = warp - 8u;
+                last_here[e] = 0u;
+                if (e == 0 ? parts.has_front : parts.has_back) {
+                    const PaPart &it = e == 0 ? parts.front : parts.back;
                     const uint32_t lo = line.part_of(it.item0), hi = line.part_of(it.item0 + it.item_tiles - 1u);
                     if (atomicAdd(&A.ticket[lo], 1u) == hi - lo) {
                         A.ticket[lo] = 0u;
-                        last_here[warp] = 1u;
+                        last_here[e] = 1u;
                     }
                 }
             }
@@ -329,14 +354,14 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 const PaPart &it = e == 0 ? parts.front : parts.back;
                 const uint32_t lo = line.part_of(it.item0), cnt = line.part_of(it.item0 + it.item_tiles - 1u) - lo + 1u;
                 const uint32_t R = min(RA_ROWS, it.seq_rows * A.group - it.row0);
-                for (uint32_t r = warp; r < R; r += 4u) join_row<HD>(A, RA_ROWS, lo, cnt, r, item_row(A, HD, it.seq_first, it.row0, it.head, r));
+                for (uint32_t r = warp - 8u; r < R; r += 4u) join_row<HD>(A, RA_ROWS, lo, cnt, r, item_row(A, HD, it.seq_first, it.row0, it.head, r));
             }
         }
-    } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 136;");
+    } else if (warp < 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         // ---- operands: q of a new item; every tile's k and v
-        const uint32_t tid = threadIdx.x - 128u, tr = tid & 63u, th = tid >> 6;  // token of the tile, half of its dimensions
-        bool bad = empty_rows<HD, RA_TT>(A, RA_ROWS, warp - 4u, 4u);
+        const uint32_t tid = threadIdx.x & 127u, tr = tid & 63u, th = tid >> 6;  // token of the tile, half of its dimensions
+        bool bad = empty_rows<HD, RA_TT>(A, RA_ROWS, warp - 12u, 4u);
         report_bad(V, bad && lane == 0);
         uint32_t items = 0, pos_hi = 0;
         auto arrive = [&](uint64_t *bar) {
@@ -365,8 +390,8 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 }
                 const int ex = (int)(__float_as_uint(top) >> 23);
                 const int e2 = top > 0.f && ex < 255 ? min(126, max(-126, 14 + 127 - max(ex, 1))) : 0;
-                const float up = __uint_as_float((uint32_t)(e2 + 127) << 23);
-                q_factor[(items % RA_QBUF) * 128u + tid] = A.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e2) << 23);
+                const float up = copysignf(__uint_as_float((uint32_t)(e2 + 127) << 23), A.scale);
+                q_factor[(items % RA_QBUF) * 128u + tid] = fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll 4
                 for (int i = 0; i < HD; i += 8) {
                     const float4 x = load4(i), y = load4(i + 4);
@@ -384,13 +409,14 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             }
             const uint32_t tok = d.tile * RA_TT;
             const bool keep = tok + tr <= pos_hi && ((d.valid >> (mixed ? tr >> pshift : 0u)) & 1u);
+#pragma unroll 1
             for (int kv = 0; kv < 2; kv++) {
                 if (kv) wait(&land_full[NL + land], land_phase);
                 uint8_t *dst = op + (size_t)(kv * NS + st) * S::OPB;
                 if constexpr (EL == 1) {
                     wait(&op_empty[kv * NS + st], st_phase ^ 1u);
                     const uint8_t *src = raw + (size_t)(kv * NL + land) * S::RAWB + tr * HD;
-#pragma unroll
+#pragma unroll 2
                     for (int j = 0; j < HD / 32; j++) {
                         const uint32_t c = th * (HD / 32) + j;  // sixteen codes
                         uint4 x = *reinterpret_cast<const uint4 *>(src + ((S::RAWSWZ ? c ^ (tr & 7u) : c) << 4));
@@ -420,10 +446,10 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 136;");
-        if (warp == 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 16) {
             // ---- copies: the pages of the next 32 slots of the item to a lane each, one tile after the other
-            uint32_t b_from = 0, b_stop = place.at, seg_stop = place.at, new_flag = 0, end_flag = 0;
+            uint32_t b_from = 0, b_stop = place.at, seg_stop = place.at, new_flag = 0, end_flag = 0, item = ~0u;
             int b_page = -1;
             float b_ks = 0.f, b_vs = 0.f;
             bool bad = false, started = false;
@@ -439,6 +465,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                         const bool ends = place.at + seg == place.tiles;
                         seg_stop = place.at + seg;
                         new_flag = PA_NEW;
+                        item++;
                         end_flag = PA_END | (place.at ? PA_HEAD : ends ? PA_WHOLE : 0u);
                         if (lane == 0) {
                             const PaPart part{place.first, place.rows, place.mb * RA_ROWS, place.head, place.item0, place.tiles};
@@ -475,8 +502,8 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0) & ((1u << n_sub) - 1u);
                 PaTile &d = desc[n % RA_DESCS];
                 if (lane == 0) {
-                    *reinterpret_cast<uint4 *>(&d.tile) = make_uint4(tile, new_flag | (place.at + 1u == seg_stop ? end_flag : 0u), valid, place.mb * RA_ROWS);
-                    if (new_flag) *reinterpret_cast<uint4 *>(&d.seq_first) = make_uint4(place.first, place.rows, place.ctx, place.head);
+                    *reinterpret_cast<uint4 *>(&d.tile) = make_uint4(tile, item << PA_ITEM | new_flag | (place.at + 1u == seg_stop ? end_flag : 0u), valid, place.mb * RA_ROWS);
+                    *reinterpret_cast<uint4 *>(&d.seq_first) = make_uint4(place.first, place.rows, place.ctx, place.head);
                 }
                 if (lane - b_from < n_sub) {
                     d.ks[lane - b_from] = b_ks;
@@ -506,7 +533,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 place.at++;
             }
             report_bad(V, bad);
-        } else if (warp == 9) {
+        } else if (warp == 17) {
             // ---- products, by one lane
             if (elect_lane()) {
                 const uint32_t q_at = smem_u32(q_smem), op_at = smem_u32(op);
@@ -520,7 +547,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     tc_fence_after();
                     const uint64_t v = desc_sw128(op_at + (NS + st) * S::OPB, 8192u);
                     const uint32_t d = tmem + S::COL_O + b * HD, p = tmem + S::COL_P + b * 64u;
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < 2; h++)  // the remainders first
 #pragma unroll
                         for (int k = 0; k < 4; k++) tc_mma_ts(d, p + (h ? 0u : 32u) + 8u * k, v + (uint64_t)(k * 2048 / 16), I_O, h || k);
@@ -536,26 +563,26 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     wait(&s_empty[b], ((n >> 1) & 1u) ^ 1u);
                     tc_fence_after();
                     const uint32_t d = tmem + b * 64u;
+                    const uint64_t q = desc_sw128(q_at, 16u), kk = desc_sw128(op_at + st * S::OPB, 16u);
+#pragma unroll 1
+                    for (uint32_t i = 0; i < 2u * S::BLOCKS; i++) {  // the remainders first; 64 dimensions at a time
+                        const uint64_t qi = q + (i < S::BLOCKS ? S::QB / 16u : 0u) + (i % S::BLOCKS) * (128u * 128u / 16u), ki = kk + (i % S::BLOCKS) * (8192u / 16u);
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int k = 0; k < HD / 16; k++) {
-                            const uint64_t q = desc_sw128(q_at + (h ? 0u : (uint32_t)S::QB) + (k / 4) * (128 * 128) + (k % 4) * 32, 16u);
-                            const uint64_t kk = desc_sw128(op_at + st * S::OPB + (k / 4) * 8192 + (k % 4) * 32, 16u);
-                            tc_mma_ss(d, q, kk, I_S, h || k);
-                        }
+                        for (uint32_t k = 0; k < 4u; k++) tc_mma_ss(d, qi + 2u * k, ki + 2u * k, I_S, i + k);
+                    }
                     tc_commit(&s_full[b]);
                     tc_commit(&k_free[EL == 1 ? st : n % NL]);
                     if (flags & PA_END) tc_commit(q_empty);
-                    if (n) weigh(n - 1u);
+                    if (n >= 2u) weigh(n - 2u);
                 }
+                if (n_tiles > 1u) weigh(n_tiles - 2u);
                 if (n_tiles) weigh(n_tiles - 1u);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 17) {
         __syncwarp();
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

@@ -31,10 +31,11 @@ struct PagedAttnArgs {
 // What the first warp tells a worker about a tile.
 struct __align__(16) PaTile {
     uint32_t tile, flags, valid, row0;        // tile of the item; PA_*; one bit for each page of the tile; first row of the block
-    uint32_t seq_first, seq_rows, ctx, head;  // with PA_NEW: first row of the sequence, its new rows, tokens before them, KV head
+    uint32_t seq_first, seq_rows, ctx, head;  // first row of the sequence, its new rows, tokens before them, KV head (kv_attn.cu: with PA_NEW)
     float ks[4], vs[4];                       // the scales of the tile's pages
 };
 enum : uint32_t { PA_NEW = 1, PA_END = 2, PA_WHOLE = 4, PA_HEAD = 8 };  // first / last tile of the segment here; item complete here; begun elsewhere
+constexpr uint32_t PA_ITEM = 4;  // with row blocks: flags >> PA_ITEM counts the items of the block
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
