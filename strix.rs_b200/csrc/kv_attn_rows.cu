@@ -172,7 +172,11 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
     const uint32_t tmem = tmem_slot;
     // a wait that has run out is the last one of the block: everything goes on without waiting, to its end
     auto wait = [&](uint64_t *bar, uint32_t parity) {
-        if (!gave_up && !mbar_wait_bounded(bar, parity, V.status)) gave_up = 1u;
+        for (uint32_t it = 0; !mbar_try_wait(bar, parity); it++)
+            if (gave_up || it >= 1u << 22) {
+                gave_up = 1u;
+                break;
+            }
     };
     const uint32_t pshift = V.page_shift;
     const bool mixed = V.page_tokens < RA_TT;
@@ -184,6 +188,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         const uint32_t t_row = tmem + (((warp & 3u) * 32u) << 16);
         float f_q = 0.f;
         uint32_t pos = 0, pos_lo = 0, pos_hi = 0, item = ~0u;
+#pragma unroll 1
         for (uint32_t n = b; n < n_tiles; n += 2u) {
             wait(&s_full[b], (n >> 1) & 1u);
             tc_fence_after();
@@ -204,6 +209,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             if (tok + RA_TT - 1u > pos_lo || valid != (1u << n_sub) - 1u || (A.window && pos_hi >= A.window && tok <= pos_hi - A.window)) {
                 const uint32_t last = pos - tok, from = A.window && pos >= A.window && pos - A.window >= tok ? pos - A.window - tok + 1u : 0u;
                 sees = pos < tok || from > 63u ? 0ull : ~0ull >> (63u - min(last, 63u)) & ~0ull << from;
+#pragma unroll 1
                 for (uint32_t j = 0; j < n_sub; j++)
                     if (!((valid >> j) & 1u)) sees &= ~((~0ull >> (64u - sub)) << (j * sub));
             }
@@ -269,6 +275,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         float o[HD], m = -INFINITY, l = 0.f;
         uint32_t it_first = 0, it_rows = 0, it_row0 = 0, it_head = 0;
         bool wrote = false;
+#pragma unroll 1
         for (uint32_t n = 0; n < n_tiles; n++) {
             const uint32_t b = n & 1u;
             const PaTile &d = desc[n % RA_DESCS];
@@ -369,6 +376,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
+#pragma unroll 1
         for (uint32_t n = 0; n < n_tiles; n++) {
             const uint32_t land = n % NL, land_phase = (n / NL) & 1u, st = n % NS, st_phase = (n / NS) & 1u;
             wait(&land_full[land], land_phase);
@@ -455,6 +463,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             bool bad = false, started = false;
             const bool leader = elect_lane();
             const uint32_t sub_at = lane & (n_sub - 1u);
+#pragma unroll 1
             for (uint32_t n = 0; n < n_tiles; n++) {
                 const uint32_t land = n % NL, land_phase = (n / NL) & 1u;
                 if (place.at == b_stop) {
@@ -510,12 +519,14 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     d.vs[lane - b_from] = b_vs;
                 }
                 __syncwarp();
+#pragma unroll 1
                 for (int kv = 0; kv < 2; kv++) {
                     uint64_t *bar = &land_full[kv * NL + land];
                     wait(&land_empty[kv * NL + land], land_phase ^ 1u);
                     if (leader) mbar_arrive_expect_tx(bar, __popc(valid) * sub * HD * EL);
                     __syncwarp();
                     uint8_t *dst = EL == 1 ? raw + (size_t)(kv * NL + land) * S::RAWB : op + (size_t)(kv * NS + land) * S::OPB;
+#pragma unroll 1
                     for (uint32_t i = 0; i < n_sub; i++) {
                         const int pg = __shfl_sync(0xffffffffu, page, i);
                         const uint32_t y = place.head * V.page_tokens + ((tile * RA_TT + i * sub) & (V.page_tokens - 1u));
@@ -555,33 +566,38 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     tc_commit(&v_free[EL == 1 ? st : n % NL]);
                 };
                 uint32_t items = 0;
-                for (uint32_t n = 0; n < n_tiles; n++) {
-                    const uint32_t b = n & 1u, st = n % NS;
-                    wait(&op_full[st], (n / NS) & 1u);
-                    const uint32_t flags = desc[n % RA_DESCS].flags;
-                    if (flags & PA_NEW) wait(q_full, items++ & 1u);
-                    wait(&s_empty[b], ((n >> 1) & 1u) ^ 1u);
-                    tc_fence_after();
-                    const uint32_t d = tmem + b * 64u;
-                    const uint64_t q = desc_sw128(q_at, 16u), kk = desc_sw128(op_at + st * S::OPB, 16u);
 #pragma unroll 1
-                    for (uint32_t i = 0; i < 2u * S::BLOCKS; i++) {  // the remainders first; 64 dimensions at a time
-                        const uint64_t qi = q + (i < S::BLOCKS ? S::QB / 16u : 0u) + (i % S::BLOCKS) * (128u * 128u / 16u), ki = kk + (i % S::BLOCKS) * (8192u / 16u);
+                for (uint32_t n = 0; n < n_tiles + 2u; n++) {
+                    if (n < n_tiles) {
+                        const uint32_t b = n & 1u, st = n % NS;
+                        wait(&op_full[st], (n / NS) & 1u);
+                        const uint32_t flags = desc[n % RA_DESCS].flags;
+                        if (flags & PA_NEW) wait(q_full, items++ & 1u);
+                        wait(&s_empty[b], ((n >> 1) & 1u) ^ 1u);
+                        tc_fence_after();
+                        const uint32_t d = tmem + b * 64u;
+                        const uint64_t q = desc_sw128(q_at, 16u), kk = desc_sw128(op_at + st * S::OPB, 16u);
+#pragma unroll 1
+                        for (uint32_t i = 0; i < 2u * S::BLOCKS; i++) {  // the remainders first; 64 dimensions at a time
+                            const uint64_t qi = q + (i < S::BLOCKS ? S::QB / 16u : 0u) + (i % S::BLOCKS) * (128u * 128u / 16u), ki = kk + (i % S::BLOCKS) * (8192u / 16u);
 #pragma unroll
-                        for (uint32_t k = 0; k < 4u; k++) tc_mma_ss(d, qi + 2u * k, ki + 2u * k, I_S, i + k);
+                            for (uint32_t k = 0; k < 4u; k++) tc_mma_ss(d, qi + 2u * k, ki + 2u * k, I_S, i + k);
+                        }
+                        tc_commit(&s_full[b]);
+                        tc_commit(&k_free[EL == 1 ? st : n % NL]);
+                        if (flags & PA_END) tc_commit(q_empty);
                     }
-                    tc_commit(&s_full[b]);
-                    tc_commit(&k_free[EL == 1 ? st : n % NL]);
-                    if (flags & PA_END) tc_commit(q_empty);
                     if (n >= 2u) weigh(n - 2u);
                 }
-                if (n_tiles > 1u) weigh(n_tiles - 2u);
-                if (n_tiles) weigh(n_tiles - 1u);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
+    if (gave_up) {  // copies may still be under way: they end before the block does
+        if (threadIdx.x == 0 && V.status) atomicOr(V.status, STATUS_WAIT_TIMEOUT);
+        for (int i = 0; i < 64; i++) __nanosleep(100000u);
+    }
     if (warp == 17) {
         __syncwarp();
         tc_fence_after();
