@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
         if (A.rope != STRIX_ROPE_NONE) turn_of(t, inv, (uint32_t)ctx + (row - first));
         Eight n = {};
         if (A.q_norm && on) load_eight(n, A.q_norm, o0, o1, false);
+#pragma unroll 1
         for (;;) {
 #pragma unroll
             for (int i = 0; i < NB; i++) {
@@ -238,6 +239,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
     }
     uint32_t row = unit * A.unit_rows;
     const uint32_t unit_end = min(V.n_rows, row + A.unit_rows);
+#pragma unroll 1
     while (row < unit_end) {
         uint32_t first, end;
         const uint32_t s = seq_of_row(V, row, first, end, bad);
@@ -265,6 +267,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
             continue;
         }
         Turn turns[KEEP ? MAXIT : 1];
+#pragma unroll 1
         for (uint32_t hh = g0; hh < g1; hh++) {
         const float *src = (is_v ? A.src_v : A.src_k) + (size_t)hh * HD;
         uint8_t *dst = cache + (size_t)page * V.page_bytes + (size_t)hh * V.head_bytes;
@@ -326,6 +329,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
             }
         };
         if (TYPE == STRIX_KV_F16) {
+#pragma unroll 1
             for (uint32_t base = 0; base < cnt; base += CHUNK) {
                 fetch(base);
                 store(base, 1.f);
@@ -333,6 +337,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
         } else {
             float m = 0.f;
             uint32_t base = 0;
+#pragma unroll 1
             for (;; base += CHUNK) {  // the last chunk stays in registers
                 m = fmaxf(m, fetch(base));
                 if (base + CHUNK >= cnt) break;
@@ -349,6 +354,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
             if (slot && s_new != s_old) {  // the page's other codes move to the new scale
                 const float f = s_old * inv_s;
                 uint4 *old = reinterpret_cast<uint4 *>(dst);
+#pragma unroll 1
                 for (uint32_t i = threadIdx.x; i < V.page_tokens * (HD / 16); i += WARPS * 32) {
                     if (i / (HD / 16) - slot < cnt) continue;  // (unsigned: slots from `slot` on, cnt of them, are the new rows')
                     uint4 u = old[i];
@@ -362,6 +368,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
                 }
             }
             store(base, inv_s);
+#pragma unroll 1
             while (base > 0u) {  // earlier chunks are prepared once more
                 base -= CHUNK;
                 fetch(base);
@@ -497,6 +504,7 @@ extern "C" int strix_cuda_kv_append_dev(strix_cuda *h, const strix_kv_pages *cac
     A.n_heads = d_q ? n_heads : 0u;
     if (prep->rope != STRIX_ROPE_NONE) {
         A.turn[0] = pow((double)prep->theta, -2.0 / (double)A.V.head_dim);
+#pragma unroll 1
         for (int b = 1; b < 8; b++) A.turn[b] = A.turn[b - 1] * A.turn[b - 1];
     }
     A.vec = ((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v) | reinterpret_cast<uintptr_t>(d_q) |

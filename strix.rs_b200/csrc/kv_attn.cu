@@ -62,6 +62,7 @@ struct PaShape {
     static int halves_for(int wm, size_t smem) {  // half tiles of a ring
         const int workers = NW / wm;
         int n = 2 * DESCS - 4;
+#pragma unroll 1
         while (n > 1 && fixed(workers, n) + rings(workers, n) > smem) n--;
         return n;
     }
@@ -130,11 +131,13 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     // ---- running tile counts of the sequences (where the rings will be)
     uint32_t *upto = reinterpret_cast<uint32_t *>(rings);
     const uint32_t total = count_tiles<TT, NW * 32>(A, rb, upto, scan);
+#pragma unroll 1
     for (uint32_t i = threadIdx.x; i < workers * halves; i += NW * 32) {
         mbar_init(&full[i], 1);
         mbar_init(&empty[i], wm);
         mbar_fence_init();
     }
+#pragma unroll 1
     for (uint32_t i = threadIdx.x; i < workers * DESCS * 4u; i += NW * 32) descs[i / 4u].ks[i & 3u] = descs[i / 4u].vs[i & 3u] = 0.f;
     if (threadIdx.x < workers) info[threadIdx.x].has_head = info[threadIdx.x].head_ended = info[threadIdx.x].has_tail = 0u;
 
@@ -196,6 +199,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     };
     // The next segment, if one has ended, and the page ids and scales of its next 32 pages.
     auto next_batch = [&] {
+#pragma unroll 1
         while (ds_left > is_left) describe();
         if (place.at == seg_stop) {
             if (started) next_item<TT>(A, rb, place);
@@ -259,6 +263,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         uint64_t *bar = &full[is_half];
         uint8_t *dst = ring + is_half * S::HALF;
         const CUtensorMap *map = is_v ? &A.v_map : &A.k_map;
+#pragma unroll 1
         for (uint32_t i = 0; i < n_sub; i++) {
             const int page = TT > 16 ? __shfl_sync(0xffffffffu, c_page, i) : c_page;
             const uint32_t y = TT > 16 ? __shfl_sync(0xffffffffu, c_y, i) : c_y;
@@ -294,12 +299,14 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     bool tail_tok = false;
     uint32_t it_first = 0, it_rows = 0, it_row0 = 0, it_head = 0;  // the item: first row of its sequence, new rows, first row of its own, KV head
     const int steps = (int)(2u * n_mine);
+#pragma unroll 1
     for (int step = wi == 0 ? -(int)min(halves, 2u * n_mine) : 0; step < steps; step++) {
         if (step >= 0) {
         const PaTile &d = desc[(uint32_t)step / 2u & (DESCS - 1u)];
         if ((step & 1) == 0) {
             if (wm > 1u) {  // (the other warps get the description with the copy)
                 if (wi == 0)
+#pragma unroll 1
                     while (ds_left > is_left) describe();
                 if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
             }
@@ -386,6 +393,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
 
             // scores: products of q with eight tokens at a time
             if (wm == 1u) {
+#pragma unroll 1
                 while (ds_left > is_left) describe();
                 if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
             }
@@ -537,6 +545,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
             }
         } else {
             if (wi == 0)
+#pragma unroll 1
                 while (ds_left > is_left) describe();
             if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
             const uint8_t *vs = ring + half * S::HALF;
@@ -716,6 +725,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     const uint32_t chains = __popc(tail_set) + front;
     constexpr int DL = (HD / 2 + 31) / 32;  // pairs of a row in a lane
     const PaWorker::Part *cross[2] = {nullptr, nullptr};  // the item that goes on in front, and behind
+#pragma unroll 1
     for (uint32_t c = 0, left = tail_set; c < chains; c++) {
         int a = -1;
         if (c > 0u || !front) {
@@ -729,6 +739,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         const bool out = a < 0 || stop == 0u;
         if (out) cross[a < 0 ? 0 : 1] = &it;
         const uint32_t R = min(rb, it.seq_rows * A.group - it.row0);
+#pragma unroll 1
         for (uint32_t row = (warp + NW - c % NW) % NW; row < R; row += NW) {
             const bool tl = (int)lane == a, mine = tl || ((members >> lane) & 1u);
             const float *p = (tl ? tails : slots) + (size_t)((mine ? lane : 0u) * rb + row) * PS;
@@ -741,6 +752,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
             float2 acc[DL];
 #pragma unroll
             for (int k = 0; k < DL; k++) acc[k] = make_float2(0.f, 0.f);
+#pragma unroll 1
             for (uint32_t set = members | (a >= 0 ? 1u << a : 0u); set; set &= set - 1u) {
                 const uint32_t w = __ffs(set) - 1u;
                 const float fw = __shfl_sync(0xffffffffu, f, w);
@@ -787,12 +799,14 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         }
     }
     __syncthreads();
+#pragma unroll 1
     for (int e = 0; e < 2; e++) {
         if (!last_here[e]) continue;
         __threadfence();
         const PaWorker::Part &it = *cross[e];
         const uint32_t lo = line.part_of(it.item0), n = line.part_of(it.item0 + it.item_tiles - 1u) - lo + 1u;
         const uint32_t R = min(rb, it.seq_rows * A.group - it.row0);
+#pragma unroll 1
         for (uint32_t row = warp; row < R; row += NW) join_row<HD>(A, rb, lo, n, row, item_row(A, HD, it.seq_first, it.row0, it.head, row));
     }
 }
@@ -812,6 +826,7 @@ static int attn_form(const PagedView &V, uint32_t group, uint32_t &wm) {
     if (rows <= 8) return FORM_NARROW;
     if (rows > ROWS_FROM && (V.head_dim == 64 || V.head_dim == 128)) return FORM_ROWS;
     const uint32_t most = V.head_dim >= 192 ? 4u : 8u;
+#pragma unroll 1
     while (wm < most && 16ull * wm < rows) wm *= 2;
     return FORM_WIDE;
 }
@@ -916,6 +931,7 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     if (!d_q || !d_out) return serve_fail(h, who, "d_q or d_out missing");
     if (!d_work || (reinterpret_cast<uintptr_t>(d_work) & 255u)) return serve_fail(h, who, "d_work must be 256-byte aligned");
     A.group = n_heads / A.V.n_kv;
+#pragma unroll 1
     while ((1u << A.g_shift) < A.group) A.g_shift++;
     A.g_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << A.g_shift) - A.group)) / A.group + 1u);
     if (work_bytes < attn_work_bytes(h, A.V, A.group)) return serve_fail(h, who, "work_bytes too small");

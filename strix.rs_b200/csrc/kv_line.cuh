@@ -101,6 +101,7 @@ __device__ __forceinline__ uint32_t seq_tiles(const PagedAttnArgs &A, uint32_t r
     if ((int)P.ctx < 0 || P.rows == 0u) return 0u;
     uint32_t n = 0, lo;
     const uint32_t blocks = (P.rows * A.group + rb - 1u) / rb;
+#pragma unroll 1
     for (uint32_t mb = 0; mb < blocks; mb++) n += block_tiles<TT>(A, rb, P.rows, P.ctx, mb, lo);
     return n * A.V.n_kv;
 }
@@ -108,6 +109,7 @@ __device__ __forceinline__ uint32_t seq_tiles(const PagedAttnArgs &A, uint32_t r
 template <int TT>
 __device__ __forceinline__ void find_place(const PagedAttnArgs &A, uint32_t rb, const uint32_t *upto, uint32_t x, PaPlace &P) {
     uint32_t lo = 0, hi = A.V.n_seq - 1u;  // the first sequence with upto > x
+#pragma unroll 1
     while (lo < hi) {
         const uint32_t mid = (lo + hi) / 2u;
         if (upto[mid] > x) hi = mid; else lo = mid + 1u;
@@ -115,6 +117,7 @@ __device__ __forceinline__ void find_place(const PagedAttnArgs &A, uint32_t rb, 
     load_seq(A, lo, P);
     uint32_t off = x - (lo ? upto[lo - 1u] : 0u), n = 0, first_tile = 0;
     const uint32_t blocks = (P.rows * A.group + rb - 1u) / rb;
+#pragma unroll 1
     for (P.mb = 0;; P.mb++) {
         n = block_tiles<TT>(A, rb, P.rows, P.ctx, P.mb, first_tile);
         if (off < n * A.V.n_kv || P.mb + 1u >= blocks) break;
@@ -133,6 +136,7 @@ __device__ __forceinline__ void next_item(const PagedAttnArgs &A, uint32_t rb, P
     P.at = 0;
     if (++P.head < A.V.n_kv) return;
     P.head = 0;
+#pragma unroll 1
     for (;;) {
         const uint32_t blocks = (P.rows * A.group + rb - 1u) / rb;
         if ((int)P.ctx >= 0 && ++P.mb < blocks) {
@@ -190,12 +194,14 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs &A, uint32_t rb, ui
     const uint32_t lane = threadIdx.x & 31u;
     auto part = [&](uint32_t i) { return A.part + (((size_t)(lo + i) * 2u + (i == 0u ? 1u : 0u)) * rb + row) * PS; };
     float M = -INFINITY, L = 0.f;
+#pragma unroll 1
     for (uint32_t i = lane; i < n; i += 32u) M = fmaxf(M, __ldcg(part(i) + HD));
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
     float2 acc[DL];
 #pragma unroll
     for (int k = 0; k < DL; k++) acc[k] = make_float2(0.f, 0.f);
+#pragma unroll 1
     for (uint32_t base = 0; base < n; base += 32u) {
         const uint32_t cnt = min(32u, n - base);
         float2 ml = make_float2(-INFINITY, 0.f);
@@ -232,6 +238,7 @@ __device__ __forceinline__ bool empty_rows(const PagedAttnArgs &A, uint32_t rb, 
     const PagedView &V = A.V;
     const uint32_t lane = threadIdx.x & 31u;
     bool bad = false;
+#pragma unroll 1
     for (uint32_t s = blockIdx.x * n_warps + warp; s < V.n_seq; s += gridDim.x * n_warps) {
         uint32_t first, end;
         seq_rows(V, s, first, end, bad);
@@ -241,12 +248,16 @@ __device__ __forceinline__ bool empty_rows(const PagedAttnArgs &A, uint32_t rb, 
         bad |= over;
         if (ctx < 0 || over) {
             const uint32_t R = rows * A.group, nb = (R + rb - 1u) / rb;
+#pragma unroll 1
             for (uint32_t mb = 0; mb < nb; mb++) {
                 uint32_t lo;
                 if (ctx >= 0 && block_tiles<TT>(A, rb, rows, (uint32_t)ctx, mb, lo)) continue;
+#pragma unroll 1
                 for (uint32_t r = mb * rb; r < min(R, (mb + 1u) * rb); r++)
+#pragma unroll 1
                     for (uint32_t h = 0; h < V.n_kv; h++) {
                         float *dst = item_row(A, HD, first, r, h, 0u);
+#pragma unroll 1
                         for (uint32_t i = lane; i < HD; i += 32u) dst[i] = 0.f;
                     }
             }
@@ -260,6 +271,7 @@ template <int TT, int THREADS>
 __device__ __forceinline__ uint32_t count_tiles(const PagedAttnArgs &A, uint32_t rb, uint32_t *upto, uint32_t *scan) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     uint32_t total = 0;
+#pragma unroll 1
     for (uint32_t c = 0; c < A.V.n_seq; c += THREADS) {
         uint32_t n = c + threadIdx.x < A.V.n_seq ? seq_tiles<TT>(A, rb, c + threadIdx.x) : 0u;
 #pragma unroll
@@ -270,6 +282,7 @@ __device__ __forceinline__ uint32_t count_tiles(const PagedAttnArgs &A, uint32_t
         if (lane == 31u) scan[warp] = n;
         __syncthreads();
         uint32_t before = total;
+#pragma unroll 1
         for (uint32_t w = 0; w < THREADS / 32; w++) {
             if (w < warp) before += scan[w];
             total += scan[w];

@@ -242,6 +242,7 @@ struct SampleRow {
         const uint32_t t = threadIdx.x;
         if (n <= 256u) {  // by rank: every entry counts the smaller ones, SAMPLE_THREADS / np threads to an entry
             uint32_t np = 32;
+#pragma unroll 1
             while (np < n) np *= 2;
             if (t < 256u) S.rank[t] = 0u;
             __syncthreads();
@@ -249,6 +250,7 @@ struct SampleRow {
             if (e < n) {
                 const u64 mine = S.list.e[e];
                 uint32_t less = 0;
+#pragma unroll 1
                 for (uint32_t j = part; j < n; j += parts) less += S.list.e[j] < mine || (S.list.e[j] == mine && j < e);
                 if (less) atomicAdd(&S.rank[e], less);
             }
@@ -260,11 +262,16 @@ struct SampleRow {
             return;
         }
         uint32_t np = 512;  // bitonic
+#pragma unroll 1
         while (np < n) np *= 2;
+#pragma unroll 1
         for (uint32_t i = n + t; i < np; i += SAMPLE_THREADS) S.list.e[i] = ~0ull;
         __syncthreads();
+#pragma unroll 1
         for (uint32_t k = 2; k <= np; k *= 2)
+#pragma unroll 1
             for (uint32_t j = k / 2; j > 0; j /= 2) {
+#pragma unroll 1
                 for (uint32_t h = t; h < np / 2; h += SAMPLE_THREADS) {
                     const uint32_t a = 2 * h - (h & (j - 1u)), b = a + j;
                     const u64 p = S.list.e[a], q = S.list.e[b];
@@ -301,6 +308,7 @@ struct SampleRow {
                 const uint32_t kr = __shfl_sync(0xffffffffu, k, r), at = __shfl_sync(0xffffffffu, upto, r) - kr;
                 if (r > 0u) {
                     const u64 *src = cg::this_cluster().map_shared_rank(&S.list.e[0], r);
+#pragma unroll 1
                     for (uint32_t i = part * 32u + lane; i < kr && at + i < SAMPLE_CAP; i += (SAMPLE_WARPS / C) * 32u) S.list.e[at + i] = src[i];
                 }
                 n = min(n, SAMPLE_CAP);
@@ -350,6 +358,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         m = fmaxf(m, v);
     }
     if (t < (-cnt & 3u)) own[cnt + t] = -INFINITY;
+#pragma unroll 1
     for (uint32_t i = t; i < SAMPLE_BINS / 2; i += SAMPLE_THREADS) S.hist[i] = 0u;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -372,6 +381,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     // this thread's stretch where index order matters (of an odd length: no bank conflicts)
     const uint32_t seg = ((cnt + SAMPLE_THREADS - 1) / SAMPLE_THREADS) | 1u, i0 = min(cnt, t * seg), i1 = min(cnt, i0 + seg);
     if (m == INFINITY) {  // only the infinite ones have weight: as if they were the only ones
+#pragma unroll 1
         for (uint32_t i = t; i < cnt; i += SAMPLE_THREADS) own[i] = own[i] == INFINITY ? 0.f : -INFINITY;
         m = 0.f;
         __syncthreads();
@@ -383,6 +393,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     if (m == -INFINITY || greedy) {  // no token, or the first of the largest
         u64 best[1] = {0xffffffffull};
         if (m > -INFINITY)
+#pragma unroll 1
             for (uint32_t i = i1; i-- > i0;)
                 if (xs[i] == m) best[0] = base + i;
         R.fold(best, OpMin());
@@ -412,6 +423,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         float sm[SAMPLE_BPT], a_total = 0.f, delta = 0.f, mid = 0.f;
         u64 all = 0;  // the weights of the whole row
         bool by_k = false;
+#pragma unroll 1
         for (float orders = SAMPLE_NEAR;; orders = SAMPLE_ORDERS) {
             R.bins_over(orders);
             mid = orders / SAMPLE_BINS;
@@ -505,6 +517,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             by_k = want_k && (uint32_t)top_k < n_weight;
             if (orders == SAMPLE_ORDERS || by_k || (!want_k && (double)a_total * (1.0 - delta) * 1099511627776.0 >= (double)top_p * (double)all)) break;
             Row::csync();  // (all have read the counts)
+#pragma unroll 1
             for (uint32_t i = t; i < SAMPLE_BINS / 2; i += SAMPLE_THREADS) S.hist[i] = 0u;
             __syncthreads();
         }
@@ -553,6 +566,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                         return x + __shfl_xor_sync(0xffffffffu, x, 4);
                     };
                     u64 rk = 0;
+#pragma unroll 1
                     for (uint32_t j = part; j < n; j += 8u) rk += S.list.e[j] < e;
                     rk = eight(rk);
                     u64 w = i < n && rk < kk ? Row::steps(R.order(v)) : 0ull;
@@ -560,6 +574,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                     __syncthreads();
                     if (nucleus) {
                         u64 bef = 0, of_k = 0;
+#pragma unroll 1
                         for (uint32_t j = part; j < n; j += 8u) {
                             of_k += weight[j];
                             bef += S.list.e[j] < e ? weight[j] : 0ull;
@@ -574,6 +589,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                     if (part == 0u) weight[i] = w;
                     __syncthreads();
                     u64 upto = 0, total = 0;
+#pragma unroll 1
                     for (uint32_t j = part; j < n; j += 8u) {
                         total += weight[j];
                         upto += (uint32_t)S.list.e[j] <= (uint32_t)e ? weight[j] : 0ull;
@@ -646,11 +662,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         // the index of the quota-th kept token with this key
         auto tie_index = [&](uint32_t key, const Cut &old, u64 quota) {
             u64 mine = 0, all;
+#pragma unroll 1
             for (uint32_t i = i0; i < i1; i++) mine += logit_key(xs[i]) == key && old.keeps(xs[i], base + i);
             const u64 bef = R.before_all(mine, all);
             u64 at[1] = {0};
             if (bef < quota && quota <= bef + mine) {
                 u64 q = bef;
+#pragma unroll 1
                 for (uint32_t i = i0; i < i1; i++)
                     if (logit_key(xs[i]) == key && old.keeps(xs[i], base + i) && ++q == quota) {
                         at[0] = base + i;
@@ -663,6 +681,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         // smallest and largest key among the tokens `in` names
         auto key_range = [&](auto in, uint32_t &lo, uint32_t &hi) {
             u64 r[2] = {0ull, 0ull};
+#pragma unroll 1
             for (uint32_t i = i0; i < i1; i++)
                 if (in(xs[i], base + i)) {
                     const uint32_t key = logit_key(xs[i]);
@@ -688,13 +707,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             } else {  // the largest key that `quota` tokens of the bin reach
                 uint32_t lo, hi;
                 key_range(in, lo, hi);
+#pragma unroll 1
                 while (lo < hi) {
                     const uint32_t mid_key = lo + (hi - lo + 1u) / 2u;
                     u64 n = 0;
+#pragma unroll 1
                     for (uint32_t i = i0; i < i1; i++) n += in(xs[i], 0u) && logit_key(xs[i]) >= mid_key;
                     if (R.sum(n) >= quota) lo = mid_key; else hi = mid_key - 1u;
                 }
                 u64 n = 0;
+#pragma unroll 1
                 for (uint32_t i = i0; i < i1; i++) n += in(xs[i], 0u) && logit_key(xs[i]) > lo;
                 n = R.sum(n);
                 cut = Cut{key_logit(lo), tie_index(lo, cut, quota - n)};
@@ -725,6 +747,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             const uint32_t b_hi = S.second, b_lo = min(S.first, b_hi);  // the uncertain bins
             // exact masses: of what lies above them, and of 2048 finer bins
             __syncthreads();
+#pragma unroll 1
             for (uint32_t i = t; i < SAMPLE_BINS; i += SAMPLE_THREADS) {
                 S.fine.mass[i] = 0ull;
                 S.fine.count[i] = 0u;
@@ -819,14 +842,17 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                 } else {  // the least key above which the mass is below `need`, then how many of its equals
                     uint32_t lo, hi;
                     key_range(in, lo, hi);
+#pragma unroll 1
                     while (lo < hi) {
                         const uint32_t mid_key = lo + (hi - lo) / 2u;
                         u64 w = 0;
+#pragma unroll 1
                         for (uint32_t i = i0; i < i1; i++)
                             if (logit_key(xs[i]) > mid_key && in(xs[i], base + i)) w += Row::steps(R.order(xs[i]));
                         if ((double)(mass_above + R.sum(w)) < need) hi = mid_key; else lo = mid_key + 1u;
                     }
                     u64 v[2] = {0ull, 0ull};
+#pragma unroll 1
                     for (uint32_t i = i0; i < i1; i++)
                         if (in(xs[i], base + i)) {
                             const uint32_t key = logit_key(xs[i]);
@@ -875,11 +901,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         const uint32_t j0 = min(s1, s0 + t * part), j1 = min(s1, j0 + part);
         auto steps = [](float w) { return w > 0.f ? max(1ull, __float2ull_rn(w * 1099511627776.f)) : 0ull; };  // (something is kept here)
         mine = 0;
+#pragma unroll 1
         for (uint32_t i = j0; i < j1; i++) mine += steps(value(xs[i], i));
         u64 of_part;
         u64 at = S.found[0] + R.before(mine, of_part);
         const u64 end = S.found[0] + of_part, goal = target < end ? target : end - 1u;
         if (at <= goal && at + mine > goal) {
+#pragma unroll 1
             for (uint32_t i = j0; i < j1; i++) {
                 const u64 v = steps(value(xs[i], i));
                 at += v;
@@ -922,6 +950,7 @@ static cudaError_t sample_launch(strix_cuda *h, const SampleArgs &A, uint32_t ro
 cudaError_t launch_sample(strix_cuda *h, const float *d_x, uint32_t n, size_t stride, uint32_t rows, const strix_sample_params &p,
                           const float *d_u, uint32_t *d_ids, float *d_probs, cudaStream_t stream) {
     uint32_t c = 1;
+#pragma unroll 1
     while (c < 8 && (n + c - 1) / c > 4096) c *= 2;
     const SampleArgs A{d_x, stride, n, ((n + c - 1) / c + 3u) & ~3u, p, d_u, d_ids, d_probs};
     static_assert(sizeof(SampleShared) + (STRIX_SAMPLE_MAX_N / 8 + 4) * 4 <= 231000, "the longest row fits eight blocks");
