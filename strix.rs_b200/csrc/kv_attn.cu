@@ -826,7 +826,6 @@ static int attn_form(const PagedView &V, uint32_t group, uint32_t &wm) {
     if (rows <= 8) return FORM_NARROW;
     if (rows > ROWS_FROM && (V.head_dim == 64 || V.head_dim == 128)) return FORM_ROWS;
     const uint32_t most = V.head_dim >= 192 ? 4u : 8u;
-#pragma unroll 1
     while (wm < most && 16ull * wm < rows) wm *= 2;
     return FORM_WIDE;
 }

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         for (uint32_t i = 0; i < RA_STATS; i++) mbar_init(&m_full[i], 4);
         mbar_fence_init();
         gave_up = 0u;
-        parts.has_front = parts.has_back = 0u;
+        parts.has_front = parts.has_back = last_here[0] = last_here[1] = 0u;
     }
     for (uint32_t i = threadIdx.x; i < RA_DESCS * 4u; i += RA_THREADS) desc[i / 4u].ks[i & 3u] = desc[i / 4u].vs[i & 3u] = 0.f;
     if (warp == 17) {
@@ -177,6 +177,21 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 gave_up = 1u;
                 break;
             }
+    };
+    // ... joins their parts, with warps 0 to 15
+    auto join = [&] {
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+#pragma unroll 1
+        for (int e = 0; e < 2; e++) {
+            if (!last_here[e]) continue;
+            __threadfence();
+            const PaCuts line(total, line_blocks);
+            const PaPart &it = e == 0 ? parts.front : parts.back;
+            const uint32_t lo = line.part_of(it.item0), cnt = line.part_of(it.item0 + it.item_tiles - 1u) - lo + 1u;
+            const uint32_t R = min(RA_ROWS, it.seq_rows * A.group - it.row0);
+#pragma unroll 1
+            for (uint32_t r = warp; r < R; r += 16u) join_row<HD>(A, RA_ROWS, lo, cnt, r, item_row(A, HD, it.seq_first, it.row0, it.head, r));
+        }
     };
     const uint32_t pshift = V.page_shift;
     const bool mixed = V.page_tokens < RA_TT;
@@ -268,6 +283,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 mbar_arrive(&p_full[b]);
             }
         }
+        join();
     } else if (warp < 12) {
         // ---- sums: warps 8-11 add the tiles' products to O, whose row is kept by a thread, and write the finished items
         asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
@@ -337,14 +353,12 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             }
             wrote |= !(flags & PA_WHOLE);
         }
-        // ---- items that several blocks have: the last of them to come here joins their parts
-        if (wrote) {
+        if (wrote) {  // items that several blocks have: is this the last of them to come here?
             const PaCuts line(total, line_blocks);
             __threadfence();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 2, 128;" ::: "memory");
             if (warp < 10u && lane == 0) {
                 const uint32_t e = warp - 8u;
-                last_here[e] = 0u;
                 if (e == 0 ? parts.has_front : parts.has_back) {
                     const PaPart &it = e == 0 ? parts.front : parts.back;
                     const uint32_t lo = line.part_of(it.item0), hi = line.part_of(it.item0 + it.item_tiles - 1u);
@@ -354,16 +368,8 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     }
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            for (int e = 0; e < 2; e++) {
-                if (!last_here[e]) continue;
-                __threadfence();
-                const PaPart &it = e == 0 ? parts.front : parts.back;
-                const uint32_t lo = line.part_of(it.item0), cnt = line.part_of(it.item0 + it.item_tiles - 1u) - lo + 1u;
-                const uint32_t R = min(RA_ROWS, it.seq_rows * A.group - it.row0);
-                for (uint32_t r = warp - 8u; r < R; r += 4u) join_row<HD>(A, RA_ROWS, lo, cnt, r, item_row(A, HD, it.seq_first, it.row0, it.head, r));
-            }
         }
+        join();
     } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         // ---- operands: q of a new item; every tile's k and v
@@ -453,6 +459,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 }
             }
         }
+        join();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 16) {

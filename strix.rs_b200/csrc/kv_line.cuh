@@ -208,7 +208,7 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs &A, uint32_t rb, ui
         if (lane < cnt) ml = __ldcg(reinterpret_cast<const float2 *>(part(base + lane) + HD));
         const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
         L += f * ml.y;
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t i = 0; i < cnt; i++) {
             const float fw = __shfl_sync(0xffffffffu, f, i);
             const float2 *src = reinterpret_cast<const float2 *>(part(base + i));
