@@ -930,7 +930,6 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     if (!d_q || !d_out) return serve_fail(h, who, "d_q or d_out missing");
     if (!d_work || (reinterpret_cast<uintptr_t>(d_work) & 255u)) return serve_fail(h, who, "d_work must be 256-byte aligned");
     A.group = n_heads / A.V.n_kv;
-#pragma unroll 1
     while ((1u << A.g_shift) < A.group) A.g_shift++;
     A.g_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << A.g_shift) - A.group)) / A.group + 1u);
     if (work_bytes < attn_work_bytes(h, A.V, A.group)) return serve_fail(h, who, "work_bytes too small");

@@ -412,6 +412,130 @@ def test_attention_bad_device_data_is_masked(torch, pkg, accel):
         check_attention(torch, accel, P, b, [0, 1], [1000], 2, q[:1], out[:1], 0.125, 0)
 
 
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 32), (64, 64), (128, 128), (128, 16)])
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("window", [0, 3, 70])
+def test_attention_row_blocks(torch, pkg, accel, kv, hd, page, window):
+    """More than 16 rows a KV head: blocks of 128 rows, ragged ones, several to a sequence, next to single tokens, an idle slot and a
+    sequence without rows; garbage (NaN codes) behind the ends; padded pages and rows that do not start on 16 bytes."""
+    run_attention(torch, pkg, accel, kv, 2, 4, page, hd, [33, 1, 70, 0, 9, 4], [0, 130, 61, 20, -1, 300], window=window, fill=0xff,
+                  pad=0 if window else 48, ldpad=1 if window == 3 else 4 if window else 0)
+
+
+@pytest.mark.parametrize("kv,hd", [(0, 128), (1, 128), (1, 64)])
+def test_attention_row_blocks_split_and_joined(torch, pkg, accel, kv, hd):
+    """Long contexts, so that several blocks share a row block and join; 40 rows of one head are one block, 140 two."""
+    run_attention(torch, pkg, accel, kv, 1, 4, 64, hd, [10, 35], [4003, 2500])
+
+
+def test_attention_row_blocks_extreme_scores_and_scales(torch, pkg, accel):
+    for kv in (pkg.KV_E4M3, pkg.KV_F16):
+        run_attention(torch, pkg, accel, kv, 1, 8, 16, 128, [5, 6], [90, 200], qs=500.0)
+        run_attention(torch, pkg, accel, kv, 1, 8, 16, 128, [5, 6], [90, 200], qs=0.0)
+    P, b, row0, q, out, w = run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 8, 16, 64, [4], [100])
+    for m, lo, hi in (("v", -15, 15), ("k", -20, -3)):
+        P.scale[m].copy_(torch.exp2(torch.linspace(lo, hi, P.n_pages, device="cuda").round())[:, None])
+    for scale in (0.125, -0.125, 0.0):
+        assert accel.attn_pages_dev(P.desc, b, 8, q.data_ptr(), out.data_ptr(), scale, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        # (a negative scale: the bound counts magnitudes)
+        check_attention(torch, accel, P, b, row0, [100], 8, q if scale >= 0 else -q, out, abs(scale), 0)
+
+
+def test_attention_row_blocks_nan_query_and_bad_pages(torch, pkg, accel):
+    P, b, row0, q, out, w = run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 4, 16, 64, [9, 20], [40, 50])
+    good = out.clone()
+    q[1, 64] = float("nan")            # row 1, head 1
+    assert accel.attn_pages_dev(P.desc, b, 4, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+    torch.cuda.synchronize()
+    assert torch.isnan(out[1, 64:128]).all()
+    out[1, 64:128] = good[1, 64:128]
+    assert torch.equal(out, good)
+    for kv in (pkg.KV_F16, pkg.KV_E4M3):
+        P = Paged(torch, pkg, kv, 1, 16, 128, [64, 16, 48], fill=0xff)
+        P.seed_random(3, [64, 16, 48])
+        P.table[0, 1], P.table[1, 0] = P.n_pages, -5
+        P.d_table.copy_(torch.from_numpy(P.table))
+        row0, ctx = [0, 6, 11, 22], [58, 3, 37]
+        hole = [np.repeat((P.table[s] < 0) | (P.table[s] >= P.n_pages), 16) for s in range(3)]
+        q = torch.randn(24, 4 * 128, device="cuda")
+        out = torch.full_like(q, 5.0)
+        b = P.batch(row0, ctx, 24)
+        w = work_of(torch, accel, P, b, 4)
+        assert accel.attn_pages_dev(P.desc, b, 4, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        assert accel.device_status() & 2
+        accel.clear_device_status()
+        assert (out[6:11] == 0).all() and (out[22:] == 5.0).all()
+        check_attention(torch, accel, P, b, row0, ctx, 4, q, out, 0.125, 0, hole=hole)
+
+
+def test_attention_graph_serves_changing_lengths(torch, pkg, accel):
+    """One captured graph, replayed on a stream of its own with other lengths, rows and pages each time; a workspace that larger and
+    smaller calls share."""
+    for new_max in (1, 24):
+        n_seq, hd, page, heads = 3, 128, 32, 4
+        P = Paged(torch, pkg, pkg.KV_E4M3, 1, page, hd, [400] * n_seq)
+        P.seed_random(9, [400] * n_seq)
+        rows = n_seq * new_max
+        q = torch.randn(rows, heads * hd, device="cuda")
+        out = torch.zeros_like(q)
+        b = P.batch([i * new_max for i in range(n_seq + 1)], [0] * n_seq, rows)
+        w = work_of(torch, accel, P, b, heads)
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                assert accel.attn_pages_dev(P.desc, b, heads, q.data_ptr(), out.data_ptr(), 0.1, w.data_ptr(), w.numel(), stream=st.cuda_stream)
+        for ctx, new in (([0, 5, 376], [1, 1, 1]), ([300, -1, 64], [1, 1, new_max]), ([376, 376, 376], [new_max] * 3), ([10, 20, 30], [0, 1, 0])):
+            row0 = np.cumsum([0] + new).tolist()
+            with torch.cuda.stream(st):
+                P.row0.copy_(_i32(torch, row0))
+                P.ctx.copy_(_i32(torch, ctx))
+                out.fill_(5.0)
+                g.replay()
+            st.synchronize()
+            assert accel.device_status() == 0 and (out[row0[-1]:] == 5.0).all()
+            check_attention(torch, accel, P, b, row0, ctx, heads, q, out, 0.1, 0)
+
+
+def test_serving_calls_refuse(torch, pkg, accel):
+    """Wrong arguments are errors with a message, other shapes are declined; nothing is launched."""
+    P = Paged(torch, pkg, pkg.KV_F16, 2, 16, 64, [32])
+    x = torch.zeros(4, 512, device="cuda")
+    b, p = P.batch([0, 1], [0]), x.data_ptr()
+    w = work_of(torch, accel, P, b, 4)
+    attn = lambda **k: accel.attn_pages_dev(P.desc, k.get("b", b), k.get("heads", 4), k.get("q", p), p, 1.0, k.get("w", w.data_ptr()),  # noqa: E731
+                                            k.get("n", w.numel()), ld_q=k.get("ld", 0))
+    for kw in (dict(q=0), dict(w=0), dict(w=w.data_ptr() + 16), dict(n=w.numel() - 1), dict(ld=255)):
+        with pytest.raises(pkg.StrixCudaError):
+            attn(**kw)
+    assert attn(heads=3) is False and attn(heads=0) is False
+    for sizes in ((8193, 8193), (1, 0x7fffffff)):
+        many = pkg.KvBatch(*sizes, P.row0.data_ptr(), P.ctx.data_ptr(), P.d_table.data_ptr(), P.ld)
+        with pytest.raises(pkg.StrixCudaError):
+            attn(b=many)
+        with pytest.raises(pkg.StrixCudaError):
+            accel.attn_pages_workspace(P.desc, many, 4)
+    prep = pkg.KvPrep(rope=pkg.ROPE_HALVES)
+    app = lambda **k: accel.kv_append_dev(P.desc, b, k.get("k", p), p, k.get("prep", prep), n_heads=k.get("heads", 0), d_q=k.get("q", 0),  # noqa: E731
+                                          d_q_out=k.get("o", 0), ld_k=k.get("ld", 0))
+    for kw in (dict(k=0), dict(ld=127), dict(heads=4, q=p), dict(prep=pkg.KvPrep(rope=3)), dict(prep=pkg.KvPrep(rope=1, theta=0.0))):
+        with pytest.raises(pkg.StrixCudaError):
+            app(**kw)
+    samp = lambda **k: accel.sample_dev(k.get("x", p), k.get("n", 16), k.get("stride", 16), k.get("rows", 2), k.get("u", p), k.get("ids", p))  # noqa: E731
+    for kw in (dict(x=0), dict(u=0), dict(ids=0), dict(n=0), dict(n=pkg.SAMPLE_MAX_N + 1, rows=1), dict(stride=15), dict(rows=1 << 31)):
+        with pytest.raises(pkg.StrixCudaError):
+            samp(**kw)
+    # nothing to do is done
+    assert samp(rows=0)
+    none = pkg.KvBatch(0, 0, P.row0.data_ptr(), P.ctx.data_ptr(), P.d_table.data_ptr(), P.ld)
+    assert attn(b=none) and accel.kv_append_dev(P.desc, none, p, p, prep)
+    torch.cuda.synchronize()
+    assert accel.device_status() == 0 and (x == 0).all()
+
+
 # ---------------------------------------------------------------- sampling
 
 def sample(torch, accel, x, u, temperature=None, top_k=None, top_p=None, min_p=None, stride=None):
@@ -528,3 +652,64 @@ def test_sample_follows_the_distribution(torch, accel):
     ids, _ = sample(torch, accel, np.tile(row, (grid, 1)), (np.arange(grid) + 0.5) / grid)
     p = np.exp(row.astype(np.float64)) / np.exp(row.astype(np.float64)).sum()
     assert (np.abs(np.bincount(ids, minlength=n) / grid - p) <= 1.0 / grid + 1e-6).all()
+
+
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_decode_step_sample_draws_from_the_logits_of_the_step(torch, pkg, orc, synth, cap):
+    """The token and its probability are those of a draw from decode_step's logits; without a configured model there is none."""
+    from test_argmax_gpu import build_model
+    hidden, qdim, kvdim, ffn, vocab, n_layers = 512, 768, 256, 1536, 3000, 2
+    acc = pkg.CudaWeightAccel(0)
+    try:
+        assert acc.decode_step_sample(np.zeros(hidden, np.float32), 0, 0.5) is None
+        build_model(acc, synth, hidden, qdim, kvdim, ffn, vocab, n_layers)
+        assert acc.configure_decode(hidden, qdim // 128, ffn, vocab, n_layers, eps=1e-6, act=pkg.ACT_F32, final_softcap=cap)
+        for seed, kw in ((1, dict()), (2, dict(temperature=0.7, top_k=40, top_p=0.9)), (3, dict(temperature=0.0)), (4, dict(min_p=0.1, temperature=1.5))):
+            h0, u = synth.normal(90 + seed, "h0", hidden), 0.17 * seed
+            logits = acc.decode_step(h0, 0)
+            tok, prob = acc.decode_step_sample(h0, 0, u, **kw)
+            one = lambda k: None if k not in kw else [kw[k]]  # noqa: E731
+            check_sample(logits[None], np.array([u], np.float32), [tok], [prob], one("temperature"), one("top_k"), one("top_p"), one("min_p"))
+        assert acc.device_status() == 0
+    finally:
+        acc.close()
+
+
+def test_a_layer_serves_a_batch_step_by_step(torch, pkg, accel, synth):
+    """The operators as a server runs them, over the framework's own projections: q, k and v rows from quantised weights, append,
+    attention, output projection, head, draw, the next tokens' rows from the drawn ids: a prompt of uneven lengths, then single
+    tokens; against 64-bit attention over the cache that the steps built, and 64-bit draws from the logits."""
+    hid, heads, n_kv, hd, vocab, page = 256, 4, 2, 64, 500, 16
+    kinds = dict(q=heads * hd, k=n_kv * hd, v=n_kv * hd, head=vocab)
+    for name, dim in kinds.items():
+        assert accel.upload_q8_0("serve." + name, synth.quant(8, 60, name, dim, hid), hid, dim)
+    assert accel.upload_q8_0("serve.o", synth.quant(8, 60, "o", hid, heads * hd), heads * hd, hid)
+    rng = np.random.RandomState(5)
+    emb = rng.randn(vocab, hid).astype(np.float32)
+    for kv in (pkg.KV_E4M3, pkg.KV_F16):
+        P = Paged(torch, pkg, kv, n_kv, page, hd, [40, 40, 40], fill=0)
+        ctx, toks = [0, 0, 0], [rng.randint(0, vocab, n) for n in (7, 1, 18)]
+        prep = pkg.KvPrep(rope=pkg.ROPE_HALVES, theta=1e4)
+        w = torch.zeros(accel.attn_pages_workspace(P.desc, P.batch([0, 7, 8, 26], ctx), heads), dtype=torch.uint8, device="cuda")
+        for step in range(4):
+            row0 = np.cumsum([0] + [len(t) for t in toks]).tolist()
+            x = emb[np.concatenate(toks)]
+            project = lambda name, a: np.stack([accel.gemv("serve." + name, r) for r in a])  # noqa: E731
+            q, k, v = (torch.from_numpy(project(n, x)).cuda() for n in "qkv")
+            b = P.batch(row0, ctx)
+            need = accel.attn_pages_workspace(P.desc, b, heads)
+            if need > w.numel():
+                w = torch.zeros(need, dtype=torch.uint8, device="cuda")
+            out = torch.zeros(row0[-1], heads * hd, device="cuda")
+            assert accel.kv_append_dev(P.desc, b, k.data_ptr(), v.data_ptr(), prep, n_heads=heads, d_q=q.data_ptr(), d_q_out=q.data_ptr(), stream=stream(torch))
+            assert accel.attn_pages_dev(P.desc, b, heads, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+            torch.cuda.synchronize()
+            check_attention(torch, accel, P, b, row0, ctx, heads, q, out, 0.125, 0)
+            last = out.cpu().numpy()[[e - 1 for e in row0[1:]]]
+            logits = project("head", x[[e - 1 for e in row0[1:]]] + project("o", last))
+            u = rng.rand(3).astype(np.float32)
+            ids, probs = sample(torch, accel, logits, u, temperature=[0.8, 0.0, 1.2], top_k=[50, 0, 0], top_p=[0.95, 1.0, 0.9])
+            check_sample(logits, u, ids, probs, [0.8, 0.0, 1.2], [50, 0, 0], [0.95, 1.0, 0.9])
+            ctx = [c + len(t) for c, t in zip(ctx, toks)]
+            toks = [[int(i)] for i in ids]
+        assert accel.device_status() == 0
