@@ -552,49 +552,64 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             }
             report_bad(V, bad);
         } else if (warp == 17) {
-            // ---- products, by one lane
+            // ---- products S, by one lane
             if (elect_lane()) {
                 const uint32_t q_at = smem_u32(q_smem), op_at = smem_u32(op);
-                constexpr uint32_t I_S = rows_idesc(RA_TT, false), I_O = rows_idesc(HD, true);
-                uint64_t *k_free = EL == 1 ? op_empty : land_empty, *v_free = k_free + (EL == 1 ? NS : NL);
-                auto weigh = [&](uint32_t n) {  // O of tile n
-                    const uint32_t b = n & 1u, st = n % NS;
-                    wait(&p_full[b], (n >> 1) & 1u);
-                    wait(&op_full[NS + st], (n / NS) & 1u);
+                constexpr uint32_t I_S = rows_idesc(RA_TT, false);
+                uint64_t *k_free = EL == 1 ? op_empty : land_empty;
+                const uint64_t q = desc_sw128(q_at, 16u);
+                uint32_t items = 0, st = 0, phase = 0;
+#pragma unroll 1
+                for (uint32_t n = 0; n < n_tiles; n++) {
+                    const uint32_t b = n & 1u;
+                    wait(&op_full[st], phase);
+                    const uint32_t flags = desc[n % RA_DESCS].flags;
+                    if (flags & PA_NEW) wait(q_full, items++ & 1u);
+                    wait(&s_empty[b], ((n >> 1) & 1u) ^ 1u);
+                    tc_fence_after();
+                    const uint32_t d = tmem + b * 64u;
+                    const uint64_t kk = desc_sw128(op_at + st * S::OPB, 16u);
+#pragma unroll
+                    for (uint32_t i = 0; i < 2u * S::BLOCKS; i++)  // the remainders first; 64 dimensions at a time
+#pragma unroll
+                        for (uint32_t k = 0; k < 4u; k++)
+                            tc_mma_ss(d, q + (i < S::BLOCKS ? S::QB / 16u : 0u) + (i % S::BLOCKS) * (128u * 128u / 16u) + 2u * k,
+                                      kk + (i % S::BLOCKS) * (8192u / 16u) + 2u * k, I_S, i + k);
+                    tc_commit(&s_full[b]);
+                    tc_commit(&k_free[st]);
+                    if (flags & PA_END) tc_commit(q_empty);
+                    if (++st == NS) {
+                        st = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        } else if (warp == 18) {
+            // ---- products O, by one lane
+            if (elect_lane()) {
+                const uint32_t op_at = smem_u32(op);
+                constexpr uint32_t I_O = rows_idesc(HD, true);
+                uint64_t *v_free = EL == 1 ? op_empty + NS : land_empty + NL;
+                uint32_t st = 0, phase = 0;
+#pragma unroll 1
+                for (uint32_t n = 0; n < n_tiles; n++) {
+                    const uint32_t b = n & 1u;
+                    wait(&op_full[NS + st], phase);
                     wait(&o_empty[b], ((n >> 1) & 1u) ^ 1u);
+                    wait(&p_full[b], (n >> 1) & 1u);
                     tc_fence_after();
                     const uint64_t v = desc_sw128(op_at + (NS + st) * S::OPB, 8192u);
                     const uint32_t d = tmem + S::COL_O + b * HD, p = tmem + S::COL_P + b * 64u;
-#pragma unroll 1
+#pragma unroll
                     for (int h = 0; h < 2; h++)  // the remainders first
 #pragma unroll
                         for (int k = 0; k < 4; k++) tc_mma_ts(d, p + (h ? 0u : 32u) + 8u * k, v + (uint64_t)(k * 2048 / 16), I_O, h || k);
                     tc_commit(&o_full[b]);
-                    tc_commit(&v_free[EL == 1 ? st : n % NL]);
-                };
-                uint32_t items = 0;
-#pragma unroll 1
-                for (uint32_t n = 0; n < n_tiles + 2u; n++) {
-                    if (n < n_tiles) {
-                        const uint32_t b = n & 1u, st = n % NS;
-                        wait(&op_full[st], (n / NS) & 1u);
-                        const uint32_t flags = desc[n % RA_DESCS].flags;
-                        if (flags & PA_NEW) wait(q_full, items++ & 1u);
-                        wait(&s_empty[b], ((n >> 1) & 1u) ^ 1u);
-                        tc_fence_after();
-                        const uint32_t d = tmem + b * 64u;
-                        const uint64_t q = desc_sw128(q_at, 16u), kk = desc_sw128(op_at + st * S::OPB, 16u);
-#pragma unroll 1
-                        for (uint32_t i = 0; i < 2u * S::BLOCKS; i++) {  // the remainders first; 64 dimensions at a time
-                            const uint64_t qi = q + (i < S::BLOCKS ? S::QB / 16u : 0u) + (i % S::BLOCKS) * (128u * 128u / 16u), ki = kk + (i % S::BLOCKS) * (8192u / 16u);
-#pragma unroll
-                            for (uint32_t k = 0; k < 4u; k++) tc_mma_ss(d, qi + 2u * k, ki + 2u * k, I_S, i + k);
-                        }
-                        tc_commit(&s_full[b]);
-                        tc_commit(&k_free[EL == 1 ? st : n % NL]);
-                        if (flags & PA_END) tc_commit(q_empty);
+                    tc_commit(&v_free[st]);
+                    if (++st == NS) {
+                        st = 0;
+                        phase ^= 1u;
                     }
-                    if (n >= 2u) weigh(n - 2u);
                 }
             }
         }
