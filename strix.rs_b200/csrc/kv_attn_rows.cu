@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         const uint32_t tid = threadIdx.x & 127u, tr = tid & 63u, th = tid >> 6;  // token of the tile, half of its dimensions
         bool bad = empty_rows<HD, RA_TT>(A, RA_ROWS, warp - 12u, 4u);
         report_bad(V, bad && lane == 0);
-        uint32_t items = 0, pos_hi = 0;
+        uint32_t items = 0, pos_hi = 0, land = 0, land_phase = 0, st = 0, st_phase = 0;
         auto arrive = [&](uint64_t *bar) {
             fence_proxy_async_smem();
             __syncwarp();
@@ -384,7 +384,6 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         };
 #pragma unroll 1
         for (uint32_t n = 0; n < n_tiles; n++) {
-            const uint32_t land = n % NL, land_phase = (n / NL) & 1u, st = n % NS, st_phase = (n / NS) & 1u;
             wait(&land_full[land], land_phase);
             const PaTile &d = desc[n % RA_DESCS];
             if (d.flags & PA_NEW) {
@@ -430,16 +429,24 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 if constexpr (EL == 1) {
                     wait(&op_empty[kv * NS + st], st_phase ^ 1u);
                     const uint8_t *src = raw + (size_t)(kv * NL + land) * S::RAWB + tr * HD;
-#pragma unroll 2
+                    uint4 x[HD / 32];
+#pragma unroll
                     for (int j = 0; j < HD / 32; j++) {
                         const uint32_t c = th * (HD / 32) + j;  // sixteen codes
-                        uint4 x = *reinterpret_cast<const uint4 *>(src + ((S::RAWSWZ ? c ^ (tr & 7u) : c) << 4));
-                        if (kv && !keep) x = make_uint4(0u, 0u, 0u, 0u);
+                        x[j] = *reinterpret_cast<const uint4 *>(src + ((S::RAWSWZ ? c ^ (tr & 7u) : c) << 4));
+                    }
+                    if (kv && !keep) {
+#pragma unroll
+                        for (int j = 0; j < HD / 32; j++) x[j] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                    for (int j = 0; j < HD / 32; j++) {
+                        const uint32_t c = th * (HD / 32) + j;
                         uint4 y, z;
-                        e4m3x4_to_f16x2(x.x, y.x, y.y);
-                        e4m3x4_to_f16x2(x.y, y.z, y.w);
-                        e4m3x4_to_f16x2(x.z, z.x, z.y);
-                        e4m3x4_to_f16x2(x.w, z.z, z.w);
+                        e4m3x4_to_f16x2(x[j].x, y.x, y.y);
+                        e4m3x4_to_f16x2(x[j].y, y.z, y.w);
+                        e4m3x4_to_f16x2(x[j].z, z.x, z.y);
+                        e4m3x4_to_f16x2(x[j].w, z.z, z.w);
                         uint8_t *row = dst + (c / 4u) * 8192u + tr * 128u;
                         const uint32_t w = (2u * c) & 7u;
                         *reinterpret_cast<uint4 *>(row + ((w ^ (tr & 7u)) << 4)) = y;
@@ -457,6 +464,14 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     }
                     arrive(&op_full[kv * NS + st]);
                 }
+            }
+            if (++land == NL) {
+                land = 0;
+                land_phase ^= 1u;
+            }
+            if (++st == NS) {
+                st = 0;
+                st_phase ^= 1u;
             }
         }
         join();
