@@ -228,13 +228,14 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 for (uint32_t j = 0; j < n_sub; j++)
                     if (!((valid >> j) & 1u)) sees &= ~((~0ull >> (64u - sub)) << (j * sub));
             }
-            auto masked16 = [&](uint32_t *s, uint32_t c) {  // the sums of sixteen tokens, which are of one page
+            auto sums32 = [&](uint32_t *s, uint32_t c) {  // the sums of 32 tokens: sixteen are of one page
                 tc_ld16(t_row + b * 64u + c, s);
-                const uint32_t bits = (uint32_t)(sees >> c) & 0xffffu;
+                tc_ld16(t_row + b * 64u + c + 16u, s + 16);
+                const uint32_t bits = (uint32_t)(sees >> c);
                 tc_wait_ld();
-                if (__any_sync(0xffffffffu, bits != 0xffffu)) {
+                if (__any_sync(0xffffffffu, bits != ~0u)) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) s[i] = (bits >> i) & 1u ? s[i] : 0xff800000u;
+                    for (int i = 0; i < 32; i++) s[i] = (bits >> i) & 1u ? s[i] : 0xff800000u;
                 }
             };
             // the factor to exponents of two is positive (the sign of the caller's scale went into q), so the largest product is the
@@ -242,35 +243,42 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             auto factor = [&](uint32_t c) { return fmaxf(d.ks[mixed ? c >> pshift : 0u] * f_q, 1.0e-30f); };
             float top = -INFINITY;
 #pragma unroll 1
-            for (uint32_t c = 0; c < RA_TT; c += 16u) {
-                uint32_t s[16];
-                masked16(s, c);
-                float t0 = __uint_as_float(s[0]), t1 = __uint_as_float(s[1]);
+            for (uint32_t c = 0; c < RA_TT; c += 32u) {
+                uint32_t s[32];
+                sums32(s, c);
 #pragma unroll
-                for (int i = 2; i < 16; i += 2) {
-                    t0 = fmaxf(t0, __uint_as_float(s[i]));
-                    t1 = fmaxf(t1, __uint_as_float(s[i + 1]));
+                for (int h = 0; h < 32; h += 16) {
+                    float t0 = __uint_as_float(s[h]), t1 = __uint_as_float(s[h + 1]);
+#pragma unroll
+                    for (int i = h + 2; i < h + 16; i += 2) {
+                        t0 = fmaxf(t0, __uint_as_float(s[i]));
+                        t1 = fmaxf(t1, __uint_as_float(s[i + 1]));
+                    }
+                    top = fmaxf(top, fmaxf(t0, t1) * factor(c + h));
                 }
-                top = fmaxf(top, fmaxf(t0, t1) * factor(c));
             }
             const float base = top == -INFINITY ? 0.f : 15.f - top;
             if (n >= 2u) wait(&o_full[b], ((n >> 1) & 1u) ^ 1u);  // the product of tile n - 2, which read this buffer of P
             tc_fence_after();
             float l0 = 0.f, l1 = 0.f;
 #pragma unroll 1
-            for (uint32_t c = 0; c < RA_TT; c += 16u) {
-                uint32_t s[16], hi[8], lo[8];
-                const float f = factor(c), w = mixed ? d.vs[c >> pshift] * rvref : 1.f;
-                masked16(s, c);
+            for (uint32_t c = 0; c < RA_TT; c += 32u) {
+                uint32_t s[32];
+                sums32(s, c);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float p0 = ex2(fmaf(__uint_as_float(s[i]), f, base)), p1 = ex2(fmaf(__uint_as_float(s[i + 1]), f, base));
-                    l0 += p0;
-                    l1 += p1;
-                    split2(p0 * w, p1 * w, hi[i / 2], lo[i / 2]);
+                for (int h = 0; h < 32; h += 16) {
+                    uint32_t hi[8], lo[8];
+                    const float f = factor(c + h), w = mixed ? d.vs[(c + h) >> pshift] * rvref : 1.f;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float p0 = ex2(fmaf(__uint_as_float(s[h + i]), f, base)), p1 = ex2(fmaf(__uint_as_float(s[h + i + 1]), f, base));
+                        l0 += p0;
+                        l1 += p1;
+                        split2(p0 * w, p1 * w, hi[i / 2], lo[i / 2]);
+                    }
+                    tc_st8(t_row + S::COL_P + b * 64u + (c + h) / 2u, hi);
+                    tc_st8(t_row + S::COL_P + b * 64u + 32u + (c + h) / 2u, lo);
                 }
-                tc_st8(t_row + S::COL_P + b * 64u + c / 2u, hi);
-                tc_st8(t_row + S::COL_P + b * 64u + 32u + c / 2u, lo);
             }
             tile_m[(n % RA_STATS) * 128u + row] = top;
             tile_l[(n % RA_STATS) * 128u + row] = l0 + l1;
