@@ -93,7 +93,7 @@ STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_p
 /* out[row][head] = softmax(scale * q k^T) v over the cached tokens the row sees: positions 0 .. its own (its own k and v
  * are in the cache by then), with window > 0 only the last `window` of them. n_heads is a multiple of n_kv; head h reads KV
  * head h / (n_heads / n_kv). q and out: [n_rows][n_heads * head_dim] f32, ld_q / ld_out floats between rows (0 = packed).
- * A row that sees no token gets zeros. Products and sums keep f32 accuracy (f16 tensor-core products of q and of the
+ * A row that sees no token gets zeros. At most 8192 sequences in one call. Products and sums keep f32 accuracy (f16 tensor-core products of q and of the
  * probabilities in two halves of 11 bits each).
  * d_work: work_bytes >= strix_cuda_attn_pages_workspace, 256-byte aligned, zeroed once before its first use; every
  * call leaves it ready for the next (of any sizes that fit). Calls that share a workspace must not run at the same time; graphs
@@ -118,7 +118,8 @@ typedef struct strix_sample_params {
  *   d_ids[row] = the least i whose kept weights up to and including i exceed d_u[row] * (sum of kept weights), d_u in [0, 1)
  * Equal logits rank by index, lower first; NaN counts as -inf; with +inf among the logits only those have weight.
  * A row without any logit above -inf gives id 0 and probability 0. d_probs (may be NULL): the drawn token's weight over the kept
- * sum. Sums run in 64-bit integers (weights in steps of 2^-40), so the draw does not depend on their order.
+ * sum. Weights are summed as 64-bit integers (in steps of 2^-40; the sum of a whole row in f32 over stretches of fixed
+ * order), so the same logits and the same u draw the same token every time.
  * The greedy choice is that of strix_cuda_argmax_dev except below its floor of -3.0e38. */
 #define STRIX_SAMPLE_MAX_N 393216
 STRIX_API int strix_cuda_sample_dev(strix_cuda *h, const float *d_x, size_t n, size_t stride, size_t rows, const strix_sample_params *params,

@@ -10,10 +10,19 @@
 // The running O is kept in registers, a row to a thread: sums over tiles then round to nearest (chained accumulation in the tensor
 // cores truncates), and a new maximum costs no pass over TMEM.
 //
-// Roles of the 12 warps: 0-3 softmax (232 registers: O), 4-7 make operands (q split, e4m3 to f16, rows of v that nobody sees
-// to zero), 8 copies by TMA, 9 issues the products. S, P and O are double-buffered in TMEM: while the softmax of tile n runs, the
-// tensor cores work on S of tile n + 1 and O of tile n - 1. What bounds it: 4 x 128 x 64 x head size multiply-adds a tile on the
-// tensor cores (1024 clocks at head size 128), and the softmax's instructions next to them (about 700 a warp and tile).
+// Roles of the 20 warps (96 registers each at launch, shared out anew: the sums get 176, the last eight warps 56):
+//   0-3, 4-7  softmax of the even and of the odd tiles. A tile's weights are relative to its own largest score, so these warps
+//             carry nothing from tile to tile: they leave the tile's maximum and sum of weights in shared memory, and
+//   8-11      the sums bring the tiles' products O to the running maximum as they add them, and write the finished rows
+//   12-15     make operands: q split, e4m3 to f16, rows of v that nobody sees to zero
+//   16        copies by TMA;   17, 18  issue the products S and O
+// S, P and O are double-buffered in TMEM. At the end warps 0-15 join the parts of items that other blocks share.
+//
+// What bounds it: the products are 1024 clocks of a tile at head size 128 (S reads both operands from shared memory, 96 bytes of
+// them for each of 64 columns). Measured are about 3300: exponentials, splits and the passes over TMEM take the softmax warps 2500 a
+// tile, at 51 % of the issue slots. Loops over tiles and columns stay rolled, because instruction fetch bounded the unrolled
+// form (135 KB, all roles at once: 460 us, 320 once rolled). 512 rows behind 8000 tokens (32 heads, 8 KV heads of 128, e4m3):
+// 219 us, 316 TFLOP/s of useful products, as many again for the second halves; 8 x 5 rows behind 1000-5000 tokens, f16: 57 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
