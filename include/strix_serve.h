@@ -92,7 +92,8 @@ STRIX_API int strix_cuda_kv_append_dev(strix_cuda *h, const strix_kv_pages *cach
 STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_pages *cache, const strix_kv_batch *batch, uint32_t n_heads);
 /* out[row][head] = softmax(scale * q k^T) v over the cached tokens the row sees: positions 0 .. its own (its own k and v
  * are in the cache by then), with window > 0 only the last `window` of them. n_heads is a multiple of n_kv; head h reads KV
- * head h / (n_heads / n_kv). q and out: [n_rows][n_heads * head_dim] f32, ld_q / ld_out floats between rows (0 = packed).
+ * head h / (n_heads / n_kv). q and out: [n_rows][n_heads * head_dim] f32, ld_q / ld_out floats between rows (0 = packed), which
+ * must not overlap. With a window, pages that end before all rows' windows are not looked at: they may be given away.
  * A row that sees no token gets zeros. At most 8192 sequences in one call. Products and sums keep f32 accuracy (f16 tensor-core products of q and of the
  * probabilities in two halves of 11 bits each).
  * d_work: work_bytes >= strix_cuda_attn_pages_workspace, 256-byte aligned, zeroed once before its first use; every

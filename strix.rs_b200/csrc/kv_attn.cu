@@ -233,7 +233,8 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         const uint32_t tok = (place.lo_tile + place.at) * TT + lane * sub, nth = tok >> V.page_shift;
         b_page = -1;
         b_ks = b_vs = 0.f;
-        if (lane < n << sub_shift && tok <= place.ctx + (place.rows - 1u) && nth < V.pages_ld) {
+        if (lane < n << sub_shift && tok <= place.ctx + (place.rows - 1u) && nth < V.pages_ld &&
+            tok + sub > first_seen(A, rb, place.ctx, place.mb)) {
             b_page = V.pages[(size_t)place.s * V.pages_ld + nth];
             if (b_page < 0 || (uint32_t)b_page >= V.n_pages) {
                 b_page = -1;
@@ -840,11 +841,12 @@ static int attn_form(const PagedView &V, uint32_t group, uint32_t &wm) {
     return FORM_WIDE;
 }
 
+static uint32_t form_rows(int form, uint32_t wm) { return form == FORM_ROWS ? 128u : form == FORM_WIDE ? 16u * wm : 8u; }  // of a block
+
 static size_t attn_work_bytes(const strix_cuda *h, const PagedView &V, uint32_t group) {
     uint32_t wm;
     const int form = attn_form(V, group, wm);
-    const size_t rb = form == FORM_ROWS ? 128u : form == FORM_WIDE ? 16u * wm : 8u;
-    const size_t part = (size_t)attn_blocks(h) * 2 * rb * (V.head_dim + 2) * 4;
+    const size_t part = (size_t)attn_blocks(h) * 2 * form_rows(form, wm) * (V.head_dim + 2) * 4;
     return (PA_MAX_BLOCKS * 4 + part + 255) & ~(size_t)255;
 }
 
@@ -906,7 +908,10 @@ static int attn_check(strix_cuda *h, const char *who, const strix_kv_pages *cach
     if (n_heads == 0 || n_heads > 65535u || n_heads % V.n_kv) return 0;
     if (V.n_seq > PA_MAX_SEQ) return serve_fail(h, who, "at most 8192 sequences in one call");
     // the line of tiles is counted in 31 bits
-    const uint64_t rb = 8, group = n_heads / V.n_kv;
+    const uint64_t group = n_heads / V.n_kv;
+    uint32_t wm;
+    const int form = attn_form(V, (uint32_t)group, wm);
+    const uint64_t rb = form_rows(form, wm);
     const uint64_t blocks = ((uint64_t)V.n_rows * group + rb - 1) / rb + V.n_seq, tiles = (uint64_t)V.pages_ld * V.page_tokens / 16 + 1;
     if ((uint64_t)V.n_rows * group > 0x7fffffffull || blocks * V.n_kv > 0x7fffffffull || blocks * V.n_kv * tiles > 0x7fffffffull)
         return serve_fail(h, who, "batch too large for one call");
@@ -938,6 +943,7 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     if (A.ld_q < qd || A.ld_out < qd) return serve_fail(h, who, "a row stride is smaller than a row");
     if (A.V.n_seq == 0 || A.V.n_rows == 0) return 1;
     if (!d_q || !d_out) return serve_fail(h, who, "d_q or d_out missing");
+    if (d_q == d_out) return serve_fail(h, who, "d_out must not be d_q: rows are read by several blocks");
     if (!d_work || (reinterpret_cast<uintptr_t>(d_work) & 255u)) return serve_fail(h, who, "d_work must be 256-byte aligned");
     A.group = n_heads / A.V.n_kv;
     while ((1u << A.g_shift) < A.group) A.g_shift++;

@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     const uint32_t tok = (place.lo_tile + place.at) * RA_TT + lane * sub, nth = tok >> pshift;
                     b_page = -1;
                     b_ks = b_vs = 0.f;
-                    if (lane < cnt * n_sub && tok <= place.ctx + (place.rows - 1u) && nth < V.pages_ld) {
+                    if (lane < cnt * n_sub && tok <= place.ctx + (place.rows - 1u) && nth < V.pages_ld &&
+                        tok + sub > first_seen(A, RA_ROWS, place.ctx, place.mb)) {
                         b_page = V.pages[(size_t)place.s * V.pages_ld + nth];
                         if (b_page < 0 || (uint32_t)b_page >= V.n_pages) {
                             b_page = -1;

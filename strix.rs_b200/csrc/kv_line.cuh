@@ -78,6 +78,12 @@ __device__ __forceinline__ uint32_t block_tiles(const PagedAttnArgs &A, uint32_t
     return hi > lo ? (hi + TT - 1u) / TT - lo_tile : 0u;
 }
 
+// The first position that any row of the block sees: pages that end before it may be anybody's by now.
+__device__ __forceinline__ uint32_t first_seen(const PagedAttnArgs &A, uint32_t rb, uint32_t ctx, uint32_t mb) {
+    const uint32_t p0 = ctx + by_group(A, mb * rb);
+    return A.window && p0 >= A.window ? p0 + 1u - A.window : 0u;
+}
+
 // A place in the line of tiles.
 struct __align__(16) PaPlace {
     uint32_t s, first, rows, ctx, mb, head, lo_tile, tiles, at;  // item: tiles of it, `at` the place within

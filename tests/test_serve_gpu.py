@@ -470,6 +470,30 @@ def test_attention_row_blocks_nan_query_and_bad_pages(torch, pkg, accel):
         check_attention(torch, accel, P, b, row0, ctx, 4, q, out, 0.125, 0, hole=hole)
 
 
+@pytest.mark.parametrize("new,group", [(1, 4), (3, 4), (3, 5), (9, 4)])
+@pytest.mark.parametrize("kv,page,hd", [(0, 16, 64), (1, 32, 128), (1, 16, 256)])
+def test_attention_window_looks_at_no_page_before_it(torch, pkg, accel, kv, page, hd, new, group):
+    """Pages that ended before the first row's window have been given away: their entries are no pages any more."""
+    window, ctx = 20, [150, 83, 4 * page + 19]
+    row0 = [0, new, 2 * new, 3 * new]
+    P = Paged(torch, pkg, kv, 1, page, hd, [c + new for c in ctx], fill=0xff)
+    P.seed_random(3, [c + new for c in ctx])
+    b = P.batch(row0, ctx)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(3 * new, group * hd, generator=g, device="cuda")
+    out = torch.zeros_like(q)
+    w = work_of(torch, accel, P, b, group)
+    full = P.table.copy()
+    for s, c in enumerate(ctx):
+        P.table[s, :(c + 1 - window) // page] = -1
+    P.d_table.copy_(torch.from_numpy(P.table))
+    assert accel.attn_pages_dev(P.desc, b, group, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), window=window, stream=stream(torch))
+    torch.cuda.synchronize()
+    assert accel.device_status() == 0
+    P.table[:] = full
+    check_attention(torch, accel, P, b, row0, ctx, group, q, out, 0.125, window)
+
+
 def test_attention_graph_serves_changing_lengths(torch, pkg, accel):
     """One captured graph, replayed on a stream of its own with other lengths, rows and pages each time; a workspace that larger and
     smaller calls share."""
@@ -506,9 +530,10 @@ def test_serving_calls_refuse(torch, pkg, accel):
     x = torch.zeros(4, 512, device="cuda")
     b, p = P.batch([0, 1], [0]), x.data_ptr()
     w = work_of(torch, accel, P, b, 4)
-    attn = lambda **k: accel.attn_pages_dev(P.desc, k.get("b", b), k.get("heads", 4), k.get("q", p), p, 1.0, k.get("w", w.data_ptr()),  # noqa: E731
+    other = torch.zeros_like(x)
+    attn = lambda **k: accel.attn_pages_dev(P.desc, k.get("b", b), k.get("heads", 4), k.get("q", p), k.get("o", other.data_ptr()), 1.0, k.get("w", w.data_ptr()),  # noqa: E731
                                             k.get("n", w.numel()), ld_q=k.get("ld", 0))
-    for kw in (dict(q=0), dict(w=0), dict(w=w.data_ptr() + 16), dict(n=w.numel() - 1), dict(ld=255)):
+    for kw in (dict(q=0), dict(w=0), dict(w=w.data_ptr() + 16), dict(n=w.numel() - 1), dict(ld=255), dict(o=0), dict(o=p)):
         with pytest.raises(pkg.StrixCudaError):
             attn(**kw)
     assert attn(heads=3) is False and attn(heads=0) is False
