@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         b_page = -1;
         b_ks = b_vs = 0.f;
         if (lane < n << sub_shift && tok <= place.ctx + (place.rows - 1u) && nth < V.pages_ld &&
-            tok + sub > first_seen(A, rb, place.ctx, place.mb)) {
+            still_seen(A, rb, place.ctx, place.mb, tok + sub - 1u)) {
             b_page = V.pages[(size_t)place.s * V.pages_ld + nth];
             if (b_page < 0 || (uint32_t)b_page >= V.n_pages) {
                 b_page = -1;

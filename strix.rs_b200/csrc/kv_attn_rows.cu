@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     b_page = -1;
                     b_ks = b_vs = 0.f;
                     if (lane < cnt * n_sub && tok <= place.ctx + (place.rows - 1u) && nth < V.pages_ld &&
-                        tok + sub > first_seen(A, RA_ROWS, place.ctx, place.mb)) {
+                        still_seen(A, RA_ROWS, place.ctx, place.mb, tok + sub - 1u)) {
                         b_page = V.pages[(size_t)place.s * V.pages_ld + nth];
                         if (b_page < 0 || (uint32_t)b_page >= V.n_pages) {
                             b_page = -1;
@@ -671,6 +671,10 @@ static cudaError_t rows_launch(const strix_cuda *h, PagedAttnArgs &A, uint32_t b
     static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic shared memory is raised for this kernel
     const uint64_t bit = 1ull << (h->device & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        cudaFuncAttributes fa;
+        const cudaError_t f = cudaFuncGetAttributes(&fa, attn_rows_kernel<HD, TYPE>);
+        if (f != cudaSuccess) return f;
+        if (fa.numRegs < 96) return cudaErrorInvalidConfiguration;  // the warps' shares (2 x 96, 176, 2 x 56) add up to five times that
         const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<HD, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
         if (e != cudaSuccess) return e;
         ready.fetch_or(bit, std::memory_order_relaxed);

@@ -78,10 +78,11 @@ __device__ __forceinline__ uint32_t block_tiles(const PagedAttnArgs &A, uint32_t
     return hi > lo ? (hi + TT - 1u) / TT - lo_tile : 0u;
 }
 
-// The first position that any row of the block sees: pages that end before it may be anybody's by now.
-__device__ __forceinline__ uint32_t first_seen(const PagedAttnArgs &A, uint32_t rb, uint32_t ctx, uint32_t mb) {
+// Does any row of the block see position `last` or a later one? Pages that end before that may be anybody's by now.
+__device__ __forceinline__ bool still_seen(const PagedAttnArgs &A, uint32_t rb, uint32_t ctx, uint32_t mb, uint32_t last) {
+    if (!A.window) return true;
     const uint32_t p0 = ctx + by_group(A, mb * rb);
-    return A.window && p0 >= A.window ? p0 + 1u - A.window : 0u;
+    return p0 < A.window || last > p0 - A.window;
 }
 
 // A place in the line of tiles.
@@ -199,33 +200,45 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs &A, uint32_t rb, ui
     constexpr int PS = HD + 2, DL = (HD / 2 + 31) / 32;  // DL: pairs of a row in a lane
     const uint32_t lane = threadIdx.x & 31u;
     auto part = [&](uint32_t i) { return A.part + (((size_t)(lo + i) * 2u + (i == 0u ? 1u : 0u)) * rb + row) * PS; };
-    float M = -INFINITY, L = 0.f;
+    constexpr int AHEAD = 4;  // parts on their way at once, from before their weights are known: a join is a chain of loads
+    float2 v[AHEAD][DL];
+    auto fetch = [&](uint32_t i0) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const float2 *src = reinterpret_cast<const float2 *>(part(i0 + j));
+#pragma unroll
+            for (int k = 0; k < DL; k++) v[j][k] = i0 + j < n && k * 32 + lane < HD / 2 ? __ldcg(src + k * 32 + lane) : make_float2(0.f, 0.f);
+        }
+    };
+    float2 ml = lane < n ? __ldcg(reinterpret_cast<const float2 *>(part(lane) + HD)) : make_float2(-INFINITY, 0.f);
+    fetch(0u);
+    float M = ml.x, L = 0.f;
 #pragma unroll 1
-    for (uint32_t i = lane; i < n; i += 32u) M = fmaxf(M, __ldcg(part(i) + HD));
+    for (uint32_t i = lane + 32u; i < n; i += 32u) M = fmaxf(M, __ldcg(part(i) + HD));
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
     float2 acc[DL];
 #pragma unroll
     for (int k = 0; k < DL; k++) acc[k] = make_float2(0.f, 0.f);
+    float f = 0.f;
 #pragma unroll 1
-    for (uint32_t base = 0; base < n; base += 32u) {
-        const uint32_t cnt = min(32u, n - base);
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < cnt) ml = __ldcg(reinterpret_cast<const float2 *>(part(base + lane) + HD));
-        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-        L += f * ml.y;
-#pragma unroll 8
-        for (uint32_t i = 0; i < cnt; i++) {
-            const float fw = __shfl_sync(0xffffffffu, f, i);
-            const float2 *src = reinterpret_cast<const float2 *>(part(base + i));
-#pragma unroll
-            for (int k = 0; k < DL; k++)
-                if (k * 32 + lane < HD / 2) {
-                    const float2 v = __ldcg(src + k * 32 + lane);
-                    acc[k].x = fmaf(fw, v.x, acc[k].x);
-                    acc[k].y = fmaf(fw, v.y, acc[k].y);
-                }
+    for (uint32_t i = 0; i < n; i += AHEAD) {
+        if ((i & 31u) == 0u) {  // the weights of the next 32 parts, one to a lane
+            if (i) ml = lane + i < n ? __ldcg(reinterpret_cast<const float2 *>(part(lane + i) + HD)) : make_float2(-INFINITY, 0.f);
+            f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+            L += f * ml.y;
         }
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const float fw = __shfl_sync(0xffffffffu, f, (i + j) & 31u);
+            if (i + j >= n) continue;  // (nothing of a part that is none, whatever the weight in its lane)
+#pragma unroll
+            for (int k = 0; k < DL; k++) {
+                acc[k].x = fmaf(fw, v[j][k].x, acc[k].x);
+                acc[k].y = fmaf(fw, v[j][k].y, acc[k].y);
+            }
+        }
+        if (i + AHEAD < n) fetch(i + AHEAD);
     }
     L = warp_sum(L);
     const float inv = L == 0.f ? 0.f : 1.0f / L;
