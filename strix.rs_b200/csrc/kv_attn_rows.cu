@@ -97,6 +97,22 @@ __device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t *r) {
 }
 #undef STRIX_R8
 #undef STRIX_W8
+// two f32 multiply-adds, or additions, in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -269,7 +285,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             const float base = top == -INFINITY ? 0.f : 15.f - top;
             if (n >= 2u) wait(&o_full[b], ((n >> 1) & 1u) ^ 1u);  // the product of tile n - 2, which read this buffer of P
             tc_fence_after();
-            float l0 = 0.f, l1 = 0.f;
+            float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll 1
             for (uint32_t c = 0; c < RA_TT; c += 32u) {
                 uint32_t s[32];
@@ -277,20 +293,31 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
 #pragma unroll
                 for (int h = 0; h < 32; h += 16) {
                     uint32_t hi[8], lo[8];
-                    const float f = factor(c + h), w = mixed ? d.vs[(c + h) >> pshift] * rvref : 1.f;
+                    const float f = factor(c + h);
+                    float2 p[8];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float p0 = ex2(fmaf(__uint_as_float(s[h + i]), f, base)), p1 = ex2(fmaf(__uint_as_float(s[h + i + 1]), f, base));
-                        l0 += p0;
-                        l1 += p1;
-                        split2(p0 * w, p1 * w, hi[i / 2], lo[i / 2]);
+                    for (int i = 0; i < 8; i++) {
+                        const float2 y = fma2(make_float2(__uint_as_float(s[h + 2 * i]), __uint_as_float(s[h + 2 * i + 1])), make_float2(f, f), make_float2(base, base));
+                        p[i] = make_float2(ex2(y.x), ex2(y.y));
+                        l2 = add2(l2, p[i]);
+                    }
+                    if (mixed) {
+                        const float w = d.vs[(c + h) >> pshift] * rvref;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) p[i] = make_float2(p[i].x * w, p[i].y * w);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        hi[i] = f32_to_f16x2(p[i].x, p[i].y);
+                        const float2 left = fma2(__half22float2(*reinterpret_cast<const __half2 *>(&hi[i])), make_float2(-1.f, -1.f), p[i]);
+                        lo[i] = f32_to_f16x2(left.x, left.y);
                     }
                     tc_st8(t_row + S::COL_P + b * 64u + (c + h) / 2u, hi);
                     tc_st8(t_row + S::COL_P + b * 64u + 32u + (c + h) / 2u, lo);
                 }
             }
             tile_m[(n % RA_STATS) * 128u + row] = top;
-            tile_l[(n % RA_STATS) * 128u + row] = l0 + l1;
+            tile_l[(n % RA_STATS) * 128u + row] = l2.x + l2.y;
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -343,7 +370,11 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 tc_ld32(t_row + S::COL_O + b * HD + c * 32, r);
                 tc_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; i++) o[c * 32 + i] = fmaf(__uint_as_float(r[i]), w, o[c * 32 + i]);
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(w, w), make_float2(o[c * 32 + i], o[c * 32 + i + 1]));
+                    o[c * 32 + i] = x.x;
+                    o[c * 32 + i + 1] = x.y;
+                }
             }
             tc_fence_before();
             __syncwarp();
