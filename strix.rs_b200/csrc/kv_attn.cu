@@ -25,8 +25,8 @@
 // the last block to arrive joins the parts, in the order of the line. Cuts that would fall into an item of at most PA_SNAP
 // tiles move to its nearer end.
 //
-// Measured (32 heads, 8 KV heads of 128, e4m3): one row behind 131071 tokens 75 us (3.6 TB/s), 61 rows behind 500-16384 each
-// 138 us (4.2 TB/s), one row behind 300 tokens 12.5 us. About 8 us of a call are its two ends (the place in the line, page ids and
+// Measured (32 heads, 8 KV heads of 128, e4m3): one row behind 131071 tokens 72 us (3.7 TB/s), 61 rows behind 500-16384 each
+// 138 us (4.2 TB/s), one row behind 300 tokens 12.7 us. About 8 us of a call are its two ends (the place in the line, page ids and
 // scales, q; the joins); in between, instruction issue bounds: some 1000 instructions a tile, of which the fragments of k and v,
 // their conversion and the two halves' products are two thirds.
 #include <cuda_runtime.h>
@@ -817,11 +817,12 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     }
 }
 
-// Above this many rows a head on average, blocks of 128 rows on tcgen05. Both forms measured (8 KV heads of 128, page 64; us):
-//   12 rows,  8 sequences of 3000 tokens: 58 with blocks, 47 without;  64 of 4000: 373 and 266
-//   16 rows, 32 of 8000: 362 and 264;  1 of 30000: 71 and 57
-//   20 rows,  8 of 3000: 63 and 75 (e4m3 61 and 67);  32 rows, 8 of 3000: 69 and 80;  32 of 8000: 375 and 555
-//   64 rows,  8 of 3000: 85 and 144;  32 of 8000: 395 and 1087
+// Above this many rows a head on average, blocks of 128 rows on tcgen05 (kv_attn_rows.cu). Both forms measured, 8 KV heads of 128,
+// 64-token pages, us with such blocks and without, f16 and e4m3:
+//   12 rows, 64 sequences of 4000 tokens: 301 and 263, 328 and 217
+//   16 rows,  8 of 3000:  51 and  44,  54 and  41;  32 of 8000: 290 and  262, 312 and 214;  1 of 30000: 62 and 54, 64 and 50
+//   20 rows,  8 of 3000:  54 and  72,  57 and  61;  32 of 8000: 295 and  548, 317 and 423;  1 of 30000: 67 and 92, 71 and 77
+//   64 rows,  8 of 3000:  71 and 131,  67 and 109;  32 of 8000: 314 and 1077, 332 and 816
 constexpr uint64_t ROWS_FROM = 16;
 
 // Blocks that the launch may have: one on each SM.

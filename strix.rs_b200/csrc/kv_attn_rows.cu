@@ -19,10 +19,11 @@
 // S, P and O are double-buffered in TMEM. At the end warps 0-15 join the parts of items that other blocks share.
 //
 // What bounds it: the products are 1024 clocks of a tile at head size 128 (S reads both operands from shared memory, 96 bytes of
-// them for each of 64 columns). Measured are about 3300: exponentials, splits and the passes over TMEM take the softmax warps 2500 a
-// tile, at 51 % of the issue slots. Loops over tiles and columns stay rolled, because instruction fetch bounded the unrolled
-// form (135 KB, all roles at once: 460 us, 320 once rolled). 512 rows behind 8000 tokens (32 heads, 8 KV heads of 128, e4m3):
-// 219 us, 316 TFLOP/s of useful products, as many again for the second halves; 8 x 5 rows behind 1000-5000 tokens, f16: 57 us.
+// them for each of 64 columns). Measured are about 3000: exponentials, splits and the passes over TMEM take the softmax warps most
+// of that, at half of the issue slots. Loops over tiles stay rolled, because instruction fetch bounded the unrolled form (135 KB,
+// all roles at once: 460 us, 320 once rolled, in earlier forms). S held in registers, so that its columns are free sooner, was
+// no faster (201 against 197 us). 512 rows behind 8000 tokens (32 heads, 8 KV heads of 128, e4m3): 197 us, 352 TFLOP/s
+// of useful products, as many again for the second halves; 8 x 5 rows behind 1000-5000 tokens, f16: 55 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
