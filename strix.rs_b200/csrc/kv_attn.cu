@@ -952,7 +952,6 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     if (work_bytes < attn_work_bytes(h, A.V, A.group)) return serve_fail(h, who, "work_bytes too small");
     A.q = d_q;
     A.out = d_out;
-    A.n_heads = n_heads;
     A.window = window;
     A.cap = A.V.pages_ld * A.V.page_tokens;
     A.scale = scale;

@@ -20,7 +20,7 @@ struct PagedAttnArgs {
     const float *q;
     float *out;
     size_t ld_q, ld_out;
-    uint32_t n_heads, group, window, cap;  // cap: tokens a row of the page table can hold
+    uint32_t group, window, cap;  // cap: tokens a row of the page table can hold
     uint32_t g_mul, g_shift;               // division by group
     float scale;
     uint32_t wm, halves, vec;  // warps of a worker; half tiles of a ring; q and out rows start on 16 bytes
@@ -89,7 +89,6 @@ __device__ __forceinline__ bool still_seen(const PagedAttnArgs &A, uint32_t rb, 
 struct __align__(16) PaPlace {
     uint32_t s, first, rows, ctx, mb, head, lo_tile, tiles, at;  // item: tiles of it, `at` the place within
     uint32_t item0;                                              // the line's index of the item's first tile
-    uint32_t left, pad;                                          // tiles of the worker from here on
 };
 
 __device__ __forceinline__ void load_seq(const PagedAttnArgs &A, uint32_t s, PaPlace &P) {

@@ -524,6 +524,32 @@ def test_attention_graph_serves_changing_lengths(torch, pkg, accel):
             check_attention(torch, accel, P, b, row0, ctx, heads, q, out, 0.1, 0)
 
 
+def test_attention_on_two_streams_at_once(torch, pkg, accel):
+    """Calls that run at the same time, each with its own workspace, give what they give alone, bit by bit."""
+    jobs = []
+    for i, (new, ctx, group) in enumerate((([1, 1, 1], [900, 17, 3000], 4), ([40, 9], [700, 1500], 4))):
+        row0 = np.cumsum([0] + new).tolist()
+        P = Paged(torch, pkg, i, 2, 32, 128, [c + n for c, n in zip(ctx, new)], seed=i)
+        P.seed_random(i, [c + n for c, n in zip(ctx, new)])
+        b = P.batch(row0, ctx)
+        q = torch.randn(row0[-1], 2 * group * 128, device="cuda")
+        jobs.append((P, b, 2 * group, q, torch.zeros_like(q), work_of(torch, accel, P, b, 2 * group), torch.cuda.Stream()))
+    go = lambda P, b, heads, q, out, w, st: accel.attn_pages_dev(P.desc, b, heads, q.data_ptr(), out.data_ptr(), 0.09, w.data_ptr(), w.numel(),  # noqa: E731
+                                                                 stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    alone = []
+    for j in jobs:
+        assert go(*j)
+        torch.cuda.synchronize()
+        alone.append(j[4].clone())
+        j[4].zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        assert all(go(*j) for j in jobs)
+    torch.cuda.synchronize()
+    assert accel.device_status() == 0 and all(torch.equal(j[4], a) for j, a in zip(jobs, alone))
+
+
 def test_serving_calls_refuse(torch, pkg, accel):
     """Wrong arguments are errors with a message, other shapes are declined; nothing is launched."""
     P = Paged(torch, pkg, pkg.KV_F16, 2, 16, 64, [32])
