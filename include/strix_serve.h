@@ -94,8 +94,10 @@ STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_p
  * are in the cache by then), with window > 0 only the last `window` of them. n_heads is a multiple of n_kv; head h reads KV
  * head h / (n_heads / n_kv). q and out: [n_rows][n_heads * head_dim] f32, ld_q / ld_out floats between rows (0 = packed), which
  * must not overlap. With a window, pages that end before all rows' windows are not looked at: they may be given away.
- * A row that sees no token gets zeros. At most 8192 sequences in one call. Products and sums keep f32 accuracy (f16 tensor-core products of q and of the
- * probabilities in two halves of 11 bits each).
+ * A row that sees no token gets zeros. Offsets that give away more rows than n_rows (possible where they go down) set the status
+ * bit and leave out as it was. At most 8192 sequences in one call, and 2^31 tiles of 16 tokens in all blocks of rows when
+ * every sequence fills its row of d_pages (-1 beyond). Products and sums keep f32 accuracy (f16 tensor-core products of q and
+ * of the probabilities in two halves of 11 bits each).
  * d_work: work_bytes >= strix_cuda_attn_pages_workspace, 256-byte aligned, zeroed once before its first use; every
  * call leaves it ready for the next (of any sizes that fit). Calls that share a workspace must not run at the same time; graphs
  * replayed on different streams therefore need one each. The result does not depend on what else runs: partial sums

@@ -26,7 +26,7 @@
 // tiles move to its nearer end.
 //
 // Measured (32 heads, 8 KV heads of 128, e4m3): one row behind 131071 tokens 72 us (3.7 TB/s), 61 rows behind 500-16384 each
-// 138 us (4.2 TB/s), one row behind 300 tokens 12.7 us. About 8 us of a call are its two ends (the place in the line, page ids and
+// 138 us (4.2 TB/s), one row behind 300 tokens 13.2 us. About 8 us of a call are its two ends (the place in the line, page ids and
 // scales, q; the joins); in between, instruction issue bounds: some 1000 instructions a tile, of which the fragments of k and v,
 // their conversion and the two halves' products are two thirds.
 #include <cuda_runtime.h>
@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
 
     // ---- running tile counts of the sequences (where the rings will be)
     uint32_t *upto = reinterpret_cast<uint32_t *>(rings);
-    const uint32_t total = count_tiles<TT, NW * 32>(A, rb, upto, scan);
+    bool over;
+    const uint32_t total = count_tiles<TT, NW * 32>(A, rb, upto, scan, over);
 #pragma unroll 1
     for (uint32_t i = threadIdx.x; i < workers * halves; i += NW * 32) {
         mbar_init(&full[i], 1);
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         is_left--;
     };
 
-    bad |= empty_rows<HD, TT>(A, rb, warp, NW);
+    bad |= over || empty_rows<HD, TT>(A, rb, warp, NW);
 
     // ---- the loop over half tiles: k to weights, v to sums. The worker's first warp runs ahead by a ring.
     float o[NO][2 * RW], m[RW], l[RW];

@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
 
     uint32_t *upto = reinterpret_cast<uint32_t *>(op);
-    const uint32_t total = count_tiles<RA_TT, RA_THREADS>(A, RA_ROWS, upto, scan);
+    bool over;
+    const uint32_t total = count_tiles<RA_TT, RA_THREADS>(A, RA_ROWS, upto, scan, over);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * NL; i++) {
             mbar_init(&land_full[i], 1);
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         // ---- operands: q of a new item; every tile's k and v
         const uint32_t tid = threadIdx.x & 127u, tr = tid & 63u, th = tid >> 6;  // token of the tile, half of its dimensions
-        bool bad = empty_rows<HD, RA_TT>(A, RA_ROWS, warp - 12u, 4u);
+        const bool bad = over || empty_rows<HD, RA_TT>(A, RA_ROWS, warp - 12u, 4u);
         report_bad(V, bad && lane == 0);
         uint32_t items = 0, pos_hi = 0, land = 0, land_phase = 0, st = 0, st_phase = 0;
         auto arrive = [&](uint64_t *bar) {

@@ -284,10 +284,28 @@ __device__ __forceinline__ bool empty_rows(const PagedAttnArgs &A, uint32_t rb, 
     return bad;
 }
 
-// Running tile counts of the sequences, by all THREADS of a block; returns the total.
+// Running tile counts of the sequences, by all THREADS of a block; returns the total. Offsets that go down may give the same rows to
+// many sequences: where they give away more rows than there are, nothing is counted and `over` is set (the sizes that the
+// host has checked hold only up to there).
 template <int TT, int THREADS>
-__device__ __forceinline__ uint32_t count_tiles(const PagedAttnArgs &A, uint32_t rb, uint32_t *upto, uint32_t *scan) {
+__device__ __forceinline__ uint32_t count_tiles(const PagedAttnArgs &A, uint32_t rb, uint32_t *upto, uint32_t *scan, bool &over) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    bool down = false;
+#pragma unroll 1
+    for (uint32_t s = threadIdx.x; s < A.V.n_seq; s += THREADS) down |= A.V.row0[s + 1u] < A.V.row0[s];
+    over = false;
+    if (__syncthreads_or(down)) {
+        uint64_t rows = 0;
+#pragma unroll 1
+        for (uint32_t s = 0; s < A.V.n_seq; s++) {
+            uint32_t first, end;
+            bool bad = false;
+            seq_rows(A.V, s, first, end, bad);
+            rows += end - first;
+        }
+        over = rows > A.V.n_rows;
+        if (over) return 0u;
+    }
     uint32_t total = 0;
 #pragma unroll 1
     for (uint32_t c = 0; c < A.V.n_seq; c += THREADS) {

@@ -524,6 +524,28 @@ def test_attention_graph_serves_changing_lengths(torch, pkg, accel):
             check_attention(torch, accel, P, b, row0, ctx, heads, q, out, 0.1, 0)
 
 
+def test_attention_offsets_that_go_down(torch, pkg, accel):
+    """A sequence whose end lies before its start has no rows; offsets that give rows away twice leave everything as it was."""
+    for new in (2, 30):
+        P = Paged(torch, pkg, pkg.KV_F16, 1, 16, 64, [64] * 4)
+        P.seed_random(3, [64] * 4)
+        q = torch.randn(4 * new, 2 * 64, device="cuda")
+        out = torch.full_like(q, 5.0)
+        call = lambda b, w: accel.attn_pages_dev(P.desc, b, 2, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))  # noqa: E731
+        b = P.batch([0, 4 * new, 0, 4 * new, 0], [5, 6, -1, 7], 4 * new)       # sequences 0 and 2 both claim all rows
+        w = work_of(torch, accel, P, b, 2)
+        assert call(b, w)
+        torch.cuda.synchronize()
+        assert accel.device_status() & 2 and (out == 5.0).all()
+        accel.clear_device_status()
+        b = P.batch([0, new, new - 1, 2 * new - 1, 2 * new - 1], [5, 6, 7, 8], 4 * new)   # row new - 1 twice, sequence 1 none: not too many
+        assert call(b, w)
+        torch.cuda.synchronize()
+        assert accel.device_status() & 2 and (out[2 * new - 1:] == 5.0).all()
+        accel.clear_device_status()
+        check_attention(torch, accel, P, b, [0, new - 1], [5], 2, q, out, 0.125, 0)
+
+
 def test_attention_on_two_streams_at_once(torch, pkg, accel):
     """Calls that run at the same time, each with its own workspace, give what they give alone, bit by bit."""
     jobs = []
