@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
             if (n_mine) find_place<TT>(A, rb, upto, lo + w0, place);
         }
     }
+    fence_proxy_async_smem();  // copies land where the counts were: all accesses to them come first
     __syncthreads();
     uint8_t *ring = rings + (size_t)worker * halves * S::HALF;
     PaTile *desc = descs + worker * DESCS;

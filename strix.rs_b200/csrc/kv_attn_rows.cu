@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         n_tiles = __shfl_sync(0xffffffffu, x, 1) - lo;
         if (n_tiles) find_place<RA_TT>(A, RA_ROWS, upto, lo, place);
     }
+    fence_proxy_async_smem();  // f16 copies land where the counts were: all accesses to them come first
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

@@ -353,6 +353,35 @@ def test_attention_long_contexts_split_and_joined(torch, pkg, accel):
     run_attention(torch, pkg, accel, pkg.KV_F16, 2, 1, 16, 64, [3], [3001])
 
 
+def test_attention_most_sequences(torch, pkg, accel):
+    """8192 sequences, the most of a call: their running counts fill 32 KB of the memory that the first copies land in."""
+    n, page = 8192, 16
+    for kv, hd, group in ((pkg.KV_F16, 64, 2), (pkg.KV_F16, 64, 20), (pkg.KV_F16, 128, 20), (pkg.KV_E4M3, 128, 2), (pkg.KV_E4M3, 128, 20)):
+        g = torch.Generator(device="cuda").manual_seed(hd + group)
+        table = torch.randperm(n, generator=g, device="cuda").int()[:, None].contiguous()
+        ctx = torch.randint(0, page, (n,), generator=g, device="cuda").int()
+        row0 = torch.arange(n + 1, device="cuda").int()
+        x = [torch.randn(n, 1, page, hd, generator=g, device="cuda") for _ in "kv"]
+        k, v = (t.half() if kv == pkg.KV_F16 else t.to(torch.float8_e4m3fn) for t in x)
+        one = torch.ones(n, 1, device="cuda")
+        P = pkg.KvPages(k.data_ptr(), v.data_ptr(), n, 1, page, hd, type=kv, d_k_scale=one.data_ptr(), d_v_scale=one.data_ptr())
+        b = pkg.KvBatch(n, n, row0.data_ptr(), ctx.data_ptr(), table.data_ptr(), 1)
+        q = torch.randn(n, group, hd, generator=g, device="cuda")
+        out = torch.full_like(q, 5.0)
+        w = torch.zeros(accel.attn_pages_workspace(P, b, group), dtype=torch.uint8, device="cuda")
+        scale = hd ** -0.5
+        assert accel.attn_pages_dev(P, b, group, q.data_ptr(), out.data_ptr(), scale, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        assert accel.device_status() == 0
+        kk, vv = (t[table[:, 0].long(), 0].double() for t in (k, v))
+        s = torch.einsum("ngd,ntd->ngt", q.double(), kk) * scale
+        s = s.masked_fill((torch.arange(page, device="cuda")[None] > ctx[:, None])[:, None], -math.inf)
+        want = torch.softmax(s, -1) @ vv
+        # (the bound of check_attention, with the largest sum of magnitudes of all rows)
+        mag = float((torch.einsum("ngd,ntd->ngt", q.double().abs(), kk.abs()) * scale).max())
+        assert float((out - want).abs().max()) <= (2 * (hd + 8) * 2.0 ** -24 * mag + 2.0 ** -20) * float(vv.abs().max())
+
+
 def test_attention_extreme_scores(torch, pkg, accel):
     """Scores of thousands: one token has all the weight; and all scores equal."""
     run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 4, 16, 64, [1, 2], [90, 200], qs=500.0)
