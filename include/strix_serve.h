@@ -99,7 +99,8 @@ STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_p
  * every sequence fills its row of d_pages (-1 beyond). Products and sums keep f32 accuracy (f16 tensor-core products of q and
  * of the probabilities in two halves of 11 bits each).
  * d_work: work_bytes >= strix_cuda_attn_pages_workspace, 256-byte aligned, zeroed once before its first use; every
- * call leaves it ready for the next (of any sizes that fit). Calls that share a workspace must not run at the same time; graphs
+ * call leaves it ready for the next (of any sizes that fit), but for one whose bounded wait ran out (bit 0 of the status): out is
+ * unspecified then and d_work has to be zeroed again. Calls that share a workspace must not run at the same time; graphs
  * replayed on different streams therefore need one each. The result does not depend on what else runs: partial sums
  * are joined in a fixed order. */
 STRIX_API int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *cache, const strix_kv_batch *batch, uint32_t n_heads,

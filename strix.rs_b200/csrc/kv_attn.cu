@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     PaWorker *info = reinterpret_cast<PaWorker *>(descs + workers * DESCS);
     uint64_t *full = reinterpret_cast<uint64_t *>(info + workers), *empty = full + workers * halves;
     __shared__ uint32_t last_here[2], scan[NW];
+    __shared__ volatile uint32_t gave_up;
 
     // ---- running tile counts of the sequences (where the rings will be)
     uint32_t *upto = reinterpret_cast<uint32_t *>(rings);
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     }
 #pragma unroll 1
     for (uint32_t i = threadIdx.x; i < workers * DESCS * 4u; i += NW * 32) descs[i / 4u].ks[i & 3u] = descs[i / 4u].vs[i & 3u] = 0.f;
+    if (threadIdx.x == 0) gave_up = 0u;
     if (threadIdx.x < workers) info[threadIdx.x].has_head = info[threadIdx.x].head_ended = info[threadIdx.x].has_tail = 0u;
 
     // ---- this block's stretch of the line and this worker's part of it
@@ -307,6 +309,16 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     bool tail_tok = false;
     uint32_t it_first = 0, it_rows = 0, it_row0 = 0, it_head = 0;  // the item: first row of its sequence, new rows, first row of its own, KV head
     const int steps = (int)(2u * n_mine);
+    // by whole warps, whose lanes come to the same answer; a wait that has run out ends all others of the block
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+#pragma unroll 1
+        for (uint32_t it = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); it++)
+            if (__any_sync(0xffffffffu, gave_up || it >= 1u << 22)) {
+                gave_up = 1u;
+                return false;
+            }
+        return true;
+    };
 #pragma unroll 1
     for (int step = wi == 0 ? -(int)min(halves, 2u * n_mine) : 0; step < steps; step++) {
         if (step >= 0) {
@@ -316,7 +328,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
                 if (wi == 0)
 #pragma unroll 1
                     while (ds_left > is_left) describe();
-                if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
+                if (!wait(&full[half], phase)) break;
             }
             if (d.flags & PA_NEW) {
                 it_first = d.seq_first;
@@ -403,7 +415,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
             if (wm == 1u) {
 #pragma unroll 1
                 while (ds_left > is_left) describe();
-                if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
+                if (!wait(&full[half], phase)) break;
             }
             const uint8_t *ks = ring + half * S::HALF;
             const uint32_t tok = d.tile * TT, valid = d.valid;
@@ -555,7 +567,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
             if (wi == 0)
 #pragma unroll 1
                 while (ds_left > is_left) describe();
-            if (!mbar_wait_bounded(&full[half], phase, V.status)) break;
+            if (!wait(&full[half], phase)) break;
             const uint8_t *vs = ring + half * S::HALF;
             const uint32_t tok = d.tile * TT, valid = d.valid, pshift = V.page_shift;
             const bool mixed = TT > 16 && V.page_tokens < TT;
@@ -689,7 +701,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
         // refill: alone, a warp refills the half it has just used; with others, the one before, which they have mostly left as well
         if (wi == 0 && is_left && (step < 0 || wm == 1u || step > 0)) {
             if (step > 0 && wm > 1u) {
-                mbar_wait_bounded(&empty[e_half], e_phase, V.status);
+                if (!wait(&empty[e_half], e_phase)) break;  // (nothing is copied over what others may still read)
                 if (++e_half == halves) {
                     e_half = 0;
                     e_phase ^= 1u;
@@ -702,6 +714,12 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
 
     // ---- parts of items that more than one worker has: tails go where the rings were
     __syncthreads();
+    if (gave_up) {  // copies may still be under way: nothing takes their place, and they end before the block does
+        if (threadIdx.x == 0 && V.status) atomicOr(V.status, STATUS_WAIT_TIMEOUT);
+#pragma unroll 1
+        for (int i = 0; i < 64; i++) __nanosleep(100000u);
+        return;
+    }
     float *tails = reinterpret_cast<float *>(rings);
     if (open_tail) {
 #pragma unroll
