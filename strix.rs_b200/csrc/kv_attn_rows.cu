@@ -198,13 +198,25 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    // a wait that has run out is the last one of the block: everything goes on without waiting, to its end
+    // A wait that has run out is the last one of the block: every role leaves its loop at its next wait and touches nothing of the tile,
+    // whose description may not be there. By whole warps, whose lanes come to the same answer; wait_lane: by one lane.
     auto wait = [&](uint64_t *bar, uint32_t parity) {
+#pragma unroll 1
+        for (uint32_t it = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); it++)
+            if (__any_sync(0xffffffffu, gave_up || it >= 1u << 22)) {
+                gave_up = 1u;
+                return false;
+            }
+        return true;
+    };
+    auto wait_lane = [&](uint64_t *bar, uint32_t parity) {
+#pragma unroll 1
         for (uint32_t it = 0; !mbar_try_wait(bar, parity); it++)
             if (gave_up || it >= 1u << 22) {
                 gave_up = 1u;
-                break;
+                return false;
             }
+        return true;
     };
     // ... joins their parts, with warps 0 to 15
     auto join = [&] {
@@ -233,7 +245,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         uint32_t pos = 0, pos_lo = 0, pos_hi = 0, item = ~0u;
 #pragma unroll 1
         for (uint32_t n = b; n < n_tiles; n += 2u) {
-            wait(&s_full[b], (n >> 1) & 1u);
+            if (!wait(&s_full[b], (n >> 1) & 1u)) break;
             tc_fence_after();
             const PaTile &d = desc[n % RA_DESCS];
             const uint32_t valid = d.valid, tok = d.tile * RA_TT;
@@ -286,7 +298,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 }
             }
             const float base = top == -INFINITY ? 0.f : 15.f - top;
-            if (n >= 2u) wait(&o_full[b], ((n >> 1) & 1u) ^ 1u);  // the product of tile n - 2, which read this buffer of P
+            if (n >= 2u && !wait(&o_full[b], ((n >> 1) & 1u) ^ 1u)) break;  // the product of tile n - 2, which read this buffer of P
             tc_fence_after();
             float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -342,7 +354,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         for (uint32_t n = 0; n < n_tiles; n++) {
             const uint32_t b = n & 1u;
             const PaTile &d = desc[n % RA_DESCS];
-            wait(&m_full[n % RA_STATS], (n / RA_STATS) & 1u);
+            if (!wait(&m_full[n % RA_STATS], (n / RA_STATS) & 1u)) break;
             const uint32_t flags = d.flags;
             if (flags & PA_NEW) {
                 it_first = d.seq_first;
@@ -365,7 +377,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < HD; i++) o[i] *= alpha;
             }
-            wait(&o_full[b], (n >> 1) & 1u);
+            if (!wait(&o_full[b], (n >> 1) & 1u)) break;
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < HD / 32; c++) {
@@ -404,10 +416,10 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             }
             wrote |= !(flags & PA_WHOLE);
         }
-        if (wrote) {  // items that several blocks have: is this the last of them to come here?
+        if (wrote) __threadfence();
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+        if (wrote && !gave_up) {  // items that several blocks have: is this the last of them to come here?
             const PaCuts line(total, line_blocks);
-            __threadfence();
-            asm volatile("bar.sync 2, 128;" ::: "memory");
             if (warp < 10u && lane == 0) {
                 const uint32_t e = warp - 8u;
                 if (e == 0 ? parts.has_front : parts.has_back) {
@@ -435,10 +447,10 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
         };
 #pragma unroll 1
         for (uint32_t n = 0; n < n_tiles; n++) {
-            wait(&land_full[land], land_phase);
+            if (!wait(&land_full[land], land_phase)) break;
             const PaTile &d = desc[n % RA_DESCS];
             if (d.flags & PA_NEW) {
-                wait(q_empty, (items & 1u) ^ 1u);
+                if (!wait(q_empty, (items & 1u) ^ 1u)) break;
                 const uint32_t R = d.seq_rows * A.group, r = d.row0 + tid, rr = min(r, R - 1u), tk = by_group(A, rr);
                 pos_hi = d.ctx + by_group(A, min(d.row0 + RA_ROWS - 1u, R - 1u));
                 const float *src = A.q + (size_t)(d.seq_first + tk) * A.ld_q + (size_t)(d.head * A.group + rr - tk * A.group) * HD;
@@ -473,12 +485,13 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             }
             const uint32_t tok = d.tile * RA_TT;
             const bool keep = tok + tr <= pos_hi && ((d.valid >> (mixed ? tr >> pshift : 0u)) & 1u);
+            bool ok = true;
 #pragma unroll 1
             for (int kv = 0; kv < 2; kv++) {
-                if (kv) wait(&land_full[NL + land], land_phase);
+                if (kv && !(ok = wait(&land_full[NL + land], land_phase))) break;
                 uint8_t *dst = op + (size_t)(kv * NS + st) * S::OPB;
                 if constexpr (EL == 1) {
-                    wait(&op_empty[kv * NS + st], st_phase ^ 1u);
+                    if (!(ok = wait(&op_empty[kv * NS + st], st_phase ^ 1u))) break;
                     const uint8_t *src = raw + (size_t)(kv * NL + land) * S::RAWB + tr * HD;
                     uint4 x[HD / 32];
 #pragma unroll
@@ -516,6 +529,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     arrive(&op_full[kv * NS + st]);
                 }
             }
+            if (!ok) break;
             if (++land == NL) {
                 land = 0;
                 land_phase ^= 1u;
@@ -593,10 +607,11 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     d.vs[lane - b_from] = b_vs;
                 }
                 __syncwarp();
+                bool ok = true;
 #pragma unroll 1
                 for (int kv = 0; kv < 2; kv++) {
                     uint64_t *bar = &land_full[kv * NL + land];
-                    wait(&land_empty[kv * NL + land], land_phase ^ 1u);
+                    if (!(ok = wait(&land_empty[kv * NL + land], land_phase ^ 1u))) break;
                     if (leader) mbar_arrive_expect_tx(bar, __popc(valid) * sub * HD * EL);
                     __syncwarp();
                     uint8_t *dst = EL == 1 ? raw + (size_t)(kv * NL + land) * S::RAWB : op + (size_t)(kv * NS + land) * S::OPB;
@@ -613,6 +628,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                         }
                     }
                 }
+                if (!ok) break;
                 new_flag = 0u;
                 b_from += n_sub;
                 place.at++;
@@ -629,10 +645,10 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
 #pragma unroll 1
                 for (uint32_t n = 0; n < n_tiles; n++) {
                     const uint32_t b = n & 1u;
-                    wait(&op_full[st], phase);
+                    if (!wait_lane(&op_full[st], phase)) break;
                     const uint32_t flags = desc[n % RA_DESCS].flags;
-                    if (flags & PA_NEW) wait(q_full, items++ & 1u);
-                    wait(&s_empty[b], ((n >> 1) & 1u) ^ 1u);
+                    if (flags & PA_NEW && !wait_lane(q_full, items++ & 1u)) break;
+                    if (!wait_lane(&s_empty[b], ((n >> 1) & 1u) ^ 1u)) break;
                     tc_fence_after();
                     const uint32_t d = tmem + b * 64u;
                     const uint64_t kk = desc_sw128(op_at + st * S::OPB, 16u);
@@ -661,9 +677,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
 #pragma unroll 1
                 for (uint32_t n = 0; n < n_tiles; n++) {
                     const uint32_t b = n & 1u;
-                    wait(&op_full[NS + st], phase);
-                    wait(&o_empty[b], ((n >> 1) & 1u) ^ 1u);
-                    wait(&p_full[b], (n >> 1) & 1u);
+                    if (!wait_lane(&op_full[NS + st], phase) || !wait_lane(&o_empty[b], ((n >> 1) & 1u) ^ 1u) || !wait_lane(&p_full[b], (n >> 1) & 1u)) break;
                     tc_fence_after();
                     const uint64_t v = desc_sw128(op_at + (NS + st) * S::OPB, 8192u);
                     const uint32_t d = tmem + S::COL_O + b * HD, p = tmem + S::COL_P + b * 64u;
