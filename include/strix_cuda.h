@@ -399,7 +399,7 @@ STRIX_API int strix_cuda_gemv_rows(strix_cuda *h, const char *key, const float *
 STRIX_API int strix_cuda_gemv_rows_dev(strix_cuda *h, int nmat, const char *const *keys, const float *d_xs, size_t b,
                              int act, float *const *d_ys, void *stream);
 
-/* Device status word written by kernels whose bounded waits ran out
+/* Device status word written by kernels: bit 0 = a bounded wait ran out, bit 1 = sizes, positions or ids a kernel cannot take
  * (0 = clean). Synchronises `stream`. */
 STRIX_API int strix_cuda_device_status(strix_cuda *h, void *stream, uint32_t *status);
 /* Resets the status word (the host-buffer entry points do so themselves when they report it with -2; a

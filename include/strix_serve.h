@@ -10,8 +10,8 @@
  * CUDA graph, and leave the calling thread's current device as it was. Lengths, page ids and sampling parameters are
  * read from device memory by the kernels, so a captured graph serves every step.
  *
- * What the device data says wrong cannot be answered by a return code: it sets bit 1 of the handle's status word
- * (strix_cuda_device_status) and the part concerned is skipped as described below. No value of row0, ctx or pages makes a
+ * What the device data says wrong cannot be answered by a return code: it sets bit 1 of the handle's status
+ * (strix_cuda_device_status; no other call reports or clears what these set) and the part concerned is skipped as described below. No value of row0, ctx or pages makes a
  * kernel read or write outside the buffers described to it.
  */
 #ifndef STRIX_SERVE_H

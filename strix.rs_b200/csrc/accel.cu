@@ -469,8 +469,8 @@ int strix_cuda_create(int device, const strix_cuda_opts *opts, strix_cuda **out)
     h->name = std::string("cuda:") + std::to_string(device) + " " + p.name + " (sm_" + std::to_string(p.major) +
               std::to_string(p.minor) + "a)";
     e = cudaStreamCreateWithFlags(&h->stream, cudaStreamNonBlocking);
-    if (e == cudaSuccess) e = cudaMalloc(&h->d_status, sizeof(uint32_t));
-    if (e == cudaSuccess) e = cudaMemset(h->d_status, 0, sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaMalloc(&h->d_status, 2 * sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaMemset(h->d_status, 0, 2 * sizeof(uint32_t));
     if (e == cudaSuccess) e = gemv_prepare_device(h->smem_optin);
     if (e == cudaSuccess) e = chain_prepare_device(h->smem_optin);
     if (e == cudaSuccess) e = gemm_prepare_device();
@@ -824,7 +824,7 @@ int strix_cuda_gemv_batch(strix_cuda *h, size_t n, const char *const *keys, cons
     CU_TRY(h, cudaStreamSynchronize(h->stream));
     const uint32_t st = h->batch_flags[BATCH_GRAPH_MAX];
     if (st != 0) {
-        h->err = "gemv: device status " + std::to_string(st) + " (a bounded wait ran out)";
+        h->err = "gemv: " + status_text(st);
         cudaMemsetAsync(h->d_status, 0, 4, h->stream);
         return -2;
     }
@@ -1095,7 +1095,7 @@ int strix_cuda_gemv_rows(strix_cuda *h, const char *key, const float *xs, size_t
     CU_TRY(h, cudaMemcpyAsync(&h->status_host, h->d_status, 4, cudaMemcpyDeviceToHost, h->stream));
     CU_TRY(h, cudaStreamSynchronize(h->stream));
     if (h->status_host != 0) {
-        h->err = "gemv_rows: device status " + std::to_string(h->status_host) + " (a bounded wait ran out)";
+        h->err = "gemv_rows: " + status_text(h->status_host);
         cudaMemsetAsync(h->d_status, 0, 4, h->stream);
         return -2;
     }
@@ -1107,9 +1107,9 @@ int strix_cuda_device_status(strix_cuda *h, void *stream, uint32_t *status) {
     h->err.clear();
     CU_TRY(h, cudaSetDevice(h->device));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    CU_TRY(h, cudaMemcpyAsync(&h->status_host, h->d_status, 4, cudaMemcpyDeviceToHost, s));
+    CU_TRY(h, cudaMemcpyAsync(h->status_both, h->d_status, 8, cudaMemcpyDeviceToHost, s));
     CU_TRY(h, cudaStreamSynchronize(s));
-    *status = h->status_host;
+    *status = h->status_both[0] | h->status_both[1];
     return 1;
 }
 
@@ -1118,7 +1118,7 @@ int strix_cuda_clear_device_status(strix_cuda *h, void *stream) {
     h->err.clear();
     CU_TRY(h, cudaSetDevice(h->device));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    CU_TRY(h, cudaMemsetAsync(h->d_status, 0, 4, s));
+    CU_TRY(h, cudaMemsetAsync(h->d_status, 0, 8, s));
     CU_TRY(h, cudaStreamSynchronize(s));
     return 1;
 }

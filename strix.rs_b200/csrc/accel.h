@@ -78,8 +78,10 @@ struct strix_cuda {
     size_t batch_small_bytes = (size_t)256 << 20;  // (measured on 1/2 and 1/4 row shards of the benchmark step: 87 against 95 us, 50 against 61 us with 64 MiB)
     volatile uint32_t *batch_flags = nullptr;  // pinned, BATCH_GRAPH_MAX words
     uint32_t *d_one = nullptr;                 // device word holding 1
+    // two words: [0] of the kernels behind the host-buffer calls, which report it with -2 and clear it; [1] of the serving
+    // operators, whose callers ask for it (strix_cuda_device_status, which has both)
     uint32_t *d_status = nullptr;
-    uint32_t status_host = 0;
+    uint32_t status_host = 0, status_both[2] = {0, 0};
     std::unordered_map<std::string, strix::Resident> weights;
     std::unordered_map<std::string, strix::DevBuf> f32s;
     // staging for the host-pointer entry points (grown on demand, never shrunk; like the
@@ -121,6 +123,14 @@ struct strix_cuda {
 };
 
 namespace strix {
+// What a non-zero status word says (STATUS_* of common.cuh)
+inline std::string status_text(uint32_t status) {
+    std::string s = "device status " + std::to_string(status);
+    if (status & 1u) s += " (a bounded wait ran out)";
+    if (status & 2u) s += " (sizes or positions a kernel cannot take)";
+    return s;
+}
+
 // Brackets the launches made while it lives with two events on `s`, when profiling is on and `s` is not being
 // captured (events inside a capture cannot be timed). `name` must be a string literal.
 struct ProfScope {

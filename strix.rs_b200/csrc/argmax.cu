@@ -213,7 +213,7 @@ int strix_cuda_lm_head_argmax_rows(strix_cuda *h, const char *key, const float *
     CU_TRY(h, cudaMemcpyAsync(h->am_pin + ARGMAX_MAX_ROWS, h->d_status, 4, cudaMemcpyDeviceToHost, h->stream));
     CU_TRY(h, cudaStreamSynchronize(h->stream));
     if (h->am_pin[ARGMAX_MAX_ROWS] != 0) {
-        h->err = "lm_head_argmax_rows: device status " + std::to_string(h->am_pin[ARGMAX_MAX_ROWS]) + " (a bounded wait ran out)";
+        h->err = "lm_head_argmax_rows: " + status_text(h->am_pin[ARGMAX_MAX_ROWS]);
         cudaMemsetAsync(h->d_status, 0, 4, h->stream);
         return -2;
     }

@@ -109,7 +109,7 @@ static int prefill_gemm_host(strix_cuda *h, int fmt, const char *key, const floa
     CU_TRY(h, cudaMemcpyAsync(&h->status_host, h->d_status, 4, cudaMemcpyDeviceToHost, h->stream));
     CU_TRY(h, cudaStreamSynchronize(h->stream));
     if (h->status_host != 0) {
-        h->err = "prefill_q8_gemm: device status " + std::to_string(h->status_host) + " (a bounded wait ran out)";
+        h->err = "prefill_q8_gemm: " + status_text(h->status_host);
         cudaMemsetAsync(h->d_status, 0, 4, h->stream);
         return -2;
     }
@@ -184,7 +184,7 @@ static int block_isums(strix_cuda *h, const char *key, const float *xs, size_t m
         return -1;
     }
     if (h->status_host != 0) {
-        h->err = "debug isums: device status " + std::to_string(h->status_host) + " (a bounded wait ran out)";
+        h->err = "debug isums: " + status_text(h->status_host);
         cudaMemsetAsync(h->d_status, 0, 4, h->stream);
         return -2;
     }

@@ -451,7 +451,7 @@ int serve_check(strix_cuda *h, const char *what, const strix_kv_pages *c, const 
     if (!b) return serve_fail(h, what, "batch missing");
     const char *why = "";
     const int rc = kv_view(c, b, *v, &why);
-    v->status = h->d_status;
+    v->status = h->d_status + 1;
     return rc < 0 ? serve_fail(h, what, why) : rc;
 }
 

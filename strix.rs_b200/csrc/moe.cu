@@ -289,7 +289,7 @@ int finish(strix_cuda *h, const char *who) {
     CU_TRY(h, cudaMemcpyAsync(&h->status_host, h->d_status, 4, cudaMemcpyDeviceToHost, h->stream));
     CU_TRY(h, cudaStreamSynchronize(h->stream));
     if (h->status_host != 0) {
-        h->err = std::string(who) + ": device status " + std::to_string(h->status_host);
+        h->err = std::string(who) + ": " + status_text(h->status_host);
         cudaMemsetAsync(h->d_status, 0, 4, h->stream);
         return -2;
     }

@@ -273,6 +273,34 @@ def test_append_bad_device_data_is_skipped(torch, pkg, accel):
         assert (v == want).all()
 
 
+def test_bad_device_data_stays_with_the_serving_calls(torch, pkg, accel, orc, synth):
+    """What a bad page id sets is there to be read and cleared, and no other call takes it for a failure of its own."""
+    w, x = synth.q8_0(71, "status", 64, 512), synth.normal(71, "status.x", 512)
+    assert accel.upload_q8_0("serve.status", w, 512, 64) and accel.upload_q8_0("serve.status.head", w, 512, 64)
+    P = Paged(torch, pkg, pkg.KV_F16, 1, 16, 64, [32], fill=0)
+    P.table[0, 0] = P.n_pages
+    P.d_table.copy_(torch.from_numpy(P.table))
+    row = torch.ones(1, 64, device="cuda")
+    b = P.batch([0, 1], [3])
+    out = torch.zeros(1, 64, device="cuda")
+    work = work_of(torch, accel, P, b, 1)
+    appended = lambda: accel.kv_append_dev(P.desc, b, row.data_ptr(), row.data_ptr(), pkg.KvPrep(rope=pkg.ROPE_NONE), stream=stream(torch))  # noqa: E731
+    attended = lambda: accel.attn_pages_dev(P.desc, b, 1, row.data_ptr(), out.data_ptr(), 0.125, work.data_ptr(), work.numel(), stream=stream(torch))  # noqa: E731
+    want = orc.qmatmul(x, w, synth.Q8_0, 512, 64)
+    try:
+        for call in (appended, attended):
+            assert call()
+            torch.cuda.synchronize()
+            for got in (accel.gemv("serve.status", x), accel.gemv_rows("serve.status", x[None], 1)[0], accel.gemv_batch([("serve.status", x)])[0]):
+                assert np.linalg.norm(got - want) <= 1e-3 * np.linalg.norm(want)   # (the tolerance of the GEMV tests)
+            ids = accel.lm_head_argmax_rows("serve.status.head", x[None], 1)
+            assert int(ids[0]) == int(np.argmax(want))
+            assert accel.device_status() == 2 and accel.device_status() == 2
+            assert accel.clear_device_status() and accel.device_status() == 0
+    finally:
+        accel.clear_device_status()
+
+
 # ---------------------------------------------------------------- attention
 
 def check_attention(torch, accel, P, b, row0, ctx, heads, q, out, scale, window, hole=None, strict=1.0):
