@@ -97,7 +97,8 @@ STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_p
  * A row that sees no token gets zeros. Offsets that give away more rows than n_rows (possible where they go down) set the status
  * bit and leave out as it was. At most 8192 sequences in one call, and 2^31 tiles of 16 tokens in all blocks of rows when
  * every sequence fills its row of d_pages (-1 beyond). Products and sums keep f32 accuracy (f16 tensor-core products of q and
- * of the probabilities in two halves of 11 bits each).
+ * of the probabilities in two halves of 11 bits each: an element of q is off by 2^-22 of itself or 2^-39 of the largest of its head, a
+ * probability times its page's scale by 2^-22 of itself or 2^-39 of the row's largest among 16 to 64 neighbouring tokens).
  * d_work: work_bytes >= strix_cuda_attn_pages_workspace, 256-byte aligned, zeroed once before its first use; every
  * call leaves it ready for the next (of any sizes that fit), but for one whose bounded wait ran out (bit 0 of the status): out is
  * unspecified then and d_work has to be zeroed again. Calls that share a workspace must not run at the same time; graphs

@@ -9,7 +9,9 @@
 // both go in as two f16 halves (value, and what rounding it left). Up to eight rows, the two halves ARE the sixteen
 // rows of one product: rows 0..7 the values, rows 8..15 the remainders, and the two accumulators of a row meet in one thread.
 // Beyond eight rows a warp has sixteen rows and issues two products. q is scaled by a power of two to use f16's range (a row's
-// largest value in [2^14, 2^15)), probabilities by 2^15: what is lost lies below 2^-33 of the row's largest. The sums over a tile
+// largest value in [2^14, 2^15)). Probabilities go in relative to the tile's largest, which becomes 2^15; where a tile holds pages of
+// different scales, the largest product of weight and scale that the row has there goes to [2^14, 2^15) instead. So a weight is off by
+// 2^-22 of itself or 2^-39 of the largest of its tile, and no page that a row does not see has a part in that. The sums over a tile
 // start from zero and are added to the f32 running sums outside the tensor cores, which round to nearest: chained
 // accumulation in the tensor cores truncates, a drift of its own over thousands of tokens.
 // The order of the head's dimensions inside a product is free as long as q and k agree, and so is the order of the
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
     uint32_t half = 0, phase = 0, e_half = 0, e_phase = 0;  // next half to use; next to refill
     uint32_t qf[S::QSMEM ? 1 : KS][WIDE ? 8 : 4];  // fragments of q: values (and remainders, in the same rows or apart)
     uint4 *qs = reinterpret_cast<uint4 *>(qsm) + warp * (KS * 2 * 32) + lane;
-    float qc[RW], vref = 0.f;                      // factor from the products to exponents of two; scale of the tile's values
+    float qc[RW], wv[RW];                          // factor from the products to exponents of two; of the tile's sums: weight and scale
     uint32_t pos[RW], pos_lo = 0, pos_hi = 0;      // positions of this thread's rows, of the warp's first and last row
     uint32_t pf[TT / 16][WIDE ? 8 : 4];            // fragments of the weights
     bool tail_tok = false;
@@ -487,11 +489,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
                     sc[j][3] *= k0 * qc[RW - 1];
                 }
             }
-            vref = d.vs[0];
-            float rvref = 1.f;
-            if (several) {  // scores, and weights before they meet the values, take what another page's scale differs by
-                vref = fmaxf(fmaxf(d.vs[0], d.vs[1]), fmaxf(d.vs[2], d.vs[3]));
-                rvref = vref > 0.f ? 1.0f / vref : 1.f;
+            if (several) {  // scores take what another page's scale differs by
                 const float rk0 = k0 > 0.f ? 1.0f / k0 : 0.f;
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
@@ -512,9 +510,11 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
                     }
                 }
             }
+            // weights are relative to the tile's own maximum, so that what two halves lose of them goes by the tile and not by the largest
+            // score so far: a tile of small weights may hold the large values
             float mx[RW];
 #pragma unroll
-            for (int i = 0; i < RW; i++) mx[i] = m[i];
+            for (int i = 0; i < RW; i++) mx[i] = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NT; j++)
 #pragma unroll
@@ -524,13 +524,13 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
             for (int i = 0; i < RW; i++) {
                 mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
                 mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-                moved |= mx[i] != m[i];
+                moved |= mx[i] > m[i];
             }
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                 for (int i = 0; i < RW; i++) {
-                    const float a = mx[i] == m[i] ? 1.f : ex2(m[i] - mx[i]);
-                    m[i] = mx[i];
+                    const float a = mx[i] > m[i] ? ex2(m[i] - mx[i]) : 1.f;
+                    m[i] = fmaxf(m[i], mx[i]);
                     l[i] *= a;
 #pragma unroll
                     for (int k = 0; k < NO; k++) {
@@ -539,28 +539,55 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
                     }
                 }
             }
-            float base[RW];
+            float base[RW], lt[RW];
 #pragma unroll
-            for (int i = 0; i < RW; i++) base[i] = m[i] == -INFINITY ? 0.f : m[i] - 15.f;  // weights carry 2^15, as their sum does
+            for (int i = 0; i < RW; i++) {
+                base[i] = mx[i] == -INFINITY ? 0.f : mx[i] - 15.f;  // weights carry 2^15, as their sum does
+                lt[i] = 0.f;
+                wv[i] = mx[i] == m[i] ? 1.f : ex2(mx[i] - m[i]);
+            }
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                float p[2 * RW];
+            for (int j = 0; j < NT; j++)
 #pragma unroll
                 for (int e = 0; e < 2 * RW; e++) {
-                    p[e] = ex2(sc[j][e] - base[e >> 1]);
-                    l[e >> 1] += p[e];
+                    sc[j][e] = ex2(sc[j][e] - base[e >> 1]);
+                    lt[e >> 1] += sc[j][e];
                 }
-                if (TT > 16 && mixed) {
-                    const float f = d.vs[(8u * j) >> pshift] * rvref;
 #pragma unroll
-                    for (int e = 0; e < 2 * RW; e++) p[e] *= f;
+            for (int i = 0; i < RW; i++) l[i] = fmaf(lt[i], wv[i], l[i]);
+            if (EL == 1 && several) {
+                float top[RW], up[RW];
+#pragma unroll
+                for (int i = 0; i < RW; i++) top[i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int e = 0; e < 2 * RW; e++) top[e >> 1] = fmaxf(top[e >> 1], sc[j][e] * (d.vs[(8u * j) >> pshift] * 0x1p-15f));
+#pragma unroll
+                for (int i = 0; i < RW; i++) {
+                    float back;
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                    row_scale(top[i], up[i], back);
+                    wv[i] *= back;
                 }
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int e = 0; e < 2 * RW; e++) sc[j][e] *= page_factor(d.vs[(8u * j) >> pshift] * 0x1p-15f, up[e >> 1]);
+            } else if (EL == 1) {
+#pragma unroll
+                for (int i = 0; i < RW; i++) wv[i] *= d.vs[0];
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const float(&p)[4] = sc[j];
                 const int u = j / 2, hf = (j & 1) * 2;
                 if constexpr (!WIDE) {
                     split2(p[0], p[1], pf[u][hf], pf[u][hf + 1]);
                 } else {
                     split2(p[0], p[1], pf[u][hf], pf[u][4 + hf]);
-                    split2(p[2], p[2 * RW - 1], pf[u][hf + 1], pf[u][4 + hf + 1]);
+                    split2(p[2], p[3], pf[u][hf + 1], pf[u][4 + hf + 1]);
                 }
             }
         } else {
@@ -634,11 +661,11 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
                     for (int e = 0; e < PER; e++) {
                         float(&oo)[2 * RW] = o[(c * (VW / 4) + w) * PER + e];
                         if constexpr (!WIDE) {
-                            oo[0] = fmaf(acc[e][0] + acc[e][2], vref, oo[0]);
-                            oo[1] = fmaf(acc[e][1] + acc[e][3], vref, oo[1]);
+                            oo[0] = fmaf(acc[e][0] + acc[e][2], wv[0], oo[0]);
+                            oo[1] = fmaf(acc[e][1] + acc[e][3], wv[0], oo[1]);
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 2 * RW; k++) oo[k] = fmaf(acc[e][k], vref, oo[k]);
+                            for (int k = 0; k < 2 * RW; k++) oo[k] = fmaf(acc[e][k], wv[k >> 1], oo[k]);
                         }
                     }
                 }

@@ -2,8 +2,8 @@
 // tcgen05 tensor cores. Contract: include/strix_serve.h; the form for few rows, the line of tiles and the joins: kv_attn.cu.
 //
 // Arithmetic as there: f16 products with f32 sums, q and the weights in two f16 halves (the value, and what rounding it left), so
-// every product runs twice; q scaled by a power of two to a largest value in [2^14, 2^15), weights by 2^15; e4m3 cache values widened
-// to f16, exactly. A tile is 64 tokens of one KV head.
+// every product runs twice; q scaled by a power of two to a largest value in [2^14, 2^15), weights relative to the tile's largest (as
+// there, with their pages' scales where those differ); e4m3 cache values widened to f16, exactly. A tile is 64 tokens of one KV head.
 //   S = Qhi K^T + Qlo K^T     128 x 64 sums in TMEM, operands in shared memory (K-major, 128-byte swizzle)
 //   P = 2^(S c - max), split  by the thread that has the row, written to TMEM as the A operand of
 //   O = Phi V + Plo V         128 x head size, from zero for every tile; V as it lies, [token][dimension] (MN-major)
@@ -50,7 +50,7 @@ struct RowsShape {
     static constexpr int NL = EL == 1 ? NR : NS;      // tiles that copies land in
     static constexpr bool RAWSWZ = HD == 128;         // rows of 128 codes are swizzled on their way, rows of 64 lie as they are
     static constexpr int BARS = 4 * NL + 4 * NS + 2 + 5 * 2 + (int)RA_STATS;
-    static constexpr size_t SMEM = 2 * QB + 2 * NS * OPB + 2 * NR * RAWB + RA_DESCS * sizeof(PaTile) + RA_QBUF * 128 * 4 + 2 * RA_STATS * 128 * 4 + BARS * 8 + 1024;
+    static constexpr size_t SMEM = 2 * QB + 2 * NS * OPB + 2 * NR * RAWB + RA_DESCS * sizeof(PaTile) + RA_QBUF * 128 * 4 + (EL == 1 ? 3 : 2) * RA_STATS * 128 * 4 + BARS * 8 + 1024;
     // TMEM columns: S 2 x 64, P 2 x (32 + 32), O 2 x HD
     static constexpr uint32_t COL_P = 128, COL_O = 256;
 };
@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
     PaTile *desc = reinterpret_cast<PaTile *>(raw + 2 * S::NR * S::RAWB);
     float *q_factor = reinterpret_cast<float *>(desc + RA_DESCS);  // [RA_QBUF][128]
     float *tile_m = q_factor + RA_QBUF * 128, *tile_l = tile_m + RA_STATS * 128;  // [RA_STATS][128]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(tile_l + RA_STATS * 128);
+    float *tile_v = tile_l + RA_STATS * 128;  // the same, with e4m3: what scales the tile's product
+    uint64_t *bars = reinterpret_cast<uint64_t *>(tile_v + (EL == 1 ? RA_STATS * 128 : 0));
     uint64_t *land_full = bars, *land_empty = land_full + 2 * NL;  // [k, v][NL]
     uint64_t *op_full = land_empty + 2 * NL, *op_empty = op_full + 2 * NS;
     uint64_t *q_full = op_empty + 2 * NS, *q_empty = q_full + 1;
@@ -257,9 +258,6 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 pos_hi = ctx + by_group(A, min(row0 + (row | 31u), R - 1u));
                 f_q = q_factor[(item % RA_QBUF) * 128u + row];
             }
-            float vref = d.vs[0];
-            if (mixed) vref = fmaxf(fmaxf(vref, d.vs[1]), fmaxf(d.vs[2], d.vs[3]));
-            const float rvref = vref > 0.f ? 1.0f / vref : 0.f;
             uint64_t sees = ~0ull;  // one bit for each token that the row sees
             if (tok + RA_TT - 1u > pos_lo || valid != (1u << n_sub) - 1u || (A.window && pos_hi >= A.window && tok <= pos_hi - A.window)) {
                 const uint32_t last = pos - tok, from = A.window && pos >= A.window && pos - A.window >= tok ? pos - A.window - tok + 1u : 0u;
@@ -281,7 +279,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             // the factor to exponents of two is positive (the sign of the caller's scale went into q), so the largest product is the
             // largest score; it multiplies inside the exponent's subtraction
             auto factor = [&](uint32_t c) { return fmaxf(d.ks[mixed ? c >> pshift : 0u] * f_q, 1.0e-30f); };
-            float top = -INFINITY;
+            float top = -INFINITY, most = 0.f;  // most: largest weight times scale, with several scales in the tile
 #pragma unroll 1
             for (uint32_t c = 0; c < RA_TT; c += 32u) {
                 uint32_t s[32];
@@ -294,13 +292,26 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                         t0 = fmaxf(t0, __uint_as_float(s[i]));
                         t1 = fmaxf(t1, __uint_as_float(s[i + 1]));
                     }
-                    top = fmaxf(top, fmaxf(t0, t1) * factor(c + h));
+                    const float t = fmaxf(t0, t1) * factor(c + h);
+                    if (EL == 1 && mixed) {
+                        const float now = fmaxf(top, t);
+                        if (now > -INFINITY) most = fmaxf(most * ex2(top - now), ex2(t - now) * d.vs[(c + h) >> pshift]);
+                        top = now;
+                    } else {
+                        top = fmaxf(top, t);
+                    }
                 }
             }
             const float base = top == -INFINITY ? 0.f : 15.f - top;
             if (n >= 2u && !wait(&o_full[b], ((n >> 1) & 1u) ^ 1u)) break;  // the product of tile n - 2, which read this buffer of P
             tc_fence_after();
             float2 l2 = make_float2(0.f, 0.f);
+            float up = 1.f;
+            if constexpr (EL == 1) {
+                float back = d.vs[0];
+                if (mixed) row_scale(most, up, back);
+                tile_v[(n % RA_STATS) * 128u + row] = back;
+            }
 #pragma unroll 1
             for (uint32_t c = 0; c < RA_TT; c += 32u) {
                 uint32_t s[32];
@@ -316,8 +327,8 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                         p[i] = make_float2(ex2(y.x), ex2(y.y));
                         l2 = add2(l2, p[i]);
                     }
-                    if (mixed) {
-                        const float w = d.vs[(c + h) >> pshift] * rvref;
+                    if (EL == 1 && mixed) {
+                        const float w = page_factor(d.vs[(c + h) >> pshift] * 0x1p-15f, up);
 #pragma unroll
                         for (int i = 0; i < 8; i++) p[i] = make_float2(p[i].x * w, p[i].y * w);
                     }
@@ -368,9 +379,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
             }
             const float m_tile = tile_m[(n % RA_STATS) * 128u + row], m_new = fmaxf(m, m_tile);
             const float alpha = m_new == m ? 1.f : ex2(m - m_new), beta = m_new == m_tile ? 1.f : ex2(m_tile - m_new);
-            float vref = d.vs[0];
-            if (mixed) vref = fmaxf(fmaxf(vref, d.vs[1]), fmaxf(d.vs[2], d.vs[3]));
-            const float w = beta * vref;
+            const float w = EL == 1 ? beta * tile_v[(n % RA_STATS) * 128u + row] : beta;
             l = fmaf(tile_l[(n % RA_STATS) * 128u + row], beta, l * alpha);
             m = m_new;
             if (__any_sync(0xffffffffu, alpha != 1.f)) {

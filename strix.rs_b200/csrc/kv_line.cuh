@@ -48,6 +48,16 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_
     const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
     lo = f32_to_f16x2(x0 - h.x, x1 - h.y);
 }
+// A tile whose pages have scales of their own: its weights meet their pages' scales before the product, and a power of two 2^u
+// brings the largest weight times scale of a row (`most`, the scales times 2^-15) to [2^14, 2^15). What multiplies the product is 2^(15 - u).
+// (u stops at 127: below scales of 2^-112 the weights are a few bits further down.)
+__device__ __forceinline__ void row_scale(float most, float &up, float &back) {
+    const int e = max((int)(__float_as_uint(most) >> 23) - 127, -113);
+    up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+    back = __uint_as_float((uint32_t)(e + 1 + 127) << 23);
+}
+// the factor of a page's weights; bounded where its weights are below 2^-126 of the row's largest
+__device__ __forceinline__ float page_factor(float vs15, float up) { return fminf(vs15 * up, 8.5e37f); }
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
                      smem_u32(dst)),

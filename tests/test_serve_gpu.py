@@ -426,6 +426,80 @@ def test_attention_scales_of_pages_far_apart(torch, pkg, accel):
     check_attention(torch, accel, P, b, row0, [100], 2, q, out, 0.125, 0)
 
 
+def check_attention_by_weight(P, s, row0, c, heads, q, out, scale, window):
+    """The rows of sequence s against 64 bits, with a bound that goes by what a row sees and how much of it: the terms of check_attention
+    times sum p |v| of the row, and what two halves of 11 bits lose of a weight (2^-38 of the largest weight times page scale, at codes of
+    up to 448: half a step of the smallest f16, 2^-25, where the largest is 2^14 or more, once for each half of a product)."""
+    hq, ho = q.cpu().numpy().reshape(q.shape[0], heads, P.hd), out.cpu().numpy().reshape(q.shape[0], heads, P.hd)
+    n, g = c + row0[s + 1] - row0[s], heads // P.n_kv
+    k, v = P.tokens("k", s, n), P.tokens("v", s, n)
+    vs = P.scale["v"].cpu().numpy().astype(np.float64)[P.table[s, np.arange(n) // P.page]]
+    for i, r in enumerate(range(row0[s], row0[s + 1])):
+        pos = c + i
+        see = np.arange(max(0, pos + 1 - window) if window else 0, pos + 1)
+        want = so.attend(hq[r], k, v, pos, scale, window)
+        for h in range(heads):
+            kk, vv, qq = k[see, h // g], v[see, h // g], hq[r, h].astype(np.float64)
+            sc = kk @ qq * scale
+            p = np.exp(sc - sc.max())
+            p /= p.sum()
+            d = 2 * (P.hd + 8) * 2.0 ** -24 * (np.abs(kk) @ np.abs(qq) * scale).max() + 2.0 ** -20
+            bound = d * (p @ np.abs(vv)).max() + 2.0 ** -38 * 448 * (p * vs[see, h // g]).max()
+            assert np.abs(ho[r, h] - want[h]).max() <= bound, (i, h, np.abs(ho[r, h] - want[h]).max(), bound)
+
+
+# (up to 8 rows a KV head, up to 16, more: the three forms; tiles of 32 and 64 tokens that hold two or four pages)
+@pytest.mark.parametrize("apart", [20, 30, 40, 100])
+@pytest.mark.parametrize("hd,page,group", [(64, 16, 1), (64, 32, 1), (96, 16, 1), (128, 16, 1), (64, 16, 2), (64, 32, 2), (96, 16, 2), (128, 16, 2),
+                                           (96, 16, 5), (64, 16, 4), (64, 32, 4), (128, 16, 4), (128, 32, 4)])
+def test_attention_small_page_next_to_a_large_one(torch, pkg, accel, hd, page, group, apart):
+    """Rows that see only the page of small scale of a tile (the large one comes later, or lies before the window) are as exact as
+    others: no page that a row does not see has a part in its result."""
+    new, c = 8, page - 4
+    for window in (0, 4):
+        P = Paged(torch, pkg, pkg.KV_E4M3, 1, page, hd, [c + new], seed=hd + page)
+        P.seed_random(group, [c + new])
+        P.scale["k"].fill_(2.0 ** -20)
+        for j in (0, 1):       # window 0: rows 0 to 3 see page 0 only; window 4: row 7 sees page 1 only
+            P.scale["v"][P.table[0, j]] = 2.0 ** (0 if (j == 0) == bool(window) else -apart)
+        b = P.batch([0, new], [c])
+        g = torch.Generator(device="cuda").manual_seed(hd)
+        q = torch.randn(new, group * hd, generator=g, device="cuda")
+        out = torch.zeros_like(q)
+        w = work_of(torch, accel, P, b, group)
+        assert accel.attn_pages_dev(P.desc, b, group, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), window=window, stream=stream(torch))
+        torch.cuda.synchronize()
+        check_attention_by_weight(P, 0, [0, new], c, group, q, out, 0.125, window)
+
+
+@pytest.mark.parametrize("kv,hd,page,group,new", [(1, 128, 64, 4, 1), (1, 192, 16, 2, 1), (0, 128, 64, 4, 1), (1, 128, 64, 4, 4), (0, 64, 32, 16, 1), (1, 256, 32, 4, 6),
+                                                  (1, 128, 64, 4, 8), (0, 64, 64, 8, 6)])
+def test_attention_small_weights_of_large_values(torch, pkg, accel, kv, hd, page, group, new):
+    """One page has nearly all the weight and tiny values, another some 2^-35 of the weight and the values that make the result."""
+    n = 2 * page
+    c = n - new
+    P = Paged(torch, pkg, kv, 1, page, hd, [n], seed=hd)
+    P.seed_random(new, [n])
+    if kv == pkg.KV_E4M3:
+        for j, ks, vs in ((0, 0.5, 2.0 ** -60), (1, 2.0 ** -20, 1.0)):
+            P.scale["k"][P.table[0, j]], P.scale["v"][P.table[0, j]] = ks, vs
+        qs = 1.0
+    else:
+        raw = {m: P.raw[m].view(torch.float16).view(P.n_pages, 1, page, hd) for m in "kv"}
+        raw["k"][int(P.table[0, 1])] *= 2.0 ** -12
+        raw["v"][int(P.table[0, 0])] *= 2.0 ** -14
+        P.scale["v"].fill_(2.0 ** -7)       # (for the bound: the largest values are near 4)
+        qs = 12.0 * (128 / hd) ** 0.5
+    b = P.batch([0, new], [c])
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    q = torch.randn(new, group * hd, generator=g, device="cuda") * qs
+    out = torch.zeros_like(q)
+    w = work_of(torch, accel, P, b, group)
+    assert accel.attn_pages_dev(P.desc, b, group, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+    torch.cuda.synchronize()
+    check_attention_by_weight(P, 0, [0, new], c, group, q, out, 0.125, 0)
+
+
 def test_attention_nan_query_stays_in_its_row(torch, pkg, accel):
     for new in ([1, 1], [3, 20]):
         P, b, row0, q, out, w = run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 2, 16, 64, new, [40, 50])
