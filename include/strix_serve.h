@@ -24,7 +24,8 @@ extern "C" {
 #endif
 
 /* Element type of a paged cache. E4M3: 8-bit floats (4 exponent, 3 mantissa bits; largest value 448) and one f32 scale
- * for each page and KV head, a cached value being code * scale. */
+ * for each page and KV head, a cached value being code * scale. Scales are positive; strix_cuda_kv_append_dev writes powers of two
+ * (with others in k, attention scores of 2^20 and more are not kept to f32 accuracy). */
 enum { STRIX_KV_F16 = 0, STRIX_KV_E4M3 = 1 };
 /* Which elements of a head a rotation pairs: none, (j, j + head_dim/2), or (2j, 2j + 1). */
 enum { STRIX_ROPE_NONE = 0, STRIX_ROPE_HALVES = 1, STRIX_ROPE_ADJACENT = 2 };
@@ -97,7 +98,7 @@ STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_p
  * A row that sees no token gets zeros. Offsets that give away more rows than n_rows (possible where they go down) set the status
  * bit and leave out as it was. At most 8192 sequences in one call, and 2^31 tiles of 16 tokens in all blocks of rows when
  * every sequence fills its row of d_pages (-1 beyond). Products and sums keep f32 accuracy (f16 tensor-core products of q and
- * of the probabilities in two halves of 11 bits each: an element of q is off by 2^-22 of itself or 2^-39 of the largest of its head, a
+ * of the probabilities in two halves of 11 bits each: an element of q is off by 2^-22 of itself or 2^-38 of the largest of its head, a
  * probability times its page's scale by 2^-22 of itself or 2^-39 of the row's largest among 16 to 64 neighbouring tokens).
  * d_work: work_bytes >= strix_cuda_attn_pages_workspace, 256-byte aligned, zeroed once before its first use; every
  * call leaves it ready for the next (of any sizes that fit), but for one whose bounded wait ran out (bit 0 of the status): out is

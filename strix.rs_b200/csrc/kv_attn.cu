@@ -32,6 +32,7 @@
 // scales, q; the joins); in between, instruction issue bounds: some 1000 instructions a tile, of which the fragments of k and v,
 // their conversion and the two halves' products are two thirds.
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <algorithm>
@@ -542,7 +543,8 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
             float base[RW], lt[RW];
 #pragma unroll
             for (int i = 0; i < RW; i++) {
-                base[i] = mx[i] == -INFINITY ? 0.f : mx[i] - 15.f;  // weights carry 2^15, as their sum does
+                // weights carry 2^15, as their sum does (rounded up: scores of 2^24 and more would else give 2^16, which f16 does not have)
+                base[i] = mx[i] == -INFINITY ? 0.f : __fsub_ru(mx[i], 15.f);
                 lt[i] = 0.f;
                 wv[i] = mx[i] == m[i] ? 1.f : ex2(mx[i] - m[i]);
             }
@@ -1002,6 +1004,9 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     A.window = window;
     A.cap = A.V.pages_ld * A.V.page_tokens;
     A.scale = scale;
+    int scale_e = 0;
+    A.scale_m = (float)frexp((double)scale * 1.4426950408889634, &scale_e);
+    A.scale_p = ldexpf(1.f, scale_e);
     A.vec = ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15u) == 0 && ((A.ld_q | A.ld_out) & 3u) == 0;
     A.ticket = static_cast<uint32_t *>(d_work);
     A.part = reinterpret_cast<float *>(static_cast<uint8_t *>(d_work) + PA_MAX_BLOCKS * 4);

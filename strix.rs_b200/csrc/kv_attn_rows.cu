@@ -2,7 +2,7 @@
 // tcgen05 tensor cores. Contract: include/strix_serve.h; the form for few rows, the line of tiles and the joins: kv_attn.cu.
 //
 // Arithmetic as there: f16 products with f32 sums, q and the weights in two f16 halves (the value, and what rounding it left), so
-// every product runs twice; q scaled by a power of two to a largest value in [2^14, 2^15), weights relative to the tile's largest (as
+// every product runs twice; q scaled to a largest value in [2^13, 2^15), weights relative to the tile's largest (as
 // there, with their pages' scales where those differ); e4m3 cache values widened to f16, exactly. A tile is 64 tokens of one KV head.
 //   S = Qhi K^T + Qlo K^T     128 x 64 sums in TMEM, operands in shared memory (K-major, 128-byte swizzle)
 //   P = 2^(S c - max), split  by the thread that has the row, written to TMEM as the A operand of
@@ -276,9 +276,10 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     for (int i = 0; i < 32; i++) s[i] = (bits >> i) & 1u ? s[i] : 0xff800000u;
                 }
             };
-            // the factor to exponents of two is positive (the sign of the caller's scale went into q), so the largest product is the
-            // largest score; it multiplies inside the exponent's subtraction
-            auto factor = [&](uint32_t c) { return fmaxf(d.ks[mixed ? c >> pshift : 0u] * f_q, 1.0e-30f); };
+            // The factor to exponents of two is positive, so the largest product is the largest score. It is a power of two (the rest of the
+            // caller's scale went into q, and the pages' scales are powers of two), so that it can multiply inside the exponent's
+            // subtraction: what is taken off there is the maximum without any rounding, however large the scores are.
+            auto factor = [&](uint32_t c) { return fmaxf(d.ks[mixed ? c >> pshift : 0u] * f_q, 0x1p-100f); };
             float top = -INFINITY, most = 0.f;  // most: largest weight times scale, with several scales in the tile
 #pragma unroll 1
             for (uint32_t c = 0; c < RA_TT; c += 32u) {
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                     }
                 }
             }
-            const float base = top == -INFINITY ? 0.f : 15.f - top;
+            const float base = top == -INFINITY ? 0.f : -__fsub_ru(top, 15.f);  // (upwards: no weight above 2^15)
             if (n >= 2u && !wait(&o_full[b], ((n >> 1) & 1u) ^ 1u)) break;  // the product of tile n - 2, which read this buffer of P
             tc_fence_after();
             float2 l2 = make_float2(0.f, 0.f);
@@ -475,8 +476,8 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 }
                 const int ex = (int)(__float_as_uint(top) >> 23);
                 const int e2 = top > 0.f && ex < 255 ? min(126, max(-126, 14 + 127 - max(ex, 1))) : 0;
-                const float up = copysignf(__uint_as_float((uint32_t)(e2 + 127) << 23), A.scale);
-                q_factor[(items % RA_QBUF) * 128u + tid] = fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e2) << 23);
+                const float up = A.scale_m * __uint_as_float((uint32_t)(e2 + 127) << 23);
+                q_factor[(items % RA_QBUF) * 128u + tid] = A.scale_p * __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll 4
                 for (int i = 0; i < HD; i += 8) {
                     const float4 x = load4(i), y = load4(i + 4);

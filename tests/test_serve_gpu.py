@@ -416,6 +416,45 @@ def test_attention_extreme_scores(torch, pkg, accel):
     run_attention(torch, pkg, accel, pkg.KV_F16, 1, 4, 16, 64, [1, 2], [90, 200], qs=0.0)
 
 
+# (rows of a KV head: few, up to 16, many)
+@pytest.mark.parametrize("kv,hd,page,group,new", [(0, 64, 16, 2, 1), (1, 128, 16, 4, 2), (0, 192, 16, 4, 3), (1, 64, 64, 4, 4), (0, 128, 32, 8, 4), (1, 64, 16, 8, 5),
+                                                  (1, 128, 64, 4, 9)])
+def test_attention_scores_beyond_two_to_the_twenty(torch, pkg, accel, kv, hd, page, group, new):
+    """Scores of up to 2^40 whose order f32 tells (one dimension, steps of a sixteenth): the largest has all the weight, so the output
+    is that token's value, up to what the two halves leave."""
+    n = 6 * page + 5
+    P = Paged(torch, pkg, kv, 1, page, hd, [n], seed=hd)
+    P.seed_random(new, [n])
+    P.scale["k"].fill_(1.0)
+    rng = np.random.RandomState(new)
+    k = np.zeros((n, hd))
+    k[:, 0] = np.array([1.0, 1.125, 1.25, 1.5, 0.5, 0.75])[rng.randint(0, 6, n)]
+    best = rng.randint(0, n - new)
+    k[best, 0] = 1.75
+    codes = {0.5: 0x30, 0.75: 0x34, 1.0: 0x38, 1.125: 0x39, 1.25: 0x3a, 1.5: 0x3c, 1.75: 0x3e, 0.0: 0}
+    raw = P.raw["k"].cpu().numpy().copy()
+    for t in range(n):
+        o = P.table[0, t // page] * P.stride + (t % page) * hd
+        if kv == pkg.KV_F16:
+            raw.view(np.float16)[o:o + hd] = k[t]
+        else:
+            raw[o:o + hd] = [codes[x] for x in k[t]]
+    P.raw["k"].copy_(torch.from_numpy(raw))
+    assert (P.tokens("k", 0, n)[:, 0] == k).all()
+    v = P.tokens("v", 0, n)[:, 0]
+    b = P.batch([0, new], [n - new])
+    out = torch.zeros(new, group * hd, device="cuda")
+    w = work_of(torch, accel, P, b, group)
+    for power in (19, 20, 22, 23, 24, 25, 26, 27, 28, 30, 40):
+        for jitter in (1.0, 1.37, 1.9):
+            q = torch.zeros(new, group, hd, device="cuda")
+            q[..., 0] = 2.0 ** power * jitter
+            assert accel.attn_pages_dev(P.desc, b, group, q.data_ptr(), out.data_ptr(), 1.0, w.data_ptr(), w.numel(), stream=stream(torch))
+            torch.cuda.synchronize()
+            got = out.cpu().numpy().reshape(new, group, hd).astype(np.float64)
+            assert (np.abs(got - v[best]) <= 2.0 ** -20 * np.abs(v[best]).max()).all(), (power, jitter)
+
+
 def test_attention_scales_of_pages_far_apart(torch, pkg, accel):
     """Pages whose scales differ by 2^30: no page overflows or hides another."""
     P, b, row0, q, out, w = run_attention(torch, pkg, accel, pkg.KV_E4M3, 1, 2, 16, 64, [1], [100])
