@@ -89,7 +89,9 @@ STRIX_API int strix_cuda_kv_append_dev(strix_cuda *h, const strix_kv_pages *cach
                              uint32_t n_heads, const float *d_k, size_t ld_k, const float *d_v, size_t ld_v, const float *d_q,
                              size_t ld_q, float *d_q_out, size_t ld_q_out, void *stream);
 
-/* Bytes of workspace for strix_cuda_attn_pages_dev with these sizes (device data is not looked at), 0 = declined. */
+/* Bytes of workspace for strix_cuda_attn_pages_dev, 0 = declined (device data is not looked at): enough for every batch of up to
+ * n_rows rows, into whatever number of sequences they divide, over any cache of this head_dim with at most as many query heads to a
+ * KV head. */
 STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_pages *cache, const strix_kv_batch *batch, uint32_t n_heads);
 /* out[row][head] = softmax(scale * q k^T) v over the cached tokens the row sees: positions 0 .. its own (its own k and v
  * are in the cache by then), with window > 0 only the last `window` of them. n_heads is a multiple of n_kv; head h reads KV
@@ -101,7 +103,7 @@ STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_p
  * of the probabilities in two halves of 11 bits each: an element of q is off by 2^-22 of itself or 2^-38 of the largest of its head, a
  * probability times its page's scale by 2^-22 of itself or 2^-39 of the row's largest among 16 to 64 neighbouring tokens).
  * d_work: work_bytes >= strix_cuda_attn_pages_workspace, 256-byte aligned, zeroed once before its first use; every
- * call leaves it ready for the next (of any sizes that fit), but for one whose bounded wait ran out (bit 0 of the status): out is
+ * call leaves it ready for the next (of any sizes that the workspace serves), but for one whose bounded wait ran out (bit 0 of the status): out is
  * unspecified then and d_work has to be zeroed again. Calls that share a workspace must not run at the same time; graphs
  * replayed on different streams therefore need one each. The result does not depend on what else runs: partial sums
  * are joined in a fixed order. */

@@ -597,7 +597,7 @@ class CudaWeightAccel:
         return self._check(rc) == 1
 
     def attn_pages_workspace(self, cache, batch, n_heads):
-        """Bytes of (once zeroed) device workspace attn_pages_dev needs for these sizes, 0 = declined."""
+        """Bytes of (once zeroed) device workspace for attn_pages_dev with batches of up to so many rows, 0 = declined."""
         n = int(self._L.strix_cuda_attn_pages_workspace(self._h, cache, batch, n_heads))
         if n == 0:
             msg = self._L.strix_cuda_last_error(self._h).decode()

@@ -893,6 +893,7 @@ static int attn_form(const PagedView &V, uint32_t group, uint32_t &wm) {
 
 static uint32_t form_rows(int form, uint32_t wm) { return form == FORM_ROWS ? 128u : form == FORM_WIDE ? 16u * wm : 8u; }  // of a block
 
+// What a call of these sizes needs.
 static size_t attn_work_bytes(const strix_cuda *h, const PagedView &V, uint32_t group) {
     uint32_t wm;
     const int form = attn_form(V, group, wm);
@@ -974,6 +975,7 @@ extern "C" size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_
     h->err.clear();
     PagedView V;
     if (attn_check(h, "attn_pages_workspace", cache, batch, n_heads, V) != 1) return 0;
+    V.n_seq = 1;  // all rows in one sequence: the form with the most rows to a block that so many rows can take
     return attn_work_bytes(h, V, n_heads / V.n_kv);
 }
 

@@ -742,6 +742,29 @@ def test_attention_on_two_streams_at_once(torch, pkg, accel):
     assert accel.device_status() == 0 and all(torch.equal(j[4], a) for j, a in zip(jobs, alone))
 
 
+@pytest.mark.parametrize("hd,group,rows", [(64, 1, 64), (128, 4, 64), (128, 4, 3), (128, 8, 2), (128, 2, 5), (96, 4, 64), (192, 2, 40), (256, 3, 64), (64, 16, 1)])
+def test_attention_workspace_of_the_most_rows_serves_all(torch, pkg, accel, hd, group, rows):
+    """A workspace for a decode batch of `rows` sequences serves the same rows, or fewer, in fewer sequences: others finish, a prompt
+    comes."""
+    page, n_kv = 32, 2
+    lengths = [30 + rows] * rows
+    P = Paged(torch, pkg, pkg.KV_E4M3, n_kv, page, hd, lengths)
+    P.seed_random(1, lengths)
+    w = work_of(torch, accel, P, P.batch(list(range(rows + 1)), [30] * rows), n_kv * group)
+    q = torch.randn(rows, n_kv * group * hd, device="cuda")
+    shapes = {(1, rows), (1, max(1, rows // 4)), (max(1, rows // 16), rows), (max(1, rows // 5), rows), (rows, rows), (max(1, rows // 2), rows)}
+    for n_seq, n_rows in sorted(shapes):
+        row0 = [n_rows * i // n_seq for i in range(n_seq + 1)]
+        b = P.batch(row0, [30] * n_seq)
+        assert accel.attn_pages_workspace(P.desc, b, n_kv * group) <= w.numel()
+        out = torch.zeros(n_rows, n_kv * group * hd, device="cuda")
+        assert accel.attn_pages_dev(P.desc, b, n_kv * group, q.data_ptr(), out.data_ptr(), 0.125, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        assert accel.device_status() == 0
+        if n_seq <= 4:
+            check_attention(torch, accel, P, b, row0, [30] * n_seq, n_kv * group, q[:n_rows], out, 0.125, 0)
+
+
 def test_serving_calls_refuse(torch, pkg, accel):
     """Wrong arguments are errors with a message, other shapes are declined; nothing is launched."""
     P = Paged(torch, pkg, pkg.KV_F16, 2, 16, 64, [32])
