@@ -49,9 +49,10 @@ typedef struct strix_kv_pages {
  * positions d_ctx[s], d_ctx[s] + 1, ... behind the d_ctx[s] tokens that are cached already. Position t lives in slot
  * t % page_tokens of page d_pages[s * pages_ld + t / page_tokens]. d_ctx[s] < 0 marks an idle slot of a padded batch: its
  * rows enter no cache and get zeros from the attention. Rows from d_row0[n_seq] on belong to nobody and are left alone.
- * Bad device data: offsets are clamped into [0, n_rows] and taken as ascending (a sequence whose end lies before its
- * start has no rows); positions at or beyond pages_ld * page_tokens and pages with an id outside [0, n_pages) are neither
- * written nor attended to. Each sets the status bit. */
+ * Bad device data: offsets are clamped into [0, n_rows], and a sequence whose end lies before its start has no rows (where
+ * offsets go down, two sequences may own a row: which of them the operators take it for, one, both or none, is unspecified);
+ * positions at or beyond pages_ld * page_tokens and pages with an id outside [0, n_pages) are neither written nor attended to.
+ * Each sets the status bit. */
 typedef struct strix_kv_batch {
     const int32_t *d_row0;  /* [n_seq + 1] */
     const int32_t *d_ctx;   /* [n_seq] */

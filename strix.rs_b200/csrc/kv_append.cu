@@ -380,7 +380,13 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
         }
         row += cnt;
     }
-    report_bad(V, bad && threadIdx.x == 0);
+    // offsets out of range or going down, whether or not a row leads to them: each sequence is looked at by one thread of the grid
+#pragma unroll 1
+    for (uint32_t s = blockIdx.x * (WARPS * 32u) + threadIdx.x; s < V.n_seq; s += A.kv_blocks * (WARPS * 32u)) {
+        uint32_t first, end;
+        seq_rows(V, s, first, end, bad);
+    }
+    report_bad(V, bad);
 }
 
 template <int HD, int TYPE>

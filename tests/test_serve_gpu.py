@@ -273,6 +273,38 @@ def test_append_bad_device_data_is_skipped(torch, pkg, accel):
         assert (v == want).all()
 
 
+def test_append_bad_offsets_that_no_row_leads_to(torch, pkg, accel):
+    """Offsets beyond the rows, below zero, going down: the status bit is set whether or not a row lies in such a sequence, rows go
+    to the sequences that attention gives them to, and where offsets go down nothing enters but at its place in a sequence that owns it."""
+    hd, page = 64, 16
+    prep = pkg.KvPrep(rope=pkg.ROPE_NONE)
+    for row0, n_rows, whole in (([0, 4, 9], 4, True), ([-3, 0, 4], 4, True), ([0, 5, 3, 8], 8, False), ([0, 5, 3, 8], 10, False), ([0, 9, 2, 3], 60, False),
+                                ([0, 1 << 30], 3, True), ([0, 40, 41, -1], 41, True)):
+        for many in (False, True):       # a row to a block, a page to a block
+            n_seq = len(row0) - 1
+            n = n_rows if not many else max(n_rows, 8 * n_seq + 1)
+            if many and n != n_rows and max(row0) > n_rows:
+                continue                 # (more rows would change what is out of range)
+            P = Paged(torch, pkg, pkg.KV_F16, 1, page, hd, [64] * n_seq, fill=0)
+            x = (torch.arange(n, device="cuda").float() + 1)[:, None].expand(n, hd).contiguous()
+            b = P.batch(row0, [3] * n_seq, n)
+            q = torch.zeros_like(x)
+            assert accel.kv_append_dev(P.desc, b, x.data_ptr(), x.data_ptr(), prep, n_heads=1, d_q=x.data_ptr(), d_q_out=q.data_ptr(), stream=stream(torch))
+            torch.cuda.synchronize()
+            assert accel.device_status() == 2, (row0, n)
+            accel.clear_device_status()
+            got = np.stack([P.tokens(m, s, 64)[:, 0] for m in "kv" for s in range(n_seq)]).reshape(2, n_seq, 64, hd)
+            assert (got[0] == got[1]).all()
+            clamp = lambda o: min(max(o, 0), n)  # noqa: E731
+            for s in range(n_seq):
+                for t in range(64):
+                    r = clamp(row0[s]) + t - 3
+                    owns = t >= 3 and r < clamp(row0[s + 1])
+                    assert (got[0, s, t] == got[0, s, t, 0]).all() and got[0, s, t, 0] in ([r + 1.0] if owns and whole else [0.0, r + 1.0] if owns else [0.0])
+            hq = q.cpu().numpy()
+            assert (((hq == 0) | (hq == x.cpu().numpy())).all())
+
+
 def test_bad_device_data_stays_with_the_serving_calls(torch, pkg, accel, orc, synth):
     """What a bad page id sets is there to be read and cleared, and no other call takes it for a failure of its own."""
     w, x = synth.q8_0(71, "status", 64, 512), synth.normal(71, "status.x", 512)
