@@ -153,8 +153,9 @@ struct SampleRow {
         split(y, hi, lo);
         return ((u64)hi << 20) + lo;
     }
-    // place in the histogram, a number below SAMPLE_BINS where there is weight
-    __device__ float bin_of(float x) const { return (m - x) * cb; }
+    // place in the histogram, a number below SAMPLE_BINS where there is weight (the product is rounded by itself: whoever asks for a
+    // token's bin, or subtracts from this, gets the same number)
+    __device__ float bin_of(float x) const { return __fmul_rn(m - x, cb); }
     __device__ static uint32_t bin(float b) { return __float_as_uint(__fadd_rd(b, 8388608.f)) & 0x7fffffu; }
 
     // folds up to two values over the cluster

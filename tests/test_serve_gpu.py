@@ -898,6 +898,38 @@ def test_sample_many_rows(torch, accel, rows, n):
     check_sample(x, u, ids, probs, T, K, TP, MP)
 
 
+def test_sample_cuts_among_very_many_tokens(torch, accel):
+    """Flat rows, where a top-p cut falls among tens of thousands of tokens of nearly equal weight, most of them beside the border of
+    some bin. The drawn token has its place at u: its kept weights, in index order, pass u of the whole there, to within the rounding of
+    the sums (2^-20 of the whole: f32 sums of up to 128 weights, whose exponents are off by 2^-21) and two tokens that the border
+    may take in or leave out."""
+    rng = np.random.RandomState(7)
+    for n, spread in ((151936, 0.02), (151936, 0.5), (40001, 0.3), (262147, 1.0)):
+        rows = 24
+        x = (rng.randn(rows, n) * spread).astype(np.float32)
+        x[::2] = np.round(x[::2] * 4096) / 4096
+        u, T, TP = rng.rand(rows).astype(np.float32), rng.choice([0.5, 1.0, 3.0], rows), rng.choice([0.3, 0.62, 0.9, 0.99], rows)
+        K = rng.choice([0, n // 2], rows)
+        ids, probs = sample(torch, accel, x, u, temperature=T, top_p=TP, top_k=K)
+        for r in range(rows):
+            order = np.argsort(-x[r].astype(np.float64), kind="stable")
+            order = order[:K[r]] if K[r] else order
+            w = np.exp((x[r][order].astype(np.float64) - x[r].max()) / float(np.float32(T[r])))
+            before = np.cumsum(w) - w
+            kept = before < float(np.float32(TP[r])) * w.sum()
+            full = np.zeros(n)
+            full[order[kept]] = w[kept]
+            total, border = full.sum(), w[kept][-1]
+            eps = 2.0 ** -20 * total + 2 * border
+            near = np.zeros(n, bool)
+            near[order[max(0, int(kept.sum()) - 2):int(kept.sum()) + 2]] = True
+            i, upto = int(ids[r]), np.cumsum(full)
+            assert full[i] > 0 or near[i]
+            assert upto[i] - full[i] - eps <= float(u[r]) * total <= upto[i] + eps, (r, i, upto[i] / total, u[r])
+            weight = np.exp((float(x[r, i]) - x[r].max()) / float(np.float32(T[r])))
+            assert abs(probs[r] - weight / total) <= (2.0 ** -17 + 2 * border / total) * weight / total
+
+
 def test_sample_ties(torch, accel):
     """Logits from a few values only (whole rows of ties): top-k and top-p cut inside the ties, lower indices first."""
     rng = np.random.RandomState(1)
