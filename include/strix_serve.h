@@ -95,7 +95,7 @@ STRIX_API int strix_cuda_kv_append_dev(strix_cuda *h, const strix_kv_pages *cach
  * KV head. */
 STRIX_API size_t strix_cuda_attn_pages_workspace(strix_cuda *h, const strix_kv_pages *cache, const strix_kv_batch *batch, uint32_t n_heads);
 /* out[row][head] = softmax(scale * q k^T) v over the cached tokens the row sees: positions 0 .. its own (its own k and v
- * are in the cache by then), with window > 0 only the last `window` of them. n_heads is a multiple of n_kv; head h reads KV
+ * are in the cache by then), with window > 0 only the last `window` of them. scale is finite. n_heads is a multiple of n_kv; head h reads KV
  * head h / (n_heads / n_kv). q and out: [n_rows][n_heads * head_dim] f32, ld_q / ld_out floats between rows (0 = packed), which
  * must not overlap. With a window, pages that end before all rows' windows are not looked at: they may be given away.
  * A row that sees no token gets zeros. Offsets that give away more rows than n_rows (possible where they go down) set the status

@@ -993,6 +993,7 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     A.ld_q = ld_q ? ld_q : qd;
     A.ld_out = ld_out ? ld_out : qd;
     if (A.ld_q < qd || A.ld_out < qd) return serve_fail(h, who, "a row stride is smaller than a row");
+    if (!isfinite(scale)) return serve_fail(h, who, "scale must be finite");
     if (A.V.n_seq == 0 || A.V.n_rows == 0) return 1;
     if (!d_q || !d_out) return serve_fail(h, who, "d_q or d_out missing");
     if (d_q == d_out) return serve_fail(h, who, "d_out must not be d_q: rows are read by several blocks");

@@ -774,6 +774,20 @@ def test_attention_on_two_streams_at_once(torch, pkg, accel):
     assert accel.device_status() == 0 and all(torch.equal(j[4], a) for j, a in zip(jobs, alone))
 
 
+def test_attention_refuses_a_scale_that_is_no_number(torch, pkg, accel):
+    P = Paged(torch, pkg, pkg.KV_F16, 1, 16, 64, [64])
+    for new in (1, 40):       # (few rows, many rows)
+        b = P.batch([0, new], [10])
+        q = torch.zeros(new, 64, device="cuda")
+        out = torch.full_like(q, 5.0)
+        w = work_of(torch, accel, P, b, 1)
+        for scale in (float("nan"), float("inf"), -float("inf")):
+            with pytest.raises(pkg.StrixCudaError):
+                accel.attn_pages_dev(P.desc, b, 1, q.data_ptr(), out.data_ptr(), scale, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        assert (out == 5.0).all()
+
+
 @pytest.mark.parametrize("hd,group,rows", [(64, 1, 64), (128, 4, 64), (128, 4, 3), (128, 8, 2), (128, 2, 5), (96, 4, 64), (192, 2, 40), (256, 3, 64), (64, 16, 1)])
 def test_attention_workspace_of_the_most_rows_serves_all(torch, pkg, accel, hd, group, rows):
     """A workspace for a decode batch of `rows` sequences serves the same rows, or fewer, in fewer sequences: others finish, a prompt
