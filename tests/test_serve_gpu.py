@@ -788,6 +788,16 @@ def test_attention_refuses_a_scale_that_is_no_number(torch, pkg, accel):
         assert (out == 5.0).all()
 
 
+@pytest.mark.parametrize("hd", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("group,rows", [(4, 3), (16, 1), (2, 8), (4, 8), (3, 21)])
+def test_attention_nine_and_more_rows_of_a_head(torch, pkg, accel, kv, hd, group, rows):
+    """Sixteen rows a warp, and from seventeen on several warps to a worker (head sizes 96, 192, 256) or row blocks: every head size, both
+    cache types, contexts long enough to be shared between blocks, other sequences beside, strides that are no multiple of four."""
+    run_attention(torch, pkg, accel, kv, 2, group, 32, hd, [rows, rows, rows], [700, 45, 16], fill=0xff, ldpad=0 if rows == 8 else 1)
+    run_attention(torch, pkg, accel, kv, 1, group, 16 if hd > 128 else 64, hd, [rows, rows], [1200, -1], window=90)
+
+
 @pytest.mark.parametrize("hd,group,rows", [(64, 1, 64), (128, 4, 64), (128, 4, 3), (128, 8, 2), (128, 2, 5), (96, 4, 64), (192, 2, 40), (256, 3, 64), (64, 16, 1)])
 def test_attention_workspace_of_the_most_rows_serves_all(torch, pkg, accel, hd, group, rows):
     """A workspace for a decode batch of `rows` sequences serves the same rows, or fewer, in fewer sequences: others finish, a prompt
