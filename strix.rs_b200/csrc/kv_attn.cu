@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
                     const int ex = (int)(__float_as_uint(top) >> 23);
                     const int e2 = top > 0.f && ex < 255 ? min(126, max(-126, 14 + 127 - max(ex, 1))) : 0;
                     const float up = __uint_as_float((uint32_t)(e2 + 127) << 23);
-                    qc[i] = A.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e2) << 23);
+                    qc[i] = A.scale * (1.4426950408889634f * __uint_as_float((uint32_t)(127 - e2) << 23));
 #pragma unroll
                     for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -1007,9 +1007,7 @@ extern "C" int strix_cuda_attn_pages_dev(strix_cuda *h, const strix_kv_pages *ca
     A.window = window;
     A.cap = A.V.pages_ld * A.V.page_tokens;
     A.scale = scale;
-    int scale_e = 0;
-    A.scale_m = (float)frexp((double)scale * 1.4426950408889634, &scale_e);
-    A.scale_p = ldexpf(1.f, scale_e);
+    A.scale_m = (float)frexp((double)scale * 1.4426950408889634, &A.scale_e);
     A.vec = ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15u) == 0 && ((A.ld_q | A.ld_out) & 3u) == 0;
     A.ticket = static_cast<uint32_t *>(d_work);
     A.part = reinterpret_cast<float *>(static_cast<uint8_t *>(d_work) + PA_MAX_BLOCKS * 4);

@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(RA_THREADS, 1) attn_rows_kernel(const __grid_c
                 const int ex = (int)(__float_as_uint(top) >> 23);
                 const int e2 = top > 0.f && ex < 255 ? min(126, max(-126, 14 + 127 - max(ex, 1))) : 0;
                 const float up = A.scale_m * __uint_as_float((uint32_t)(e2 + 127) << 23);
-                q_factor[(items % RA_QBUF) * 128u + tid] = A.scale_p * __uint_as_float((uint32_t)(127 - e2) << 23);
+                q_factor[(items % RA_QBUF) * 128u + tid] = __uint_as_float((uint32_t)(min(127, max(-126, A.scale_e - e2)) + 127) << 23);
 #pragma unroll 4
                 for (int i = 0; i < HD; i += 8) {
                     const float4 x = load4(i), y = load4(i + 4);

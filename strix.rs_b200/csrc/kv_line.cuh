@@ -22,8 +22,8 @@ struct PagedAttnArgs {
     size_t ld_q, ld_out;
     uint32_t group, window, cap;  // cap: tokens a row of the page table can hold
     uint32_t g_mul, g_shift;               // division by group
-    float scale;
-    float scale_m, scale_p;                // scale log2(e) = scale_m (of magnitude [1/2, 1), or 0) times a power of two (row blocks)
+    float scale, scale_m;
+    int scale_e;               // row blocks: scale log2(e) = scale_m (of magnitude [1/2, 1), or 0) times 2^scale_e
     uint32_t wm, halves, vec;  // warps of a worker; half tiles of a ring; q and out rows start on 16 bytes
     uint32_t *ticket;          // [PA_MAX_BLOCKS]
     float *part;               // [blocks][2][rows of a worker][HD + 2]

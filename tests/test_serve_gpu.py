@@ -774,6 +774,18 @@ def test_attention_on_two_streams_at_once(torch, pkg, accel):
     assert accel.device_status() == 0 and all(torch.equal(j[4], a) for j, a in zip(jobs, alone))
 
 
+@pytest.mark.parametrize("kv,hd,new", [(0, 64, 1), (1, 128, 3), (1, 256, 4), (0, 64, 6), (1, 128, 9)])
+def test_attention_largest_and_smallest_scales(torch, pkg, accel, kv, hd, new):
+    """A scale near the ends of f32 with queries that make up for it gives what 1 gives: neither overflows on the way."""
+    P, b, row0, q, out, w = run_attention(torch, pkg, accel, kv, 1, 4, 32, hd, [new], [90])
+    for scale, qs in ((-3.0e38, -1.0e-38 / 3), (3.0e38, 1.0e-36 / 3), (1.0e-38, 1.0e37), (1.0e-39, 5.0e37)):
+        x = q * qs
+        assert accel.attn_pages_dev(P.desc, b, 4, x.data_ptr(), out.data_ptr(), scale, w.data_ptr(), w.numel(), stream=stream(torch))
+        torch.cuda.synchronize()
+        want = torch.from_numpy(x.cpu().numpy().astype(np.float64) * float(np.float32(scale)))       # (the scale in the query, then 1)
+        check_attention(torch, accel, P, b, row0, [90], 4, want, out, 1.0, 0)
+
+
 def test_attention_refuses_a_scale_that_is_no_number(torch, pkg, accel):
     P = Paged(torch, pkg, pkg.KV_F16, 1, 16, 64, [64])
     for new in (1, 40):       # (few rows, many rows)
