@@ -748,6 +748,36 @@ def test_attention_offsets_that_go_down(torch, pkg, accel):
         check_attention(torch, accel, P, b, [0, new - 1], [5], 2, q, out, 0.125, 0)
 
 
+def test_prompts_and_single_tokens_in_two_calls(torch, pkg, accel):
+    """A batch whose single tokens come first, as one call and as two over the same arrays (the second from the first prompt on): the
+    same cache bit by bit, the same queries, and attention that agrees with 64 bits either way."""
+    hd, page, n_kv, heads, n = 128, 32, 2, 8, 9
+    new, ctx = [1] * n + [70, 40], [5, 33, 0, 64, 31, -1, 100, 95, 7] + [0, 50]
+    row0 = np.cumsum([0] + new).tolist()
+    for kv in (pkg.KV_F16, pkg.KV_E4M3):
+        caches = []
+        for split in (False, True):
+            P = Paged(torch, pkg, kv, n_kv, page, hd, [c + m if c >= 0 else 0 for c, m in zip(ctx, new)], seed=3, fill=0)
+            P.seed_random(4, [max(c, 0) for c in ctx])
+            b = P.batch(row0, ctx)
+            parts = [b] if not split else [
+                pkg.KvBatch(n, n, P.row0.data_ptr(), P.ctx.data_ptr(), P.d_table.data_ptr(), P.ld),
+                pkg.KvBatch(2, row0[-1], P.row0.data_ptr() + 4 * n, P.ctx.data_ptr() + 4 * n, P.d_table.data_ptr() + 4 * n * P.ld, P.ld)]
+            g = torch.Generator(device="cuda").manual_seed(1)
+            q, k, v = (torch.randn(row0[-1], h * hd, generator=g, device="cuda") for h in (heads, n_kv, n_kv))
+            out = torch.full_like(q, 5.0)
+            w = work_of(torch, accel, P, b, heads)
+            for part in parts:
+                assert accel.kv_append_dev(P.desc, part, k.data_ptr(), v.data_ptr(), pkg.KvPrep(theta=1e4), n_heads=heads, d_q=q.data_ptr(), d_q_out=q.data_ptr(),
+                                           stream=stream(torch))
+                assert accel.attn_pages_dev(P.desc, part, heads, q.data_ptr(), out.data_ptr(), 0.09, w.data_ptr(), w.numel(), stream=stream(torch))
+            torch.cuda.synchronize()
+            assert accel.device_status() == 0
+            check_attention(torch, accel, P, b, row0, ctx, heads, q, out, 0.09, 0)
+            caches.append([P.raw[m] for m in "kv"] + [P.scale[m] for m in "kv"] + [q])
+        assert all(torch.equal(a, z) for a, z in zip(*caches))
+
+
 def test_attention_on_two_streams_at_once(torch, pkg, accel):
     """Calls that run at the same time, each with its own workspace, give what they give alone, bit by bit."""
     jobs = []
