@@ -5,6 +5,7 @@
     python profile_case.py attn <context> [steps]
     python profile_case.py chain <layers> [tokens]
     python profile_case.py multi <act 0|1> [launches]
+    python profile_case.py pages <context> <new rows> <f16 0|1> [launches]
 
 `multi`: the four small weights of the benchmark step (Q8_0 and Q6_K, 2560 -> 9728 and 9728 -> 2560) as one
 gemv_batch_dev call, i.e. side by side in one launch (``-k regex:gemv_multi_kernel``).
@@ -14,6 +15,9 @@ gemv_batch_dev call, i.e. side by side in one launch (``-k regex:gemv_multi_kern
 
 `attn`: a two-layer model with the benchmark's attention geometry (32 query heads, 8 KV heads of 128,
 hidden 2560) and a KV cache seeded up to <context>; runs decode_step at that position (``-k regex:sdpa_split``).
+
+`pages`: attn_pages_dev for one sequence of <new rows> rows behind <context> tokens, 32 query heads, 8 KV heads of 128, 64-token pages,
+e4m3 or f16 (``-k regex:attn_rows_kernel``, or ``paged_attn_kernel`` for up to four rows).
 
 Uploads one seeded synthetic weight through the C ABI and launches the device-resident entry
 point a few times on cuda:0. Run it plain first, then under ncu with ``-k regex:gemv_kernel``
@@ -108,6 +112,23 @@ def main():
         h0 = synth.normal(1, "h0", hidden)
         for _ in range(reps):
             y = torch.from_numpy(acc.decode_step(h0, ctx))
+    elif kind == "pages":
+        ctx, new, f16 = (int(a) for a in sys.argv[2:5])
+        reps = int(sys.argv[5]) if len(sys.argv) > 5 else 3
+        heads, n_kv, hd, page, n_pages = 32, 8, 128, 64, (ctx + new + 63) // 64
+        k, v = (torch.randn(n_pages, n_kv, page, hd, device=dev) for _ in "kv")
+        k, v = (t.half() if f16 else (t * 64).to(torch.float8_e4m3fn) for t in (k, v))
+        scale = torch.full((n_pages, n_kv), 2.0 ** -6, device=dev)
+        row0, before = (torch.tensor(a, dtype=torch.int32, device=dev) for a in ([0, new], [ctx]))
+        table = torch.randperm(n_pages, device=dev).int()
+        cache = pkg.KvPages(k.data_ptr(), v.data_ptr(), n_pages, n_kv, page, hd, type=pkg.KV_F16 if f16 else pkg.KV_E4M3, d_k_scale=scale.data_ptr(),
+                            d_v_scale=scale.data_ptr())
+        batch = pkg.KvBatch(1, new, row0.data_ptr(), before.data_ptr(), table.data_ptr(), n_pages)
+        work = torch.zeros(acc.attn_pages_workspace(cache, batch, heads), dtype=torch.uint8, device=dev)
+        q = torch.randn(new, heads, hd, device=dev) * 1.5
+        y = torch.zeros_like(q)
+        for _ in range(reps):
+            assert acc.attn_pages_dev(cache, batch, heads, q.data_ptr(), y.data_ptr(), hd ** -0.5, work.data_ptr(), work.numel(), stream=s)
     else:
         m, k, n = (int(a) for a in sys.argv[2:5])
         reps = int(sys.argv[5]) if len(sys.argv) > 5 else 3
