@@ -49,6 +49,9 @@ typedef struct strix_kv_pages {
  * positions d_ctx[s], d_ctx[s] + 1, ... behind the d_ctx[s] tokens that are cached already. Position t lives in slot
  * t % page_tokens of page d_pages[s * pages_ld + t / page_tokens]. d_ctx[s] < 0 marks an idle slot of a padded batch: its
  * rows enter no cache and get zeros from the attention. Rows from d_row0[n_seq] on belong to nobody and are left alone.
+ * Both operators choose one form of their kernel for a call, by n_rows / n_seq. Where prompts and single tokens come together, put the
+ * single tokens first and make two calls, one with the n sequences and rows of these, one with d_row0 + n, d_ctx + n,
+ * d_pages + n * pages_ld, the other sequences and all n_rows: that is several times as fast.
  * Bad device data: offsets are clamped into [0, n_rows], and a sequence whose end lies before its start has no rows (where
  * offsets go down, two sequences may own a row: which of them the operators take it for, one, both or none, is unspecified);
  * positions at or beyond pages_ld * page_tokens and pages with an id outside [0, n_pages) are neither written nor attended to.
@@ -127,7 +130,8 @@ typedef struct strix_sample_params {
  *   d_ids[row] = the least i whose kept weights up to and including i exceed d_u[row] * (sum of kept weights), d_u in [0, 1)
  * Equal logits rank by index, lower first; NaN counts as -inf; with +inf among the logits only those have weight.
  * A row without any logit above -inf gives id 0 and probability 0. d_probs (may be NULL): the drawn token's weight over the kept
- * sum. Weights are summed as 64-bit integers (in steps of 2^-40; the sum of a whole row in f32 over stretches of fixed
+ * sum. A weight is off by about 2^-22 (1 + |x_i - max x| / temperature) of itself (f32 exponent); min_p and top_p
+ * cut to that accuracy. Weights are summed as 64-bit integers (in steps of 2^-40; the sum of a whole row in f32 over stretches of fixed
  * order), so the same logits and the same u draw the same token every time.
  * The greedy choice is that of strix_cuda_argmax_dev except below its floor of -3.0e38. */
 #define STRIX_SAMPLE_MAX_N 393216

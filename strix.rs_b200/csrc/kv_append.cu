@@ -3,7 +3,8 @@
 //
 // What bounds it: a prompt is HBM traffic (4 bytes read for every element of q, k, v, 4 written for q, 1 or 2 for k and v);
 // a decode step is one launch and a chain of four dependent loads (row0, ctx, page id, old scale).
-// Measured (32 + 2 x 8 heads of 128): prompts of 8064 rows in all 84 us (4.1 TB/s), 64 rows into f16 5.8 us, one row 3.4 us.
+// Measured (32 + 2 x 8 heads of 128): prompts of 8064 rows in all 85 us into e4m3 (4.1 TB/s), 78 into f16; 64 rows into f16 (16 + 2 x 8
+// heads of 256) 5.9 us, one row 3.6 us.
 //
 // Work split. The cache side goes by pages, because a page and head share one scale: a block takes one (page, head) of k
 // or v (four heads of it in turn, where sequences bring many rows), holds its new rows in registers, reduces their largest
@@ -518,6 +519,13 @@ extern "C" int strix_cuda_kv_append_dev(strix_cuda *h, const strix_kv_pages *cac
               reinterpret_cast<uintptr_t>(d_q_out)) & 15u) == 0 &&
             ((A.ld_k | A.ld_v | (d_q ? A.ld_q | A.ld_qo : 0)) & 3u) == 0;
     const uint64_t n_rows = A.V.n_rows;
+    // A unit of a page's rows, or of one row, by the rows that a sequence brings on average. Both measured (us, a page's and a row's, f16 and
+    // e4m3, 64-token pages, 32 + 2 x 8 heads of 128):
+    //   64 sequences of 1 row 269 and 5.7, 375 and 7.0; of 4: 74 and 13, 102 and 14; of 8: 41 and 22, 55 and 23; of 12: 33 and 32, 45 and 32;
+    //   of 16: 28 and 41, 39 and 41; of 64: 50 and 157, 58 and 161.  8 sequences of 8: 35 and 4.9, 48 and 5.3; of 32: 20 and 11, 27 and 13;
+    //   of 64: 14 and 20, 18 and 23.  1 of 16: 6.9 and 3.7, 8.5 and 4.3; of 256: 14 and 11, 18 and 15; of 2048: 22 and 63, 23 and 66.
+    // So with few sequences a row's unit would still be the better one for some hundred rows. One form serves a call: 512 rows of a prompt
+    // beside 60 single rows, whose pages then fall to one unit, take 361 us, in two calls 18.5.
     const bool by_page = n_rows > 8ull * A.V.n_seq;
     A.unit_rows = by_page ? A.V.page_tokens : 1u;
     A.kv_group = by_page ? 4u : 1u;

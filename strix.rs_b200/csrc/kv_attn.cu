@@ -27,10 +27,11 @@
 // the last block to arrive joins the parts, in the order of the line. Cuts that would fall into an item of at most PA_SNAP
 // tiles move to its nearer end.
 //
-// Measured (32 heads, 8 KV heads of 128, e4m3): one row behind 131071 tokens 72 us (3.7 TB/s), 61 rows behind 500-16384 each
-// 138 us (4.2 TB/s), one row behind 300 tokens 13.2 us. About 8 us of a call are its two ends (the place in the line, page ids and
-// scales, q; the joins); in between, instruction issue bounds: some 1000 instructions a tile, of which the fragments of k and v,
-// their conversion and the two halves' products are two thirds.
+// Measured (32 heads, 8 KV heads of 128, e4m3): one row behind 131071 tokens 74 us (3.6 TB/s), 61 rows behind 500-16384 each
+// 138 us (4.2 TB/s), one row behind 300 tokens 13.5 us. About 8 us of a call are its two ends (the place in the line, page ids and
+// scales, q; the joins where items are shared); in between, instruction issue bounds: some 1000 instructions a tile, of which the
+// fragments of k and v, their conversion and the two halves' products are two thirds. With four query heads to a KV head half of the
+// sixteen rows of every product are empty, and a tile is 32 tokens (head size 128, e4m3), so what a tile costs besides is paid often.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -868,10 +869,12 @@ __global__ void __launch_bounds__(PaShape<HD, TYPE, WIDE>::NW * 32, 1) paged_att
 
 // Above this many rows a head on average, blocks of 128 rows on tcgen05 (kv_attn_rows.cu). Both forms measured, 8 KV heads of 128,
 // 64-token pages, us with such blocks and without, f16 and e4m3:
-//   12 rows, 64 sequences of 4000 tokens: 301 and 263, 328 and 217
-//   16 rows,  8 of 3000:  51 and  44,  54 and  41;  32 of 8000: 290 and  262, 312 and 214;  1 of 30000: 62 and 54, 64 and 50
-//   20 rows,  8 of 3000:  54 and  72,  57 and  61;  32 of 8000: 295 and  548, 317 and 423;  1 of 30000: 67 and 92, 71 and 77
-//   64 rows,  8 of 3000:  71 and 131,  67 and 109;  32 of 8000: 314 and 1077, 332 and 816
+//   12 rows, 64 sequences of 4000 tokens: 283 and 259, 336 and 214
+//   16 rows,  8 of 3000:  49 and  45,  54 and  42;  32 of 8000: 275 and  258, 331 and 212;  1 of 30000: 61 and 56, 65 and 51
+//   20 rows,  8 of 3000:  52 and  71,  57 and  61;  32 of 8000: 280 and  532, 321 and 411;  1 of 30000: 66 and 92, 71 and 76
+//   64 rows,  8 of 3000:  70 and 130,  67 and 107;  32 of 8000: 307 and 1050, 368 and 805
+// One form serves a call, so a batch of very uneven sequences gets the wrong one for some of them: 512 rows beside 60 single tokens
+// behind 4000 each take 1139 us, in two calls 189 (150 rows: 403 and 186).
 constexpr uint64_t ROWS_FROM = 16;
 
 // Blocks that the launch may have: one on each SM.

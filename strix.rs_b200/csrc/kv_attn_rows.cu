@@ -23,7 +23,8 @@
 // of that, at half of the issue slots. Loops over tiles stay rolled, because instruction fetch bounded the unrolled form (135 KB,
 // all roles at once: 460 us, 320 once rolled, in earlier forms). S held in registers, so that its columns are free sooner, was
 // no faster (201 against 197 us). 512 rows behind 8000 tokens (32 heads, 8 KV heads of 128, e4m3): 197 us, 352 TFLOP/s
-// of useful products, as many again for the second halves; 8 x 5 rows behind 1000-5000 tokens, f16: 55 us.
+// of useful products, as many again for the second halves (220 us with 16-token pages, whose scales meet the weights row by
+// row); 8 x 5 rows behind 1000-5000 tokens, f16: 55 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

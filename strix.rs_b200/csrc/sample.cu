@@ -20,8 +20,10 @@
 // Weights are summed as 64-bit integers in steps of 2^-40 (the sum over all as f32 within a thread's stretch, whose order is
 // fixed), so no sum depends on the order of atomics, and neither does the draw.
 //
-// Measured: one row of 151936 13.6 us, 64 of them with mixed parameters 55 us, 16 rows of 262147 with top-p over most of their mass
-// 44 us. 33 clusters of eight such blocks run at a time, so 64 rows go in two waves.
+// Measured: one row of 151936 12.8-18 us, 64 of them with mixed parameters 44-62 us, 16 rows of 262147 with top-p over most of their mass
+// 30-60 us, depending on where the cuts fall (three inputs each). 33 clusters of eight such blocks run at a time, so 64 rows go in two waves.
+//
+// A weight is ex2 of an f32 exponent, so it is off by about 2^-22 (1 + |x - max| / T) of itself.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -950,7 +952,9 @@ static cudaError_t sample_launch(strix_cuda *h, const SampleArgs &A, uint32_t ro
 }
 
 // A row takes as many blocks as make it 4096 logits or fewer to a block, at most 8: more blocks shorten every pass, a barrier among
-// them costs the same (4 instead of 8 for 151936 logits: 18.7 against 15.8 us a row, 80 against 69 for 64, in an earlier form).
+// them costs the same, but fewer rows run at once. Measured, us with up to 8 and up to 4 blocks for 151936 logits: one row 12.5 and 15.4,
+// 16 nucleus rows 47 and 52, 64 mixed rows 57 and 54. With 4096 and with 8192 to a block: 64 mixed rows of 20000 logits 25 and 13, one
+// row 9.2 and 9.0; of 5000 logits 9.9 and 8.3, 8.0 and 6.8. (2048 to a block: 25, 9.2, 11.6, 8.1.)
 cudaError_t launch_sample(strix_cuda *h, const float *d_x, uint32_t n, size_t stride, uint32_t rows, const strix_sample_params &p,
                           const float *d_u, uint32_t *d_ids, float *d_probs, cudaStream_t stream) {
     uint32_t c = 1;
