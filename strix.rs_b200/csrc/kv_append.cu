@@ -383,9 +383,9 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_kernel(const AppendArgs 
     }
     // offsets out of range or going down, whether or not a row leads to them: each sequence is looked at by one thread of the grid
 #pragma unroll 1
-    for (uint32_t s = blockIdx.x * (WARPS * 32u) + threadIdx.x; s < V.n_seq; s += A.kv_blocks * (WARPS * 32u)) {
+    for (uint64_t s = (uint64_t)blockIdx.x * (WARPS * 32u) + threadIdx.x; s < V.n_seq; s += (uint64_t)A.kv_blocks * (WARPS * 32u)) {  // (may pass 32 bits)
         uint32_t first, end;
-        seq_rows(V, s, first, end, bad);
+        seq_rows(V, (uint32_t)s, first, end, bad);
     }
     report_bad(V, bad);
 }
